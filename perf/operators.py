@@ -281,7 +281,7 @@ def _adamw_plain(s):
         m = _from_codes(s["exp_avg"], s["exp_avg_scale"])
         v = _from_codes(s["exp_avg_rms"], s["exp_avg_rms_scale"]).square_()
     m.mul_(BETA1).add_(g * (1.0 - BETA1))
-    v.mul_(BETA2).add_(g.mul_(g).mul_(1.0 - BETA2))
+    v.mul_(BETA2).add_((g * g).mul_(1.0 - BETA2))
     root = v.sqrt()
     step = m / (root * (1.0 / math.sqrt(1.0 - BETA2 ** t)) + EPS)
     p = s["master"] if case["master"] else s["param"].float()
