@@ -45,6 +45,7 @@
 #include <mutex>
 #include <vector>
 
+#include "dgnn_internal.h"
 #include "dgnn_spmm.h"
 
 namespace {
@@ -1620,9 +1621,11 @@ int noalloc_scratch(unsigned char** out) {
 size_t round256(size_t b) { return (b + 255) / 256 * 256; }
 }  // namespace
 
+int dgnn_fail(int code, const char* fmt, const char* a, long long b) { return fail(code, fmt, a, b); }
+
 extern "C" {
 
-int dgnn_version(void) { return 280; }   // 280: dgnn_spmm_strip_overwrite_f32; 270: dgnn_strip_plan.ent lines hold the 32 meta words first, then the 32 values; 260: dgnn_strip_plan, dgnn_spmm_strip_f32, dgnn_prof_end_by_kernel, dgnn_set_variant only in -DDGNN_EXPERIMENTS builds; 250: dgnn_dense_plan, dgnn_spmm_dense_f32; 240: dgnn_bundle_plan, dgnn_spmm_bundle_f32; 230: dgnn_plan.hot_rows / hot_cols / seg_hot; 220: dgnn_spmm_coo_noalloc_f32 (210: dgnn_plan.covers_rows, dgnn_spmm_plan_overwrite_f32)
+int dgnn_version(void) { return 290; }   // 290: dgnn_train.h (dgnn_adamw, dgnn_linear_*); 280: dgnn_spmm_strip_overwrite_f32; 270: dgnn_strip_plan.ent lines hold the 32 meta words first, then the 32 values; 260: dgnn_strip_plan, dgnn_spmm_strip_f32, dgnn_prof_end_by_kernel, dgnn_set_variant only in -DDGNN_EXPERIMENTS builds; 250: dgnn_dense_plan, dgnn_spmm_dense_f32; 240: dgnn_bundle_plan, dgnn_spmm_bundle_f32; 230: dgnn_plan.hot_rows / hot_cols / seg_hot; 220: dgnn_spmm_coo_noalloc_f32 (210: dgnn_plan.covers_rows, dgnn_spmm_plan_overwrite_f32)
 
 const char* dgnn_last_error(void) { return g_err; }
 

@@ -90,11 +90,15 @@ _SIGNATURES = {                          # argument types, in the order of inclu
     'dgnn_spmm_strip_overwrite_f32': [ctypes.POINTER(_CStripPlan), _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _i32, _f32, _p],
     'dgnn_spmm_plan_overwrite_f32': [ctypes.POINTER(_CPlan), _p, _p, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _i32, _f32, _p],
 }
-for _name, _args in _SIGNATURES.items():
+_TRAIN_SIGNATURES = {                    # argument types, in the order of include/dgnn_train.h
+    'dgnn_adamw': [_p, _i32, _i32, _i32, _p, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, _p],
+}
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}         # DGNN_F32, DGNN_BF16, DGNN_F16
+for _name, _args in (_SIGNATURES | _TRAIN_SIGNATURES).items():
     getattr(_lib, _name).argtypes = _args
     getattr(_lib, _name).restype = ctypes.c_int
 _lib.dgnn_last_error.restype = ctypes.c_char_p
-_ABI = 280                                # struct layouts and entry points of include/dgnn_spmm.h this stub was written for
+_ABI = 290                                # struct layouts and entry points of include/dgnn_spmm.h this stub was written for
 if _lib.dgnn_version() != _ABI:
     raise RuntimeError(f'spmm_cpp: {os.path.normpath(_LIB_PATH)} is version {_lib.dgnn_version()}, this stub needs {_ABI}: '
                        'rebuild it (python -c "import __graft_entry__ as g; g.build(force=True)")')
@@ -1451,3 +1455,7 @@ def _dense_for(A):
             D = None
         A.__dict__['_dense_plan'] = D
     return A.__dict__['_dense_plan']
+
+
+# --------------------------------------------------------------------------- what a training step computes beside the aggregation
+from .adamw import AdamW  # noqa: E402,F401

@@ -1,0 +1,288 @@
+"""AdamW over many tensors at once (C ABI: dgnn_adamw, include/dgnn_train.h).
+
+The reference's training loop steps ``torch.optim.Adam`` (light_dist_gnn/dist_train.py:32,45), a dozen passes over every
+parameter. Here a step is one pass over parameter, gradient and moments, for up to 64 tensors a launch, with the moments
+in 32 or in 8 bits.
+"""
+import ctypes
+import math
+import operator
+
+import numpy as np
+import torch
+
+from . import _check, _lib, _stream, _DTYPES
+
+_T, _NONE = torch.Tensor, type(None)
+_grad_of, _dtype_of, _layout_of = operator.attrgetter('grad'), operator.attrgetter('dtype'), operator.attrgetter('is_sparse')
+
+BLOCK = 256                       # elements that share a scale; a tensor starts at a multiple of it in the state buffers
+
+_TENSOR = np.dtype([('param', np.uint64), ('grad', np.uint64), ('numel', np.int64), ('start', np.int64), ('decay', np.float32),
+                    ('rate', np.float32), ('root', np.float32), ('turn', np.uint32), ('index', np.int32), ('reserved', np.int32)])
+
+
+class _CState(ctypes.Structure):          # struct dgnn_adamw_state (include/dgnn_train.h)
+    _fields_ = [(n, ctypes.c_void_p) for n in ('exp_avg', 'exp_avg_sq', 'exp_avg_scale', 'exp_avg_sq_scale', 'master',
+                                               'steps', 'factors')]
+
+
+def _kinds(bits, master):
+    """{state name: (type, elements per scale or 1)} of one tensor."""
+    if bits == 32:
+        kinds = {'exp_avg': (torch.float32, 1), 'exp_avg_sq': (torch.float32, 1)}
+    else:
+        kinds = {'exp_avg': (torch.float8_e4m3fn, 1), 'exp_avg_scale': (torch.float32, BLOCK),
+                 'exp_avg_rms': (torch.float8_e4m3fn, 1), 'exp_avg_rms_scale': (torch.float32, BLOCK)}
+    if master:
+        kinds['master'] = (torch.float32, 1)
+    return kinds
+
+
+class _Segment:
+    """The parameters of one group that share a device and a type, and their state: one flat buffer per kind, every tensor's
+    part starting at a multiple of 256 elements. What the kernel's table needs of them and does not change is kept filled."""
+
+    def __init__(self, params, bits, master, capturable):
+        self.params, self.bits, self.has_master, self.capturable = params, bits, master, capturable
+        self.device, self.dtype = params[0].device, params[0].dtype
+        sizes = np.array([p.numel() for p in params], dtype=np.int64)
+        blocks = -(-sizes // BLOCK)
+        self.starts = (np.cumsum(blocks) - blocks) * BLOCK
+        self.size_list, self.where = sizes.tolist(), None
+        self.sizes, total = sizes, int(blocks.sum()) * BLOCK
+        self.kinds = _kinds(bits, master)
+        self.flat = {}
+        for name, (dtype, per) in self.kinds.items():
+            self.flat[name] = torch.zeros(max(total // per, 4), dtype=torch.uint8 if dtype.itemsize == 1 else dtype,
+                                          device=self.device).view(dtype)[:total // per]
+        if capturable:
+            self.steps = torch.zeros(len(params), dtype=torch.int64, device=self.device)
+            self.factors = torch.zeros(len(params), 4, dtype=torch.float32, device=self.device)
+        else:
+            self.host_steps = np.zeros(len(params), dtype=np.int64)
+            self.steps = torch.from_numpy(self.host_steps)
+        self.table = np.zeros(len(params), dtype=_TENSOR)
+        self.table['numel'], self.table['start'] = sizes, self.starts
+        self.table['index'] = np.arange(len(params))
+        st = self.cstate = _CState()
+        f = self.flat
+        st.exp_avg = f['exp_avg'].data_ptr()
+        st.exp_avg_sq = f['exp_avg_sq' if bits == 32 else 'exp_avg_rms'].data_ptr()
+        if bits == 8:
+            st.exp_avg_scale, st.exp_avg_sq_scale = f['exp_avg_scale'].data_ptr(), f['exp_avg_rms_scale'].data_ptr()
+        if master:
+            st.master = f['master'].data_ptr()
+        if capturable:
+            st.steps, st.factors = self.steps.data_ptr(), self.factors.data_ptr()
+
+    def views(self, i):
+        """The state dict entry of parameter i: views of the flat buffers."""
+        at, n = int(self.starts[i]), int(self.sizes[i])
+        shape = self.params[i].shape
+        one = {'step': self.steps[i]}
+        for name, (_, per) in self.kinds.items():
+            one[name] = self.flat[name][at:at + n].view(shape) if per == 1 else self.flat[name][at // per:at // per + -(-n // per)]
+        return one
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) on the GPU, all tensors of a parameter group in one pass:
+
+        m <- b1 m + (1 - b1) g,   v <- b2 v + (1 - b2) g^2
+        p <- p (1 - lr weight_decay) - lr / (1 - b1^t)  m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    computed in fp32 whatever the parameters' type (fp32, bf16, fp16), p rounded once at the end.
+
+    ``state_bits=8`` keeps m and sqrt(v) as e4m3 codes with one fp32 scale per 256 elements (2.03 bytes of state an element
+    instead of 8). Codes are rounded with a dither that depends on the element and the step alone: plain rounding would hold
+    a slow average where it is (v moves 0.1 % a step, a code's gap is 6 to 12 %); results are still reproducible to the bit.
+    A gradient that is not finite spoils its block of 256 elements, not its element alone.
+
+    ``master_weights=True`` (bf16 / fp16 parameters) keeps fp32 values that are updated and rounded into the parameters. An
+    element of a parameter that is not its master rounded was written by somebody else since (a loaded checkpoint, a
+    broadcast) and becomes its master's new value: the step reads the parameter for that (2 bytes of 18 an element).
+
+    ``capturable=True`` keeps the step counts on the device, so that ``step()`` can be captured in a HIP graph and replayed;
+    lr and weight_decay are those of the capture, and the gradients have to stay where they were. Take one step, or call
+    ``init_state()``, before the capture. A counter belongs to a parameter: one without a gradient is left out and not counted.
+
+    State tensors are views of flat buffers (``state_buffers()``): write into them or use ``load_state_dict``; putting
+    other tensors in their place is not seen. Parameters must be contiguous and must not overlap."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False,
+                 capturable=False):
+        for name, x in (('lr', lr), ('eps', eps), ('weight_decay', weight_decay)):
+            if isinstance(x, torch.Tensor) or not x >= 0 or math.isinf(x):
+                raise ValueError(f'AdamW: {name} must be a finite number >= 0, got {x!r}')
+        if len(betas) != 2 or not all(0 <= b < 1 for b in betas):
+            raise ValueError(f'AdamW: betas must lie in [0, 1), got {betas!r}')
+        if state_bits not in (8, 32):
+            raise ValueError(f'AdamW: state_bits must be 8 or 32, got {state_bits!r}')
+        self._segments = None
+        self.state_bits, self.master_weights, self.capturable = state_bits, bool(master_weights), bool(capturable)
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    # ------------------------------------------------------------------ state
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        seen = set()
+        for group in self.param_groups:
+            for p in group['params']:
+                if not p.is_cuda:
+                    raise RuntimeError(f'AdamW: a parameter is on {p.device}; this optimiser has no CPU path')
+                if p.dtype not in _DTYPES:
+                    raise RuntimeError(f'AdamW: parameters must be fp32, bf16 or fp16, got {p.dtype}')
+                if p.is_sparse or not p.is_contiguous():
+                    raise RuntimeError('AdamW: parameters must be dense and contiguous')
+                if self.master_weights and p.dtype == torch.float32:
+                    raise RuntimeError('AdamW: master_weights is for bf16 and fp16 parameters')
+                if id(p) in seen:
+                    raise RuntimeError('AdamW: a parameter is given twice')
+                seen.add(id(p))
+        spans = sorted((p.device.index, p.data_ptr(), p.data_ptr() + p.numel() * p.element_size())
+                       for g in self.param_groups for p in g['params'] if p.numel())
+        for a, b in zip(spans, spans[1:]):
+            if a[0] == b[0] and b[1] < a[2]:
+                raise RuntimeError('AdamW: two parameters overlap in memory')
+
+    @torch.no_grad()
+    def init_state(self):
+        """Allocates the state of parameters that have none yet (zeros; a master takes its parameter's value)."""
+        if self._segments is None:
+            self._segments = [[] for _ in self.param_groups]
+            given = {p: s for p, s in self.state.items() if s}
+        else:
+            given = {}
+        self._segments += [[] for _ in self.param_groups[len(self._segments):]]
+        for group, segments in zip(self.param_groups, self._segments):
+            known = {id(p) for s in segments for p in s.params}
+            sorts = {}
+            for p in group['params']:
+                if id(p) not in known:
+                    sorts.setdefault((p.device, p.dtype), []).append(p)
+            for params in sorts.values():
+                seg = _Segment(params, self.state_bits, self.master_weights, self.capturable)
+                for i, p in enumerate(params):
+                    one = seg.views(i)
+                    if p in given:
+                        self._take(one, given[p])
+                    elif seg.has_master:
+                        one['master'].copy_(p.detach())
+                    self.state[p] = one
+                segments.append(seg)
+
+    def _take(self, to, given):
+        """Copies a state entry of a state dict (or of another copy of this optimiser) into the views ``to``."""
+        if set(given) != set(to):
+            raise ValueError(f'AdamW: a state with {sorted(given)} does not fit state_bits={self.state_bits}, '
+                             f'master_weights={self.master_weights} (wanted: {sorted(to)})')
+        for name, x in to.items():
+            y = given[name]
+            if name == 'step':
+                x.fill_(int(y))
+                continue
+            if not isinstance(y, torch.Tensor) or y.numel() != x.numel():
+                raise ValueError(f'AdamW: state {name} does not have the parameter\'s size')
+            if x.dtype.itemsize == 1:
+                if y.dtype != x.dtype:
+                    raise ValueError(f'AdamW: state {name} must be {x.dtype}, got {y.dtype}')
+                x.view(torch.uint8).view(-1).copy_(y.contiguous().view(torch.uint8).view(-1))
+            else:
+                x.view(-1).copy_(y.reshape(-1))
+
+    def state_buffers(self):
+        """{name: flat tensor} of all state, in the order of the parameters, every tensor's part starting at a multiple of
+        256 elements (of its 1 scale per 256): what a sharded or asynchronous checkpoint copies in a few pieces. Names of a
+        second, third, ... set of parameters (another group, device or type) end in .1, .2, ..."""
+        self.init_state()
+        found = [s for segments in self._segments for s in segments]
+        return {name + (f'.{i}' if i else ''): t for i, s in enumerate(found) for name, t in s.flat.items()}
+
+    def load_state_dict(self, state_dict):
+        packed = state_dict['state']
+        super().load_state_dict({'state': {}, 'param_groups': state_dict['param_groups']})
+        ids = [i for g in state_dict['param_groups'] for i in g['params']]
+        params = [p for g in self.param_groups for p in g['params']]
+        self._segments = None
+        self.state.clear()
+        self.init_state()
+        for i, p in zip(ids, params):
+            if i in packed:
+                self._take(self.state[p], packed[i])
+
+    def __getstate__(self):
+        return {**super().__getstate__(), 'state_bits': self.state_bits, 'master_weights': self.master_weights,
+                'capturable': self.capturable}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._segments = None                             # a copy: flat buffers of its own, filled from the copied state
+        if any(self.state.values()):
+            self.init_state()
+
+    # ------------------------------------------------------------------ step
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step of every parameter that has a gradient; asynchronous on each device's current stream."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if self._segments is None or any(sum(len(s.params) for s in segs) != len(g['params'])
+                                         for segs, g in zip(self._segments + [[]] * len(self.param_groups), self.param_groups)):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError('AdamW: take a step or call init_state() before capturing one in a graph')
+            self.init_state()
+        for group, segments in zip(self.param_groups, self._segments):
+            for seg in segments:
+                self._step_segment(group, seg)
+        return loss
+
+    def _step_segment(self, group, seg):
+        # The host's time a step is what a few attributes of every tensor cost (0.14 us each): they are read column by column
+        # in C loops. A parameter at the address that it had in the last step is the tensor that was checked then.
+        params, table, sizes = seg.params, seg.table, seg.size_list
+        grads = list(map(_grad_of, params))
+        live = slice(None)
+        if _NONE in set(map(type, grads)):
+            live = [i for i, g in enumerate(grads) if g is not None]
+            if not live:
+                return
+            params, grads, sizes, table = [params[i] for i in live], [grads[i] for i in live], [sizes[i] for i in live], table[live]
+        dev, dtype, n = seg.device, seg.dtype, len(params)
+        where = list(map(_T.data_ptr, params))
+        if where != seg.where:
+            if any(p.device != dev or p.dtype is not dtype or not p.is_contiguous() for p in params):
+                raise RuntimeError(f'AdamW: a parameter is not a contiguous {dtype} tensor on {dev} any more')
+        if list(map(_dtype_of, grads)).count(dtype) != n or list(map(_T.get_device, grads)).count(dev.index) != n:
+            raise RuntimeError(f'AdamW: a gradient is not {dtype} on {dev}, as its parameter is')
+        if any(map(_layout_of, grads)):
+            raise RuntimeError('AdamW: a gradient is sparse')
+        if list(map(_T.numel, params)) != sizes or list(map(_T.numel, grads)) != sizes:
+            raise RuntimeError('AdamW: a parameter or its gradient changed its size')
+        if list(map(_T.is_contiguous, grads)).count(True) != n:
+            grads = [g.contiguous() for g in grads]
+        with torch.cuda.device(dev):
+            if not seg.capturable and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError('AdamW: a step is captured in a graph, but the optimiser was made without capturable=True')
+            b1, b2 = group['betas']
+            lr = float(group['lr'])
+            table['param'] = where
+            table['grad'] = list(map(_T.data_ptr, grads))
+            table['decay'] = 1.0 - lr * group['weight_decay']
+            if not seg.capturable:
+                steps = seg.host_steps[live] + 1
+                first = int(steps[0])
+                if (steps == first).all():
+                    table['rate'], table['root'] = lr / (1.0 - b1 ** first), 1.0 / math.sqrt(1.0 - b2 ** first)
+                else:
+                    table['rate'], table['root'] = lr / (1.0 - b1 ** steps.astype(np.float64)), 1.0 / np.sqrt(1.0 - b2 ** steps.astype(np.float64))
+                table['turn'] = steps & 0xFFFFFFFF
+            _check(_lib.dgnn_adamw(table.ctypes.data, n, _DTYPES[dtype], seg.bits, ctypes.byref(seg.cstate), lr, b1, b2,
+                                   float(group['eps']), _stream(params[0])), 'adamw')
+        seg.where = where
+        if not seg.capturable:
+            seg.host_steps[live] += 1
+        # the kernel writes behind autograd's back: a graph that saved a parameter has to notice
+        torch.autograd.graph.increment_version(params)

@@ -1,0 +1,74 @@
+/*
+ * dgnn_train.h -- C ABI of libdgnn_spmm.so for what a training step computes beside the aggregation: the dense layer
+ * transform with its epilogue and gradients, and the optimiser step. Same conventions as dgnn_spmm.h: plain device
+ * pointers and sizes, an explicit HIP stream passed as void*, an int status with dgnn_last_error(); nothing allocates
+ * device memory, nothing synchronises, every call can be captured in a HIP graph.
+ */
+#ifndef DGNN_TRAIN_H
+#define DGNN_TRAIN_H
+
+#include "dgnn_spmm.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define DGNN_F32  0
+#define DGNN_BF16 1
+#define DGNN_F16  2
+
+/*
+ * One AdamW step over `count` tensors (a handful of launches for hundreds of them). With g a tensor's gradient, t the
+ * number of its step:
+ *     m <- b1 m + (1 - b1) g                 v <- b2 v + (1 - b2) g^2
+ *     p <- p decay - rate m / (sqrt(v) root + eps)
+ *     decay = 1 - lr * weight_decay,  rate = lr / (1 - b1^t),  root = 1 / sqrt(1 - b2^t)
+ * all in fp32, each operation rounded once and in this order, p rounded to its type at the end.
+ *
+ *   param, grad   device, numel elements of `dtype` (DGNN_F32 | DGNN_BF16 | DGNN_F16), element-aligned, contiguous
+ *   start         first element of the tensor in the state buffers, a multiple of 256
+ *   index         the tensor's entry of `steps` / `factors` (only read when they are given)
+ *   decay, rate, root, turn    the factors above and t mod 2^32 (unused when `steps` is given)
+ *
+ * State buffers (device, 16-byte aligned, shared by all tensors of the call):
+ *   master        NULL, or the fp32 values that are updated in place of param; param receives them rounded. An element of
+ *                 param that is not its master rounded replaces it first (somebody else wrote it)
+ *   state_bits 32: exp_avg, exp_avg_sq are float; the scales are NULL
+ *   state_bits 8:  exp_avg holds m and exp_avg_sq holds sqrt(v) as e4m3 codes, one float scale per 256 elements
+ *     (value = code * scale). A block's scale is max(largest value, 2^-100) / 448. A value x is rounded at the e4m3 step s
+ *     of its magnitude (2^(e-3), at least 2^-9) to s floor(|x| / s + u), u in [0, 1) a 16-bit fraction that depends on
+ *     the element's index in its tensor and on t alone (two Weyl sequences), so that a slow average does not stick to one
+ *     code; a root above zero keeps at least 2^-9, so no denominator vanishes. A value that is not finite makes its
+ *     block's values NaN from the next step on.
+ * In all buffers elements between a tensor's end and the next multiple of 256 are free to be written.
+ *
+ * steps (device int64[], or NULL) and factors (device float[4 * entries]): when given, a first launch advances
+ * steps[index] of every tensor and derives rate, root and t from it on the device with lr, beta1, beta2 -- what a captured
+ * graph needs, whose host arguments are frozen; lr and weight_decay stay those of the capture.
+ */
+struct dgnn_adamw_tensor {
+  void* param;
+  const void* grad;
+  int64_t numel, start;
+  float decay, rate, root;
+  uint32_t turn;
+  int32_t index, reserved;
+};
+
+struct dgnn_adamw_state {
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  float* master;
+  int64_t* steps;
+  float* factors;
+};
+
+int dgnn_adamw(const struct dgnn_adamw_tensor* tensors, int32_t count, int32_t dtype, int32_t state_bits,
+               const struct dgnn_adamw_state* state, double lr, double beta1, double beta2, double eps, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* DGNN_TRAIN_H */
