@@ -4,6 +4,7 @@ parameters, moments in 32 or 8 bits).
 
 Where `own` is false, `run` computes the same from elementary torch operations in 32 bits, rounded once at the end."""
 import math
+import sys
 
 import torch
 
@@ -171,10 +172,7 @@ def prepare(case, seed):
         return _linear_inputs(case, seed)
     s = _adamw_inputs(case, seed)
     if own:                      # the optimiser that a training program makes once and keeps
-        import sys
-        if "dist-gnn_amd" not in sys.path:
-            sys.path.insert(0, "dist-gnn_amd")
-        import spmm_cpp
+        spmm_cpp = _package()
         params = [torch.nn.Parameter(s["param"][at:at + n]) for at, n in zip(s["starts"], s["sizes"])]
         for p, at, n in zip(params, s["starts"], s["sizes"]):
             p.grad = s["grad"][at:at + n]
@@ -229,8 +227,15 @@ def _linear_plain(s, wide=torch.float32):
     return got
 
 
-def _linear_own(s):
+def _package():
+    if "dist-gnn_amd" not in sys.path:
+        sys.path.insert(0, "dist-gnn_amd")
     import spmm_cpp
+    return spmm_cpp
+
+
+def _linear_own(s):
+    spmm_cpp = _package()
     case = s["case"]
     y = spmm_cpp.linear(s["x"], s["weight"], s["bias"], activation=case["act"], residual=s["residual"])
     got = {"y": y}
