@@ -1,0 +1,397 @@
+// dgnn_gemm.h -- the matrix product behind dgnn_linear_*: C[M x N] = A[M x K] B[K x N] on the matrix cores with the layer's
+// epilogue. Compiled once per element type (dgnn_gemm_f32.hip, dgnn_gemm_bf16.hip, dgnn_gemm_f16.hip).
+//
+// Each operand comes in one of two layouts: "along" keeps the contraction contiguous in memory (x and P in x W and P W^T, W in
+// P W^T), "across" keeps the other dimension contiguous (W in x W, both operands of x^T P). Either way a tile is staged in
+// LDS as 16-byte chunks of 8 consecutive contraction elements of one row (or column), chunk-major: what one lane hands to
+// v_mfma_f32_32x32x16 is one ds_read_b128, and 32 lanes read 512 consecutive bytes. "Across" tiles are turned in registers: a
+// lane loads 8 contraction rows of a few columns and writes one chunk per column.
+//
+// fp32 operands: gfx950 has no wide fp32 matrix instruction (its 32-bit rate is a sixteenth of bf16's), so an fp32 value is
+// split into three bf16 pieces a = a1 + a2 + a3, each the rounding of what the ones before leave (8 bits each, 24 in all, so
+// the split is exact up to 2^-25 |a|), and the six products of at least 2^-16 relative size are summed in the fp32
+// accumulators: a1 b1 + a1 b2 + a2 b1 + a2 b2 + a1 b3 + a3 b1. What is left out is at most 2^-24 |a| |b| a term, as much as
+// one fp32 rounding. Values under 2^-109 lose bits (their last pieces are below bf16's smallest number): absolute
+// errors of 2^-134 |b|. An infinity's pieces are not finite and would give NaN where fp32 gives infinity, so an output that
+// is not finite is computed again as a chain of fused multiply-adds, whose infinities and NaN are fp32's own.
+#pragma once
+#include "dgnn_internal.h"
+
+namespace dgnn {
+
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
+
+struct Gemm {
+  const void* a;
+  const void* b;
+  int64_t lda, ldb;
+  bool a_along, b_along;
+  int64_t M, N, K;
+  // epilogue: c = act(acc + bias) + residual; save receives acc + bias (or, for relu, a bit per value that is > 0)
+  const void* bias;
+  const void* residual;
+  int64_t ld_residual;
+  void* c;
+  int64_t ldc;
+  void* save;
+  int64_t ld_save;
+  int act;
+  float* partial;          // slices x M x N when slices > 1
+  int slices;
+  int64_t slice_k;         // contraction elements a slice takes, a multiple of 64
+  hipStream_t stream;
+};
+
+__device__ __forceinline__ float act_of(int act, float t) {
+  switch (act) {
+    case ACT_RELU: return t <= 0.f ? 0.f : t;
+    case ACT_GELU: return 0.5f * t * (1.f + erff(t * 0.70710678118654752f));
+    case ACT_SILU: return t / (1.f + expf(-t));
+    default: return t;
+  }
+}
+
+template <typename T> struct Unit;          // W: elements of a 16-byte load
+template <> struct Unit<float> { static constexpr int W = 4, PLANES = 3, BK = 32; };
+template <> struct Unit<__bf16> { static constexpr int W = 8, PLANES = 1, BK = 64; };
+template <> struct Unit<_Float16> { static constexpr int W = 8, PLANES = 1, BK = 64; };
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+// 16 bytes at an address that is only element-aligned
+template <typename T> __device__ __forceinline__ u4 load16(const T* p) {
+  if constexpr (sizeof(T) == 4) return *reinterpret_cast<const u4_at4*>(p);
+  else return *reinterpret_cast<const u4_at2*>(p);
+}
+
+// W elements of which only the first `n` (0..W) exist; the others are zero
+template <typename T> __device__ __forceinline__ u4 load_some(const T* p, int64_t n) {
+  constexpr int W = Unit<T>::W;
+  union { u4 v; T e[W]; } r;
+  r.v = u4{0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+    if (i < n) r.e[i] = p[i];
+  return r.v;
+}
+
+__device__ __forceinline__ uint32_t pack_bf(float x, float y) {
+  union { bf2 h; uint32_t u; } r;
+  r.h = __builtin_convertvector(f2{x, y}, bf2);
+  return r.u;
+}
+
+// 8 fp32 values -> 3 chunks of 8 bf16: their exact sum is the value to 24 bits
+__device__ __forceinline__ void split8(const float (&v)[8], u4 (&out)[3]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float x = v[2 * i], y = v[2 * i + 1];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const uint32_t h = pack_bf(x, y);
+      out[p][i] = h;
+      if (p < 2) { x -= __uint_as_float(h << 16); y -= __uint_as_float(h & 0xffff0000u); }
+    }
+  }
+}
+
+// One operand's tile: ROWS rows (or columns) by BK contraction elements, fetched by THREADS lanes into registers and stored
+// to LDS as PLANES x BK/8 chunk columns.
+template <typename T, bool ALONG, int ROWS, int THREADS> struct Tile {
+  static constexpr int W = Unit<T>::W, BK = Unit<T>::BK, PL = Unit<T>::PLANES, CH = BK / 8;
+  static constexpr int COLUMN = ROWS * 16 + 32;               // bytes of a chunk column; the 32 spread chunk columns over banks
+  static constexpr int BYTES = PL * CH * COLUMN;
+  static constexpr int UNITS = ALONG ? ROWS * CH : (ROWS / W) * CH;
+  static constexpr int PER = (UNITS + THREADS - 1) / THREADS;
+  static constexpr int QUADS = ALONG ? 8 / W : 8;             // 16-byte loads of a unit
+  u4 r[PER][QUADS];
+
+  // chunks of neighbouring rows lie side by side; the exchange inside groups of 8 spreads the writes of turned tiles,
+  // whose lanes are W rows apart, over the banks
+  static __device__ __forceinline__ int place(int row) { return row ^ ((row >> 4) & 7); }
+
+  __device__ __forceinline__ void fetch(const T* base, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int64_t kend, int tid) {
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int id = tid + u * THREADS;
+      if (UNITS % THREADS != 0 && id >= UNITS) break;
+      if constexpr (ALONG) {
+        const int64_t row = row0 + id / CH;
+        const T* p = base + (row < rows ? row : rows - 1) * ld + k0 + 8 * (id % CH);
+        const int64_t left = kend - k0 - 8 * (id % CH);
+        if (left >= 8) {
+#pragma unroll
+          for (int q = 0; q < QUADS; ++q) r[u][q] = load16(p + q * W);
+        } else {
+#pragma unroll
+          for (int q = 0; q < QUADS; ++q) r[u][q] = load_some(p + q * W, left - q * W);
+        }
+      } else {
+        const int64_t col = row0 + (id % (ROWS / W)) * W;
+        const int64_t k = k0 + 8 * (id / (ROWS / W));
+        const T* p = base + k * ld + col;
+        const int64_t left = rows - col;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if (k + q >= kend) r[u][q] = u4{0, 0, 0, 0};
+          else if (left >= W) r[u][q] = load16(p + q * ld);
+          else r[u][q] = load_some(p + q * ld, left);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void store(char* lds, int tid) const {
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int id = tid + u * THREADS;
+      if (UNITS % THREADS != 0 && id >= UNITS) break;
+      if constexpr (ALONG) {
+        char* at = lds + (id % CH) * COLUMN + place(id / CH) * 16;
+        if constexpr (PL == 3) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[u][i / 4][i % 4]);
+          u4 h[3];
+          split8(v, h);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) *reinterpret_cast<u4*>(at + p * CH * COLUMN) = h[p];
+        } else {
+          *reinterpret_cast<u4*>(at) = r[u][0];
+        }
+      } else {
+        const int row = (id % (ROWS / W)) * W;
+        char* col = lds + (id / (ROWS / W)) * COLUMN;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          char* at = col + place(row + w) * 16;
+          if constexpr (PL == 3) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[u][i][w]);
+            u4 h[3];
+            split8(v, h);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<u4*>(at + p * CH * COLUMN) = h[p];
+          } else {
+            u4 h;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)                       // half w of rows 2i and 2i + 1
+              h[i] = __builtin_amdgcn_perm(r[u][2 * i + 1][w / 2], r[u][2 * i][w / 2], w % 2 ? 0x07060302u : 0x05040100u);
+            *reinterpret_cast<u4*>(at) = h;
+          }
+        }
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c, __bf16) {
+  union { u4 u; bf8 h; } x, y;
+  x.u = a; y.u = b;
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.h, y.h, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c, float) { return mfma(a, b, c, __bf16()); }
+__device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c, _Float16) {
+  union { u4 u; h8 h; } x, y;
+  x.u = a; y.u = b;
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, y.h, c, 0, 0, 0);
+}
+
+// what one output element becomes: bias, saved slope data (not relu's, which is one bit), activation, residual
+template <typename T>
+__device__ __forceinline__ void finish(const Gemm& g, int64_t row, int64_t col, float t) {
+  if (g.save && g.act > ACT_RELU) ((T*)g.save)[row * g.ld_save + col] = (T)t;
+  t = act_of(g.act, t);
+  if (g.residual) t += (float)((const T*)g.residual)[row * g.ld_residual + col];
+  ((T*)g.c)[row * g.ldc + col] = (T)t;
+}
+
+template <typename T, bool AA, bool BA, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm g) {
+  constexpr int THREADS = WM * WN * 64, BK = Unit<T>::BK, PL = Unit<T>::PLANES;
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+  using TA = Tile<T, AA, BM, THREADS>;
+  using TB = Tile<T, BA, BN, THREADS>;
+  __shared__ __attribute__((aligned(16))) char lds[2][TA::BYTES + TB::BYTES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wm = wave % WM, wn = wave / WM;
+  const int64_t tiles_n = (g.N + BN - 1) / BN;
+  const int64_t row0 = (int64_t)(blockIdx.x / tiles_n) * BM, col0 = (int64_t)(blockIdx.x % tiles_n) * BN;
+  const int64_t k0 = (int64_t)blockIdx.y * g.slice_k;
+  const int64_t kend = k0 + g.slice_k < g.K ? k0 + g.slice_k : g.K;
+  const T* a = (const T*)g.a;
+  const T* b = (const T*)g.b;
+
+  f16v acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+
+  TA ta;
+  TB tb;
+  if (k0 < kend) {
+    ta.fetch(a, g.lda, row0, g.M, k0, kend, tid);
+    tb.fetch(b, g.ldb, col0, g.N, k0, kend, tid);
+    ta.store(lds[0], tid);
+    tb.store(lds[0] + TA::BYTES, tid);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int64_t k = k0; k < kend; k += BK) {
+    const bool more = k + BK < kend;
+    if (more) {
+      ta.fetch(a, g.lda, row0, g.M, k + BK, kend, tid);
+      tb.fetch(b, g.ldb, col0, g.N, k + BK, kend, tid);
+    }
+    const char* la = lds[buf];
+    const char* lb = lds[buf] + TA::BYTES;
+#pragma unroll
+    for (int s = 0; s < BK / 16; ++s) {
+      const int chunk = 2 * s + (lane >> 5);
+      u4 fa[TM][PL], fb[TN][PL];
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+          fa[i][p] = *reinterpret_cast<const u4*>(la + (p * (BK / 8) + chunk) * TA::COLUMN + TA::place((wm * TM + i) * 32 + (lane & 31)) * 16);
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+          fb[j][p] = *reinterpret_cast<const u4*>(lb + (p * (BK / 8) + chunk) * TB::COLUMN + TB::place((wn * TN + j) * 32 + (lane & 31)) * 16);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          if constexpr (PL == 3) {                             // small products first
+            acc[i][j] = mfma(fa[i][2], fb[j][0], acc[i][j], T());
+            acc[i][j] = mfma(fa[i][0], fb[j][2], acc[i][j], T());
+            acc[i][j] = mfma(fa[i][1], fb[j][1], acc[i][j], T());
+            acc[i][j] = mfma(fa[i][1], fb[j][0], acc[i][j], T());
+            acc[i][j] = mfma(fa[i][0], fb[j][1], acc[i][j], T());
+          }
+          acc[i][j] = mfma(fa[i][0], fb[j][0], acc[i][j], T());
+        }
+    }
+    if (more) {
+      ta.store(lds[buf ^ 1], tid);
+      tb.store(lds[buf ^ 1] + TA::BYTES, tid);
+    }
+    __syncthreads();
+    buf ^= 1;
+  }
+
+  // element i of a lane's 16: row 8 (i / 4) + 4 (lane / 32) + i % 4, column lane % 32 of the 32 x 32 tile
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int64_t col = col0 + (wn * TN + j) * 32 + (lane & 31);
+    const bool in_n = col < g.N;
+    const float bias = g.bias && in_n && g.slices == 1 ? (float)((const T*)g.bias)[col] : 0.f;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int64_t row = row0 + (wm * TM + i) * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+        const bool in = in_n && row < g.M;
+        float t = acc[i][j][e];
+        if constexpr (PL == 3) {
+          if (in && !(fabsf(t) < __builtin_huge_valf())) {
+            t = 0.f;
+            for (int64_t k = k0; k < kend; ++k)
+              t = fmaf((float)a[AA ? row * g.lda + k : k * g.lda + row], (float)b[BA ? col * g.ldb + k : k * g.ldb + col], t);
+          }
+        }
+        if (g.slices > 1) {
+          if (in) g.partial[((int64_t)blockIdx.y * g.M + row) * g.N + col] = t;
+          continue;
+        }
+        t += bias;
+        if (g.save && g.act == ACT_RELU) {
+          const uint64_t bits = __ballot(in && !(t <= 0.f));
+          if (row < g.M && (lane & 31) == 0 && in_n)
+            ((uint32_t*)g.save)[row * g.ld_save + col / 32] = (uint32_t)(bits >> (lane & 32));
+        }
+        if (in) finish<T>(g, row, col, t);
+      }
+    }
+  }
+}
+
+// Joins the slices of a product that was cut along its contraction, in their order, and finishes it. A wave takes 64
+// consecutive columns of a row, so relu's bits are whole words.
+template <typename T>
+__global__ __launch_bounds__(256) void gemm_join_kernel(const Gemm g) {
+  const int lane = threadIdx.x & 63;
+  const int64_t wide = (g.N + 63) / 64;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= g.M * wide) return;
+  const int64_t row = at / wide, col = at % wide * 64 + lane;
+  const bool in = col < g.N;
+  float t = 0.f;
+  if (in)
+    for (int s = 0; s < g.slices; ++s) t += g.partial[((int64_t)s * g.M + row) * g.N + col];
+  if (in && g.bias) t += (float)((const T*)g.bias)[col];
+  if (g.save && g.act == ACT_RELU) {
+    const uint64_t bits = __ballot(in && !(t <= 0.f));
+    if ((lane & 31) == 0 && in) ((uint32_t*)g.save)[row * g.ld_save + col / 32] = (uint32_t)(bits >> (lane & 32));
+  }
+  if (in) finish<T>(g, row, col, t);
+}
+
+struct Shape { int bm, bn; };
+
+// Tile by the sides of the output: the narrowest that covers it once, else 128 x 256 (the operand with fewer bytes a
+// multiply-add to move; 8 waves of 64 x 64).
+inline Shape shape_of(int64_t M, int64_t N) {
+  if (M <= 32) return {32, 128};
+  if (N <= 32) return {128, 32};
+  if (N <= 64) return {128, 64};
+  if (N <= 128) return {128, 128};
+  return {128, 256};
+}
+
+inline int64_t tiles_of(Shape s, int64_t M, int64_t N) { return ((M + s.bm - 1) / s.bm) * ((N + s.bn - 1) / s.bn); }
+
+template <typename T, bool AA, bool BA>
+int gemm_launch(const Gemm& g) {
+  const Shape s = shape_of(g.M, g.N);
+  const int64_t tiles = tiles_of(s, g.M, g.N);
+  if (tiles > 0x7fffffffLL) return dgnn_fail(DGNN_E_BADARG, "linear: too many tiles%s (%lld)", "", tiles);
+  const dim3 grid((uint32_t)tiles, (uint32_t)g.slices);
+  switch (s.bm * 1000 + s.bn) {
+    case 32128: hipLaunchKernelGGL((gemm_kernel<T, AA, BA, 32, 128, 1, 4>), grid, dim3(256), 0, g.stream, g); break;
+    case 128032: hipLaunchKernelGGL((gemm_kernel<T, AA, BA, 128, 32, 4, 1>), grid, dim3(256), 0, g.stream, g); break;
+    case 128064: hipLaunchKernelGGL((gemm_kernel<T, AA, BA, 128, 64, 4, 1>), grid, dim3(256), 0, g.stream, g); break;
+    case 128128: hipLaunchKernelGGL((gemm_kernel<T, AA, BA, 128, 128, 2, 2>), grid, dim3(256), 0, g.stream, g); break;
+    default: hipLaunchKernelGGL((gemm_kernel<T, AA, BA, 128, 256, 2, 4>), grid, dim3(512), 0, g.stream, g); break;
+  }
+  DGNN_LAUNCHED();
+  if (g.slices > 1) {
+    const int64_t waves = g.M * ((g.N + 63) / 64);
+    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, g.stream, g);
+    DGNN_LAUNCHED();
+  }
+  return DGNN_OK;
+}
+
+template <typename T>
+int gemm_typed(const Gemm& g) {
+  if (g.a_along && !g.b_along) return gemm_launch<T, true, false>(g);
+  if (g.a_along && g.b_along) return gemm_launch<T, true, true>(g);
+  return gemm_launch<T, false, false>(g);
+}
+
+__attribute__((visibility("hidden"))) int gemm_f32(const Gemm& g);
+__attribute__((visibility("hidden"))) int gemm_bf16(const Gemm& g);
+__attribute__((visibility("hidden"))) int gemm_f16(const Gemm& g);
+
+}  // namespace dgnn

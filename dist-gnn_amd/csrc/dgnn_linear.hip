@@ -1,0 +1,303 @@
+// dgnn_linear.hip -- C entries of the layer transform y = act(x W + b) + r and its gradients (include/dgnn_train.h): the
+// argument checks, how a product is cut over the chip, and the slope / column-sum kernel. The matrix products themselves are
+// in dgnn_gemm.h.
+
+#include "dgnn_gemm.h"
+
+namespace {
+
+using namespace dgnn;
+
+// ---------------------------------------------------------------------------------------
+// p = dy act'(x W + b) and the sums of p's columns. Reads dy and what the forward pass saved once and writes p once. A row
+// is taken by the fewest lanes (a power of two) that cover it with 4 columns each, 64 at most, so narrow rows fill a
+// wave too; a lane keeps its columns' sums over the block's rows, in fp32, the block adds its lanes in a fixed order and a
+// second launch adds the blocks': no atomics, the same bits every run.
+// ---------------------------------------------------------------------------------------
+struct Slope {
+  const void* dy;
+  const void* save;
+  void* p;
+  int64_t ld_dy, ld_save, ld_p, M, N, slab;      // rows a block takes
+  float* partial;                                // gridDim.y x N, or null
+  int act, lanes;
+};
+
+__device__ __forceinline__ float slope_of(int act, float t) {
+  if (act == ACT_GELU) return 0.5f * (1.f + erff(t * 0.70710678118654752f)) + t * expf(-0.5f * t * t) * 0.39894228040143268f;
+  const float s = 1.f / (1.f + expf(-t));
+  return s * (1.f + t * (1.f - s));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void slope_kernel(const Slope g) {
+  typedef T quad __attribute__((ext_vector_type(4), aligned(sizeof(T) == 4 ? 4 : 2)));
+  __shared__ float sums[256][4];
+  const int lane = threadIdx.x % g.lanes, group = threadIdx.x / g.lanes, groups = 256 / g.lanes;
+  const int64_t col = ((int64_t)blockIdx.x * g.lanes + lane) * 4;
+  const int64_t first = (int64_t)blockIdx.y * g.slab;
+  const int64_t last = first + g.slab < g.M ? first + g.slab : g.M;
+  const int have = g.N - col >= 4 ? 4 : (g.N > col ? (int)(g.N - col) : 0);
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (have > 0) {
+    for (int64_t row = first + group; row < last; row += groups) {
+      const T* dy = (const T*)g.dy + row * g.ld_dy + col;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (have == 4) {
+        const quad q = *reinterpret_cast<const quad*>(dy);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (float)q[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < have) v[i] = (float)dy[i];
+      }
+      if (g.act == ACT_RELU) {
+        const uint32_t word = ((const uint32_t*)g.save)[row * g.ld_save + col / 32] >> (col & 31);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (word >> i) & 1 ? v[i] : 0.f;
+      } else if (g.act != ACT_NONE) {
+        const T* pre = (const T*)g.save + row * g.ld_save + col;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < have) v[i] *= slope_of(g.act, (float)pre[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] += v[i];
+      if (g.p) {
+        T* p = (T*)g.p + row * g.ld_p + col;
+        if (have == 4) {
+          quad q;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q[i] = (T)v[i];
+          *reinterpret_cast<quad*>(p) = q;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i < have) p[i] = (T)v[i];
+        }
+      }
+    }
+  }
+  if (!g.partial) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sums[threadIdx.x][i] = sum[i];
+  __syncthreads();
+  if (group == 0) {
+    for (int k = 1; k < groups; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] += sums[k * g.lanes + lane][i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < have) g.partial[(int64_t)blockIdx.y * g.N + col + i] = sum[i];
+  }
+}
+
+// sums of the slabs' columns: 16 columns a block, 16 lanes each take every 16th slab, added in their order
+template <typename T>
+__global__ __launch_bounds__(256) void slab_join_kernel(const float* __restrict__ partial, int64_t slabs, int64_t N, T* __restrict__ out) {
+  __shared__ float sums[16][17];
+  const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
+  const int64_t col = (int64_t)blockIdx.x * 16 + c;
+  float t = 0.f;
+  if (col < N)
+    for (int64_t s = k; s < slabs; s += 16) t += partial[s * N + col];
+  sums[k][c] = t;
+  __syncthreads();
+  if (k == 0 && col < N) {
+    for (int i = 1; i < 16; ++i) t += sums[i][c];
+    out[col] = (T)t;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+constexpr int64_t kCompute = 256;              // compute units
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// A product with fewer output tiles than compute units is cut along its contraction, at 128 elements a slice or more.
+void cut(Gemm& g) {
+  const int64_t tiles = tiles_of(shape_of(g.M, g.N), g.M, g.N);
+  int64_t want = kCompute / (tiles > 0 ? tiles : 1);
+  const int64_t most = ceil_div(g.K, 128);
+  if (want > most) want = most;
+  if (want < 1) want = 1;
+  g.slice_k = ceil_div(ceil_div(g.K, want), 64) * 64;
+  if (g.slice_k == 0) g.slice_k = 64;
+  g.slices = (int)ceil_div(g.K, g.slice_k);
+  if (g.slices < 1) g.slices = 1;
+}
+
+int64_t slope_lanes(int64_t N) {
+  int64_t lanes = 1;
+  while (lanes < 64 && lanes * 4 < N) lanes *= 2;
+  return lanes;
+}
+
+int64_t slope_slab(int64_t M, int64_t N) {
+  const int64_t groups = 256 / slope_lanes(N), across = ceil_div(N, 4 * slope_lanes(N));
+  const int64_t blocks = 2048 / (across < 2048 ? across : 2048);
+  return ceil_div(ceil_div(M, blocks < 1 ? 1 : blocks), groups) * groups;
+}
+
+bool known_type(int32_t dtype) { return dtype == DGNN_F32 || dtype == DGNN_BF16 || dtype == DGNN_F16; }
+int64_t width(int32_t dtype) { return dtype == DGNN_F32 ? 4 : 2; }
+
+bool sizes_ok(int64_t M, int64_t K, int64_t N) {
+  const int64_t most = 0x7fffffffLL;
+  return M >= 0 && K >= 0 && N >= 0 && M <= most && K <= most && N <= most;
+}
+
+// a row-major rows x cols matrix: present, rows that do not overlap, elements aligned
+bool matrix_ok(const void* p, int64_t ld, int64_t rows, int64_t cols, int64_t w) {
+  if (rows == 0 || cols == 0) return true;
+  return p && ld >= cols && (uintptr_t)p % (uintptr_t)w == 0;
+}
+
+bool apart(const void* a, int64_t lda, int64_t ra, int64_t ca, const void* b, int64_t ldb, int64_t rb, int64_t cb, int64_t w) {
+  if (!a || !b || ra == 0 || ca == 0 || rb == 0 || cb == 0) return true;
+  const char* a0 = (const char*)a, *b0 = (const char*)b;
+  const char* a1 = a0 + ((ra - 1) * lda + ca) * w, *b1 = b0 + ((rb - 1) * ldb + cb) * w;
+  return a1 <= b0 || b1 <= a0;
+}
+
+int run(const Gemm& g, int32_t dtype, void* workspace, int64_t bytes, const char* who) {
+  Gemm h = g;
+  cut(h);
+  if (h.slices > 1) {
+    if (!workspace || bytes < (int64_t)h.slices * h.M * h.N * 4 || (uintptr_t)workspace % 4)
+      return dgnn_fail(DGNN_E_BADARG, "%s: workspace too small (%lld bytes wanted)", who, (long long)h.slices * h.M * h.N * 4);
+    h.partial = (float*)workspace;
+  }
+  if (dtype == DGNN_F32) return gemm_f32(h);
+  if (dtype == DGNN_BF16) return gemm_bf16(h);
+  return gemm_f16(h);
+}
+
+}  // namespace
+
+extern "C" {
+
+int dgnn_linear_workspace(int32_t pass, int64_t M, int64_t K, int64_t N, int32_t dtype, int64_t* bytes) {
+  if (!bytes || !known_type(dtype) || !sizes_ok(M, K, N)) return dgnn_fail(DGNN_E_BADARG, "linear_workspace: bad argument%s");
+  *bytes = 0;
+  Gemm g{};
+  switch (pass) {
+    case DGNN_LINEAR_FORWARD: g.M = M; g.N = N; g.K = K; break;
+    case DGNN_LINEAR_GRAD_INPUT: g.M = M; g.N = K; g.K = N; break;
+    case DGNN_LINEAR_GRAD_WEIGHT: g.M = K; g.N = N; g.K = M; break;
+    case DGNN_LINEAR_SLOPE:
+      if (M > 0 && N > 0) *bytes = ceil_div(M, slope_slab(M, N)) * N * 4;
+      return DGNN_OK;
+    default: return dgnn_fail(DGNN_E_BADARG, "linear_workspace: unknown pass%s (%lld)", "", pass);
+  }
+  if (g.M == 0 || g.N == 0) return DGNN_OK;
+  cut(g);
+  if (g.slices > 1) *bytes = (int64_t)g.slices * g.M * g.N * 4;
+  return DGNN_OK;
+}
+
+int dgnn_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                        const void* residual, int64_t ldr, void* y, int64_t ldy, void* save, int64_t lds,
+                        int64_t M, int64_t K, int64_t N, int32_t dtype, int32_t act,
+                        void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!known_type(dtype)) return dgnn_fail(DGNN_E_BADARG, "linear_forward: unknown type%s (%lld)", "", dtype);
+  if (act < ACT_NONE || act > ACT_SILU) return dgnn_fail(DGNN_E_BADARG, "linear_forward: unknown activation%s (%lld)", "", act);
+  if (!sizes_ok(M, K, N)) return dgnn_fail(DGNN_E_BADARG, "linear_forward: bad sizes%s");
+  if (M == 0 || N == 0) return DGNN_OK;
+  const int64_t b = width(dtype);
+  if (!matrix_ok(x, ldx, M, K, b) || !matrix_ok(w, ldw, K, N, b) || !matrix_ok(y, ldy, M, N, b) || (uintptr_t)bias % b
+      || (residual && !matrix_ok(residual, ldr, M, N, b)))
+    return dgnn_fail(DGNN_E_BADARG, "linear_forward: null, misaligned or overlapping rows%s");
+  if (save && act != ACT_NONE) {
+    const bool fits = act == ACT_RELU ? lds >= (N + 31) / 32 && (uintptr_t)save % 4 == 0 : lds >= N && (uintptr_t)save % b == 0;
+    if (!fits) return dgnn_fail(DGNN_E_BADARG, "linear_forward: save is too narrow or misaligned%s");
+  }
+  if (!apart(y, ldy, M, N, x, ldx, M, K, b) || !apart(y, ldy, M, N, w, ldw, K, N, b) || !apart(y, ldy, M, N, residual, ldr, M, N, b))
+    return dgnn_fail(DGNN_E_BADARG, "linear_forward: y overlaps an input%s");
+  Gemm g{};
+  g.a = x; g.lda = ldx; g.a_along = true;
+  g.b = w; g.ldb = ldw; g.b_along = false;
+  g.M = M; g.N = N; g.K = K;
+  g.bias = bias; g.residual = residual; g.ld_residual = ldr;
+  g.c = y; g.ldc = ldy;
+  g.save = act == ACT_NONE ? nullptr : save; g.ld_save = lds;
+  g.act = act;
+  g.stream = (hipStream_t)stream;
+  return run(g, dtype, workspace, workspace_bytes, "linear_forward");
+}
+
+int dgnn_linear_slope(const void* dy, int64_t ldd, const void* save, int64_t lds, void* p, int64_t ldp, void* dbias,
+                      int64_t M, int64_t N, int32_t dtype, int32_t act, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!known_type(dtype)) return dgnn_fail(DGNN_E_BADARG, "linear_slope: unknown type%s (%lld)", "", dtype);
+  if (act < ACT_NONE || act > ACT_SILU) return dgnn_fail(DGNN_E_BADARG, "linear_slope: unknown activation%s (%lld)", "", act);
+  if (!sizes_ok(M, 0, N)) return dgnn_fail(DGNN_E_BADARG, "linear_slope: bad sizes%s");
+  if (N == 0) return DGNN_OK;
+  const int64_t b = width(dtype);
+  hipStream_t s = (hipStream_t)stream;
+  if ((uintptr_t)dbias % b) return dgnn_fail(DGNN_E_BADARG, "linear_slope: misaligned dbias%s");
+  if (M > 0) {
+    if (!matrix_ok(dy, ldd, M, N, b) || (p && !matrix_ok(p, ldp, M, N, b)) || (act == ACT_RELU && (!save || lds < (N + 31) / 32 || (uintptr_t)save % 4))
+        || (act > ACT_RELU && !matrix_ok(save, lds, M, N, b)))
+      return dgnn_fail(DGNN_E_BADARG, "linear_slope: null, misaligned or overlapping rows%s");
+  }
+  const int64_t lanes = slope_lanes(N), slab = M > 0 ? slope_slab(M, N) : 1, slabs = ceil_div(M, slab);
+  if (dbias && slabs > 0 && (!workspace || workspace_bytes < slabs * N * 4 || (uintptr_t)workspace % 4))
+    return dgnn_fail(DGNN_E_BADARG, "linear_slope: workspace too small%s (%lld bytes wanted)", "", slabs * N * 4);
+  if (M > 0 && (p || dbias)) {
+    const Slope g{dy, save, p, ldd, lds, ldp, M, N, slab, dbias ? (float*)workspace : nullptr, act, (int)lanes};
+    const dim3 grid((uint32_t)ceil_div(N, 4 * lanes), (uint32_t)slabs);
+    if (dtype == DGNN_F32) hipLaunchKernelGGL((slope_kernel<float>), grid, dim3(256), 0, s, g);
+    else if (dtype == DGNN_BF16) hipLaunchKernelGGL((slope_kernel<__bf16>), grid, dim3(256), 0, s, g);
+    else hipLaunchKernelGGL((slope_kernel<_Float16>), grid, dim3(256), 0, s, g);
+    DGNN_LAUNCHED();
+  }
+  if (dbias) {
+    const dim3 grid((uint32_t)ceil_div(N, 16));
+    if (dtype == DGNN_F32) hipLaunchKernelGGL((slab_join_kernel<float>), grid, dim3(256), 0, s, (const float*)workspace, slabs, N, (float*)dbias);
+    else if (dtype == DGNN_BF16) hipLaunchKernelGGL((slab_join_kernel<__bf16>), grid, dim3(256), 0, s, (const float*)workspace, slabs, N, (__bf16*)dbias);
+    else hipLaunchKernelGGL((slab_join_kernel<_Float16>), grid, dim3(256), 0, s, (const float*)workspace, slabs, N, (_Float16*)dbias);
+    DGNN_LAUNCHED();
+  }
+  return DGNN_OK;
+}
+
+int dgnn_linear_grad_input(const void* p, int64_t ldp, const void* w, int64_t ldw, void* dx, int64_t ldx,
+                           int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!known_type(dtype)) return dgnn_fail(DGNN_E_BADARG, "linear_grad_input: unknown type%s (%lld)", "", dtype);
+  if (!sizes_ok(M, K, N)) return dgnn_fail(DGNN_E_BADARG, "linear_grad_input: bad sizes%s");
+  if (M == 0 || K == 0) return DGNN_OK;
+  const int64_t b = width(dtype);
+  if (!matrix_ok(p, ldp, M, N, b) || !matrix_ok(w, ldw, K, N, b) || !matrix_ok(dx, ldx, M, K, b))
+    return dgnn_fail(DGNN_E_BADARG, "linear_grad_input: null, misaligned or overlapping rows%s");
+  if (!apart(dx, ldx, M, K, p, ldp, M, N, b) || !apart(dx, ldx, M, K, w, ldw, K, N, b))
+    return dgnn_fail(DGNN_E_BADARG, "linear_grad_input: dx overlaps an input%s");
+  Gemm g{};
+  g.a = p; g.lda = ldp; g.a_along = true;
+  g.b = w; g.ldb = ldw; g.b_along = true;
+  g.M = M; g.N = K; g.K = N;
+  g.c = dx; g.ldc = ldx;
+  g.stream = (hipStream_t)stream;
+  return run(g, dtype, workspace, workspace_bytes, "linear_grad_input");
+}
+
+int dgnn_linear_grad_weight(const void* x, int64_t ldx, const void* p, int64_t ldp, void* dw, int64_t ldw,
+                            int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!known_type(dtype)) return dgnn_fail(DGNN_E_BADARG, "linear_grad_weight: unknown type%s (%lld)", "", dtype);
+  if (!sizes_ok(M, K, N)) return dgnn_fail(DGNN_E_BADARG, "linear_grad_weight: bad sizes%s");
+  if (K == 0 || N == 0) return DGNN_OK;
+  const int64_t b = width(dtype);
+  if (!matrix_ok(x, ldx, M, K, b) || !matrix_ok(p, ldp, M, N, b) || !matrix_ok(dw, ldw, K, N, b))
+    return dgnn_fail(DGNN_E_BADARG, "linear_grad_weight: null, misaligned or overlapping rows%s");
+  if (!apart(dw, ldw, K, N, x, ldx, M, K, b) || !apart(dw, ldw, K, N, p, ldp, M, N, b))
+    return dgnn_fail(DGNN_E_BADARG, "linear_grad_weight: dw overlaps an input%s");
+  Gemm g{};
+  g.a = x; g.lda = ldx; g.a_along = false;
+  g.b = p; g.ldb = ldp; g.b_along = false;
+  g.M = K; g.N = N; g.K = M;
+  g.c = dw; g.ldc = ldw;
+  g.stream = (hipStream_t)stream;
+  return run(g, dtype, workspace, workspace_bytes, "linear_grad_weight");
+}
+
+}  // extern "C"

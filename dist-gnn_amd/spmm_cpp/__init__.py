@@ -91,6 +91,11 @@ _SIGNATURES = {                          # argument types, in the order of inclu
     'dgnn_spmm_plan_overwrite_f32': [ctypes.POINTER(_CPlan), _p, _p, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _i32, _f32, _p],
 }
 _TRAIN_SIGNATURES = {                    # argument types, in the order of include/dgnn_train.h
+    'dgnn_linear_workspace': [_i32, _i64, _i64, _i64, _i32, _pi64],
+    'dgnn_linear_forward': [_p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _i32, _p, _i64, _p],
+    'dgnn_linear_slope': [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i32, _i32, _p, _i64, _p],
+    'dgnn_linear_grad_input': [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _p, _i64, _p],
+    'dgnn_linear_grad_weight': [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _p, _i64, _p],
     'dgnn_adamw': [_p, _i32, _i32, _i32, _p, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, _p],
 }
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}         # DGNN_F32, DGNN_BF16, DGNN_F16
@@ -1459,3 +1464,4 @@ def _dense_for(A):
 
 # --------------------------------------------------------------------------- what a training step computes beside the aggregation
 from .adamw import AdamW  # noqa: E402,F401
+from .linear import ACTIVATIONS, linear, linear_forward, linear_grad_input, linear_grad_weight, linear_slope  # noqa: E402,F401

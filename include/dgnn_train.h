@@ -18,6 +18,43 @@ extern "C" {
 #define DGNN_F16  2
 
 /*
+ * The layer transform  y = act(x W + b) + r  and its gradients. All matrices row-major with `ld*` elements between rows
+ * (>= the row's width) and element-aligned, of one type (DGNN_F32 | DGNN_BF16 | DGNN_F16): x [M x K], W [K x N], b [N] or
+ * NULL, r [M x N] or NULL, y [M x N]. Products and sums in fp32 (fp32 operands: six products of bf16 pieces, as close to
+ * the exact sum as a chain of fp32 operations), one rounding at the end. relu(NaN) is NaN.
+ *   act    DGNN_ACT_*: none, relu, gelu (0.5 t (1 + erf(t / sqrt 2))), silu (t / (1 + e^-t))
+ *   save   NULL, or what dgnn_linear_slope needs: for relu uint32 [M][lds], bit n % 32 of word n / 32 set where x W + b is
+ *          not <= 0 (lds >= ceil(N / 32), bits past N zero); for gelu and silu x W + b in the matrices' type (lds >= N)
+ * With a gradient dy of y:
+ *   dgnn_linear_slope         p = dy act'(x W + b) (p may be NULL), dbias[n] = sum over m of p[m][n] (may be NULL); p may be
+ *                             dy itself. act DGNN_ACT_NONE: p is a copy of dy
+ *   dgnn_linear_grad_input    dx = p W^T
+ *   dgnn_linear_grad_weight   dw = x^T p      (M = 0: zeros)
+ * workspace: device memory of dgnn_linear_workspace(pass, ...) bytes, 4-byte aligned (0 bytes: may be NULL), free to be used
+ * again once the call's kernels have run. Sums over many rows are cut by a rule of the sizes alone and joined in a fixed
+ * order: the same bits every run. Outputs must not overlap inputs (but p may be dy).
+ */
+#define DGNN_ACT_NONE 0
+#define DGNN_ACT_RELU 1
+#define DGNN_ACT_GELU 2
+#define DGNN_ACT_SILU 3
+#define DGNN_LINEAR_FORWARD     0   /* passes of dgnn_linear_workspace */
+#define DGNN_LINEAR_SLOPE       1
+#define DGNN_LINEAR_GRAD_INPUT  2
+#define DGNN_LINEAR_GRAD_WEIGHT 3
+int dgnn_linear_workspace(int32_t pass, int64_t M, int64_t K, int64_t N, int32_t dtype, int64_t* bytes);
+int dgnn_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                        const void* residual, int64_t ldr, void* y, int64_t ldy, void* save, int64_t lds,
+                        int64_t M, int64_t K, int64_t N, int32_t dtype, int32_t act,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+int dgnn_linear_slope(const void* dy, int64_t ldd, const void* save, int64_t lds, void* p, int64_t ldp, void* dbias,
+                      int64_t M, int64_t N, int32_t dtype, int32_t act, void* workspace, int64_t workspace_bytes, void* stream);
+int dgnn_linear_grad_input(const void* p, int64_t ldp, const void* w, int64_t ldw, void* dx, int64_t ldx,
+                           int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int dgnn_linear_grad_weight(const void* x, int64_t ldx, const void* p, int64_t ldp, void* dw, int64_t ldw,
+                            int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * One AdamW step over `count` tensors (a handful of launches for hundreds of them). With g a tensor's gradient, t the
  * number of its step:
  *     m <- b1 m + (1 - b1) g                 v <- b2 v + (1 - b2) g^2

@@ -1,0 +1,77 @@
+"""The layer transform's refusals: its C entries' checks (nothing is launched) and the binding's."""
+import ctypes
+
+import pytest
+import torch
+
+import spmm_cpp
+
+A, B, C, D = 1 << 22, 2 << 22, 3 << 22, 4 << 22             # addresses nobody reads: every call here is refused before a launch
+lib = spmm_cpp.lib
+
+
+def _forward(x=A, ldx=8, w=B, ldw=8, bias=None, res=None, ldr=0, y=C, ldy=8, save=None, lds=0, M=4, K=8, N=8, dtype=0, act=0, ws=None, n=0):
+    return lib.dgnn_linear_forward(x, ldx, w, ldw, bias, res, ldr, y, ldy, save, lds, M, K, N, dtype, act, ws, n, None)
+
+
+def _slope(dy=A, ldd=8, save=B, lds=8, p=C, ldp=8, db=None, M=4, N=8, dtype=0, act=2, ws=None, n=0):
+    return lib.dgnn_linear_slope(dy, ldd, save, lds, p, ldp, db, M, N, dtype, act, ws, n, None)
+
+
+def _grad_input(p=A, ldp=8, w=B, ldw=8, dx=C, ldx=8, M=4, K=8, N=8, dtype=0, ws=None, n=0):
+    return lib.dgnn_linear_grad_input(p, ldp, w, ldw, dx, ldx, M, K, N, dtype, ws, n, None)
+
+
+def _grad_weight(x=A, ldx=8, p=B, ldp=8, dw=C, ldw=8, M=4, K=8, N=8, dtype=0, ws=None, n=0):
+    return lib.dgnn_linear_grad_weight(x, ldx, p, ldp, dw, ldw, M, K, N, dtype, ws, n, None)
+
+
+@pytest.mark.parametrize('call,kw', [
+    (_forward, dict(dtype=3)), (_forward, dict(act=4)), (_forward, dict(act=-1)), (_forward, dict(M=-1)), (_forward, dict(K=1 << 31)),
+    (_forward, dict(x=None)), (_forward, dict(w=None)), (_forward, dict(y=None)), (_forward, dict(ldx=7)), (_forward, dict(ldw=7)),
+    (_forward, dict(ldy=7)), (_forward, dict(x=A + 2)), (_forward, dict(bias=A + 1)), (_forward, dict(res=D, ldr=7)),
+    (_forward, dict(y=A + 64)), (_forward, dict(y=B)), (_forward, dict(res=C + 32, ldr=8)), (_forward, dict(act=1, save=D, lds=0)),
+    (_forward, dict(act=2, save=D, lds=7)), (_forward, dict(M=1, K=4096, N=64, ldx=4096, ldw=64, ldy=64)),      # cut, no workspace
+    (_slope, dict(dtype=-1)), (_slope, dict(act=9)), (_slope, dict(save=None)), (_slope, dict(lds=7)), (_slope, dict(dy=None)),
+    (_slope, dict(ldp=7)), (_slope, dict(act=1, lds=0)), (_slope, dict(db=D)), (_slope, dict(db=D, ws=D, n=4)), (_slope, dict(db=D + 2)),
+    (_grad_input, dict(dtype=5)), (_grad_input, dict(p=None)), (_grad_input, dict(ldx=7)), (_grad_input, dict(dx=A)), (_grad_input, dict(N=-2)),
+    (_grad_weight, dict(dtype=5)), (_grad_weight, dict(x=None)), (_grad_weight, dict(ldw=7)), (_grad_weight, dict(dw=B)),
+    (_grad_weight, dict(M=1 << 31)), (_grad_weight, dict(M=100000, dw=1 << 40)),                                # cut, no workspace
+])
+def test_c_entries_refuse(call, kw):
+    assert call(**kw) == 1 and b'linear' in lib.dgnn_last_error()
+
+
+def test_c_entries_with_nothing_to_do():
+    assert _forward(M=0, x=None, y=None) == 0 and _forward(N=0, w=None, y=None) == 0 and _grad_input(M=0, p=None, dx=None) == 0
+    assert _grad_weight(K=0, x=None, dw=None) == 0 and _slope(N=0, dy=None, save=None, p=None) == 0 and _slope(M=0, dy=None, save=None, p=None) == 0
+
+
+def test_workspace_is_bounded():
+    """Only products with fewer tiles than compute units are cut, so the partial sums stay under 256 tiles of 128 x 256 floats."""
+    n = ctypes.c_int64()
+    for kind in range(4):
+        for M in (0, 1, 7, 33, 2708, 232965, 2449029):
+            for K in (0, 1, 100, 602, 4096):
+                for N in (0, 1, 16, 41, 256, 4096):
+                    for dtype in range(3):
+                        assert lib.dgnn_linear_workspace(kind, M, K, N, dtype, ctypes.byref(n)) == 0
+                        assert 0 <= n.value <= (256 * 128 * 256 * 4 if kind != 1 else 4096 * max(N, 1) * 4)
+    assert lib.dgnn_linear_workspace(4, 1, 1, 1, 0, ctypes.byref(n)) == 1
+    assert lib.dgnn_linear_workspace(0, -1, 1, 1, 0, ctypes.byref(n)) == 1
+    assert lib.dgnn_linear_workspace(0, 1, 1, 1, 0, None) == 1
+
+
+def test_binding_refuses_cpu_tensors_and_other_things():
+    x, w = torch.zeros(3, 4), torch.zeros(4, 5)
+    with pytest.raises(RuntimeError, match='no CPU path'):
+        spmm_cpp.linear(x, w)
+    with pytest.raises(RuntimeError, match='no CPU path'):
+        spmm_cpp.linear(x.requires_grad_(True), w)
+    with pytest.raises(RuntimeError, match='must be a torch.Tensor'):
+        spmm_cpp.linear([[1.0]], w)
+    for f in (spmm_cpp.linear_grad_input, spmm_cpp.linear_grad_weight):
+        with pytest.raises(RuntimeError, match='no CPU path'):
+            f(x, w)
+    with pytest.raises(RuntimeError, match='no CPU path'):
+        spmm_cpp.linear_slope(x.detach(), None, 'none')

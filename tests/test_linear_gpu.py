@@ -1,0 +1,388 @@
+"""The layer transform against its definition in 64 bits.
+
+Bounds, with h = eps / 2 of the type (2^-24, bf16 2^-8, fp16 2^-11) and S = sum of |products|:
+  sums        the fp32 accumulation of K products in 16s: at most (10 + 12 K / 16) 2^-24 S (six products an fp32 pair, each
+              addition rounded once or truncated), a sixth of the K part for 16-bit operands; n additions of a column sum: n 2^-24 S
+  result      h |result| on top
+  activation  |act'| <= 1.13, |act''| <= 0.8; its own evaluation 16 2^-24 (|act| + |argument|)
+  slope       what is saved of x W + b is rounded once: 0.8 (h |pre| + its error) |dy|, and relu's bit may be either where
+              |pre| is within its error; p is rounded once more (h |p|) before the products
+"""
+import itertools
+
+import numpy as np
+import pytest
+import torch
+
+import spmm_cpp
+
+pytestmark = pytest.mark.gpu
+
+DT = {'f32': torch.float32, 'bf16': torch.bfloat16, 'f16': torch.float16}
+HALF = {k: torch.finfo(t).eps / 2 for k, t in DT.items()}
+U = 2.0 ** -24
+SIZES = [(1, 1, 1), (1, 602, 256), (2, 3, 5), (7, 4096, 130), (33, 17, 31), (31, 64, 32), (64, 1433, 16), (129, 40, 41), (257, 602, 256),
+         (128, 256, 257), (300, 33, 300), (1000, 7, 64), (4099, 100, 47), (20000, 31, 129)]
+
+
+def _inputs(m, k, n, dtype, bias, residual, seed, pad=0):
+    gen = torch.Generator(device='cuda').manual_seed(seed)
+
+    def t(*shape):
+        wide = torch.full(shape[:-1] + (shape[-1] + pad,), float('nan'), device='cuda')          # what lies between rows is not a value
+        wide[..., :shape[-1]] = torch.randn(*shape, generator=gen, device='cuda')
+        return wide.to(DT[dtype])[..., :shape[-1]]
+    x, w, dy = t(m, k), t(k, n), t(m, n)
+    b = torch.randn(n, generator=gen, device='cuda').to(DT[dtype]) if bias else None
+    return x, w, b, t(m, n) if residual else None, dy
+
+
+def _d(t):
+    return None if t is None else t.detach().double().cpu()
+
+
+def _sum_bound(k, dtype):
+    return (10 + (12 if dtype == 'f32' else 2) * k / 16) * U
+
+
+def _act(a, act):
+    if act == 'relu':
+        return a.clamp_min(0), (a > 0).double()
+    if act == 'gelu':
+        cdf = 0.5 * torch.special.erfc(-a / 2 ** 0.5)
+        return a * cdf, cdf + a * torch.exp(-a * a / 2) / (2 * np.pi) ** 0.5
+    if act == 'silu':
+        s = torch.sigmoid(a)
+        return a * s, s * (1 + a * (1 - s))
+    return a, torch.ones_like(a)
+
+
+def _near(got, want, bound, name):
+    off = (_d(got) - want).abs()
+    assert got.shape == want.shape, name
+    assert bool((off <= bound).all()), f'{name}: {float((off / bound.clamp_min(1e-300)).max()):.3g} times its bound'
+
+
+def _definition(x, w, b, r, dy, dtype, act):
+    """{name: (value, bound)} of the output and the gradients."""
+    h, (x, w, b, r, dy) = HALF[dtype], map(_d, (x, w, b, r, dy))
+    (m, k), n = x.shape, w.shape[1]
+    pre, size = x @ w, x.abs() @ w.abs()
+    if b is not None:
+        pre, size = pre + b, size + b.abs()
+    e_pre = _sum_bound(k, dtype) * size + U * pre.abs()
+    y, slope = _act(pre, act)
+    e_y = 1.13 * e_pre + 16 * U * (y.abs() + pre.abs())
+    if r is not None:
+        y = y + r
+        e_y = e_y + U * y.abs()
+    out = {'y': (y, e_y + h * y.abs() + 1e-40 + (2.0 ** -25 if dtype == 'f16' else 0))}
+    p = dy * slope
+    if act == 'none':
+        e_p = torch.zeros_like(p)
+    elif act == 'relu':
+        e_p = dy.abs() * (pre.abs() <= e_pre)
+    else:
+        e_p = dy.abs() * (0.8 * (h * pre.abs() + 2 * e_pre) + 16 * U * (1 + pre.abs()))
+    tiny = 2.0 ** -25 if dtype == 'f16' else 0               # fp16's smallest half step
+    e_round = e_p + (h * (p.abs() + e_p) + tiny if act in ('gelu', 'silu') else 0)
+    for name, a, c, e, count in (('dx', p, w.t(), None, n), ('dw', x.t(), p, None, m)):
+        v = a @ c
+        e = (e_round @ w.abs().t()) if name == 'dx' else (x.abs().t() @ e_round)
+        e = e + _sum_bound(count, dtype) * (a.abs() @ c.abs() + e)
+        out[name] = (v, e + h * v.abs() + 1e-40 + tiny)
+    v = p.sum(0)
+    e = e_p.sum(0) + (m + 2) * U * (p.abs() + e_p).sum(0)
+    out['db'] = (v, e + h * v.abs() + 1e-40 + tiny)
+    out['dr'] = (dy, torch.zeros_like(dy))
+    return out
+
+
+def _run(x, w, b, r, dy, act):
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b, r) if t is not None]
+    it = iter(leaves)
+    xl, wl = next(it), next(it)
+    bl = next(it) if b is not None else None
+    rl = next(it) if r is not None else None
+    y = spmm_cpp.linear(xl, wl, bl, activation=act, residual=rl)
+    names = ['dx', 'dw'] + (['db'] if b is not None else []) + (['dr'] if r is not None else [])
+    return {'y': y.detach(), **dict(zip(names, torch.autograd.grad(y, leaves, dy)))}
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+@pytest.mark.parametrize('m,k,n', SIZES)
+def test_output_and_gradients(m, k, n, dtype):
+    for i, act in enumerate(('none', 'relu', 'gelu', 'silu')):
+        case = _inputs(m, k, n, dtype, i != 1, i >= 1, seed=m * 7 + n, pad=(0, 3, 8, 1)[i])
+        want = _definition(*case, dtype, act)
+        mine = _run(*case, act)
+        for name, got in mine.items():
+            assert got.dtype == DT[dtype]
+            _near(got, *want[name], f'{act} {name}')
+        assert torch.equal(spmm_cpp.linear(case[0], case[1], case[2], act, case[3]), mine['y'])      # saving nothing: the same bits
+
+
+@pytest.mark.parametrize('m,k,n', [(0, 5, 4), (3, 0, 4), (3, 5, 0), (0, 0, 0), (1, 0, 1)])
+def test_empty_sides(m, k, n):
+    for dtype, act in itertools.product(DT, ('none', 'relu', 'silu')):
+        case = _inputs(m, k, n, dtype, True, True, seed=1)
+        want = _definition(*case, dtype, act)
+        for name, got in _run(*case, act).items():
+            _near(got, *want[name], f'{act} {name}')
+
+
+def test_fp32_is_as_exact_as_fp32_arithmetic():
+    """The error against 64 bits is at most twice that of a plain chain of fp32 operations, over all outputs, for operands of
+    ordinary size, of mixed sizes and with sums that cancel."""
+    for seed, (m, k, n) in enumerate([(64, 8, 40), (64, 602, 64), (40, 4096, 300)]):
+        x, w, _, _, _ = _inputs(m, k, n, 'f32', False, False, seed)
+        for kind in ('plain', 'mixed', 'cancel'):
+            if kind == 'mixed':
+                x = x * torch.exp2(torch.randint(-20, 20, x.shape, device='cuda').float())
+            if kind == 'cancel':
+                x, w = torch.cat([x, x], 1), torch.cat([w, -w * (1 + 2.0 ** -10)], 0)
+            want = _d(x) @ _d(w)
+            xn, wn = x.cpu().numpy(), w.cpu().numpy()
+            acc = np.zeros((m, n), np.float32)
+            for i in range(x.shape[1]):
+                acc += xn[:, i:i + 1] * wn[i]
+            chain = float((torch.from_numpy(acc).double() - want).norm())
+            mine = float((_d(spmm_cpp.linear(x, w)) - want).norm())
+            assert mine <= 2 * chain, (kind, mine / chain)
+
+
+def test_fp32_values_that_are_not_finite_or_near_the_edge():
+    m, k, n = 70, 64, 80
+    x, w, _, _, _ = _inputs(m, k, n, 'f32', False, False, 3)
+    inf, big = float('inf'), 3.4e38
+    x[3, 5], x[7, 1], x[9, 0], x[9, 1] = inf, -inf, inf, float('nan')
+    x[12], w[:, 9] = 0, 0                                     # inf * 0 where row 3 meets column 9
+    w[5, 11] = 0
+    x[20] = 0
+    x[20, 4] = big                                            # rounds to infinity in 8 bits
+    w[:, 30] = 0
+    w[4, 30] = 1.0
+    w[2, 40] = inf
+    for y, (a, b) in ((spmm_cpp.linear(x, w), (x, w)), (spmm_cpp.linear_grad_weight(x.t().contiguous(), w), (x, w)),
+                      (spmm_cpp.linear_grad_input(x, w.t().contiguous()), (x, w))):
+        want = (_d(a).unsqueeze(2) * _d(b).unsqueeze(0)).sum(1)        # the products as they are: inf * 0 is NaN
+        want = want.float()                                            # and what passes fp32's range is infinity
+        got = y.cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+        assert torch.equal(got[torch.isinf(got)], want[torch.isinf(want)])
+        assert float(got[20, 30]) == float(torch.tensor(big))
+        fine = torch.isfinite(want)
+        assert torch.allclose(got[fine], want[fine], rtol=2e-5, atol=0.01)
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+def test_16_bit_values_that_are_not_finite(dtype):
+    x, w, _, r, _ = _inputs(40, 64, 48, dtype, False, True, 4)
+    x[3, 5], x[9, 1], r[11, 2] = float('inf'), float('nan'), float('nan')
+    y = spmm_cpp.linear(x, w, None, 'relu', r)
+    want = (_d(x).unsqueeze(2) * _d(w).unsqueeze(0)).sum(1)
+    want = torch.where(want <= 0, torch.zeros_like(want), want) + _d(r)
+    assert torch.equal(torch.isnan(y).cpu(), torch.isnan(want)) and torch.equal(torch.isinf(y).cpu(), torch.isinf(want))
+
+
+def test_small_fp32_values():
+    """Values of 2^-110 keep an absolute error of 2^-134 a unit of the other operand (bf16's smallest number is 2^-133)."""
+    x, w, _, _, _ = _inputs(20, 40, 30, 'f32', False, False, 5)
+    x = x * 2.0 ** -110
+    want = _d(x) @ _d(w)
+    bound = _sum_bound(40, 'f32') * (_d(x).abs() @ _d(w).abs()) + 3 * 2.0 ** -134 * _d(w).abs().sum(0)
+    assert bool(((_d(spmm_cpp.linear(x, w)) - want).abs() <= bound).all())
+
+
+def test_gradients_against_differences():
+    """d loss along a random direction, from differences of the 64-bit definition at +-1e-6."""
+    for act in ('gelu', 'silu', 'none'):
+        x, w, b, r, dy = _inputs(37, 50, 45, 'f32', True, True, 6)
+        g = _run(x, w, b, r, dy, act)
+        gen = torch.Generator().manual_seed(1)
+        for name, t in (('dx', x), ('dw', w), ('db', b), ('dr', r)):
+            step = torch.randn(t.shape, generator=gen, dtype=torch.float64)
+
+            def loss(e):
+                args = [_d(x), _d(w), _d(b), _d(r)]
+                args[('dx', 'dw', 'db', 'dr').index(name)] += e * step
+                return float(((_act(args[0] @ args[1] + args[2], act)[0] + args[3]) * _d(dy)).sum())
+            want = (loss(1e-6) - loss(-1e-6)) / 2e-6
+            got = float((_d(g[name]) * step).sum())
+            assert abs(got - want) <= 1e-4 * float((_d(g[name]).abs() * step.abs()).sum()), (act, name)
+
+
+def test_only_what_is_asked_for():
+    x, w, b, r, dy = _inputs(50, 20, 30, 'f32', True, True, 7)
+    full = _run(x, w, b, r, dy, 'relu')
+    for which in ('x', 'w', 'b', 'r'):
+        ts = {'x': x.clone(), 'w': w.clone(), 'b': b.clone(), 'r': r.clone()}
+        ts[which].requires_grad_(True)
+        y = spmm_cpp.linear(ts['x'], ts['w'], ts['b'], 'relu', ts['r'])
+        got, = torch.autograd.grad(y, ts[which], dy)
+        assert torch.equal(got, full['d' + which])
+    w = w.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError):                         # no second derivative
+        g, = torch.autograd.grad(spmm_cpp.linear(x, w).sum(), w, create_graph=True)
+        g.sum().backward()
+
+
+def test_gradients_that_are_expanded_or_transposed():
+    x, w, _, r, _ = _inputs(40, 24, 40, 'f32', False, True, 8)
+    x.requires_grad_(True)
+    y = spmm_cpp.linear(x, w, None, 'silu', r)
+    a, = torch.autograd.grad(y.sum(), x)
+    y = spmm_cpp.linear(x, w, None, 'silu', r)
+    b, = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert torch.equal(a, b)
+    y = spmm_cpp.linear(x, w, None, 'silu', r)
+    t = torch.randn(40, 40, device='cuda')
+    c, = torch.autograd.grad(y.t(), x, t)
+    y = spmm_cpp.linear(x, w, None, 'silu', r)
+    d, = torch.autograd.grad(y, x, t.t().contiguous())
+    assert torch.equal(c, d)
+
+
+def test_columns_between_rows_are_left_alone():
+    """The C entries write rows of any distance and nothing between them."""
+    x, w, b, r, dy = _inputs(100, 40, 70, 'f32', True, True, 9)
+    y, saved = spmm_cpp.linear_forward(x, w, b, 'silu', r, save=True)
+    p, db = spmm_cpp.linear_slope(dy, saved, 'silu')
+    dx, dw = spmm_cpp.linear_grad_input(p, w), spmm_cpp.linear_grad_weight(x, p)
+    lib, s = spmm_cpp.lib, spmm_cpp._stream(x)
+
+    def room(m, n):
+        return torch.full((m + 1, n + 5), 7.0, device='cuda')
+    ws = torch.empty(1 << 22, device='cuda')
+    Y, P, X, W = room(100, 70), room(100, 70), room(100, 40), room(40, 70)
+    assert lib.dgnn_linear_forward(x.data_ptr(), 40, w.data_ptr(), 70, b.data_ptr(), r.data_ptr(), 70, Y.data_ptr(), 75, None, 0,
+                                   100, 40, 70, 0, 3, ws.data_ptr(), ws.numel() * 4, s) == 0
+    assert lib.dgnn_linear_slope(dy.data_ptr(), 70, saved.data_ptr(), 70, P.data_ptr(), 75, None, 100, 70, 0, 3, None, 0, s) == 0
+    assert lib.dgnn_linear_grad_input(p.data_ptr(), 70, w.data_ptr(), 70, X.data_ptr(), 45, 100, 40, 70, 0, ws.data_ptr(), ws.numel() * 4, s) == 0
+    assert lib.dgnn_linear_grad_weight(x.data_ptr(), 40, p.data_ptr(), 70, W.data_ptr(), 75, 100, 40, 70, 0, ws.data_ptr(), ws.numel() * 4, s) == 0
+    for big, small in ((Y, y), (P, p), (X, dx), (W, dw)):
+        m, n = small.shape
+        assert torch.equal(big[:m, :n], small)
+        assert bool((big[m:] == 7).all()) and bool((big[:, n:] == 7).all())
+
+
+def test_refusals_on_the_device():
+    x, w, b, r, _ = _inputs(6, 4, 5, 'f32', True, True, 10)
+    for kw in (dict(x=x.t()), dict(x=x.half()), dict(x=x.double()), dict(x=x[0]), dict(w=w.bfloat16()), dict(w=w[:3]), dict(b=b[:4]),
+               dict(b=b.half()), dict(b=b.view(1, 5)), dict(r=r[:5]), dict(r=r[:1].expand(6, 5)), dict(act='tanh'), dict(act=None),
+               dict(x=x[:1].expand(6, 4)), dict(w=w.cpu())):
+        a = {**dict(x=x, w=w, b=b, r=r, act='relu'), **kw}
+        with pytest.raises(RuntimeError, match='spmm_cpp.linear'):
+            spmm_cpp.linear(a['x'], a['w'], a['b'], a['act'], a['r'])
+    y, saved = spmm_cpp.linear_forward(x, w, b, 'gelu', r, save=True)
+    for bad in (None, saved[:3], saved.half(), saved.t()):
+        with pytest.raises(RuntimeError, match='saved'):
+            spmm_cpp.linear_slope(y, bad, 'gelu')
+    with pytest.raises(RuntimeError, match='shape'):
+        spmm_cpp.linear_grad_weight(x, y[:5])
+    with pytest.raises(RuntimeError, match='shape'):
+        spmm_cpp.linear_grad_input(x, w)
+
+
+@pytest.mark.parametrize('dtype,act,shape', [('f32', 'relu', (300, 602, 41)), ('bf16', 'gelu', (5, 600, 256)), ('f32', 'silu', (5000, 64, 64))])
+def test_captured_and_replayed(dtype, act, shape):
+    """Forward and backward captured twice, replayed with new inputs between eager work, the two graphs on two streams at once."""
+    cases = [_inputs(*shape, dtype, True, True, seed) for seed in (11, 12)]
+    graphs, outs = [], []
+    leaves = [[t.clone().requires_grad_(True) for t in c[:4]] for c in cases]
+
+    def work(l, dy):
+        y = spmm_cpp.linear(l[0], l[1], l[2], act, l[3])
+        return (y.detach(),) + torch.autograd.grad(y, l, dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work(leaves[0], cases[0][4])
+    torch.cuda.current_stream().wait_stream(side)
+    for l, c in zip(leaves, cases):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(work(l, c[4]))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(3):
+        with torch.no_grad():
+            for l in leaves:
+                for t in l:
+                    t.add_(0.25)
+        want = [work(l, c[4]) for l, c in zip(leaves, cases)]
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                for _ in range(3):
+                    g.replay()
+        torch.cuda.synchronize()
+        for o, e in zip(outs, want):
+            for a, b in zip(o, e):
+                assert torch.equal(a, b), turn
+
+
+def test_two_streams_at_once():
+    """Calls that cut their sums, on two streams: each has a workspace of its own."""
+    cases = [_inputs(9, 4096, 200, 'f32', True, False, seed) for seed in (13, 14)]
+    want = [spmm_cpp.linear(x, w, b, 'gelu') for x, w, b, _, _ in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                x, w, b, _, _ = cases[i]
+                got[i].append(spmm_cpp.linear(x, w, b, 'gelu'))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, t) for t in g)
+
+
+def test_offsets_past_32_bits():
+    """Rows more than 2^32 bytes behind the first: 2^21 rows 1100 floats apart, the last ones checked."""
+    m, k, n = 1 << 21, 40, 33
+    buf = torch.zeros(m, 1100, device='cuda')
+    x = buf[:, :k]
+    gen = torch.Generator(device='cuda').manual_seed(0)
+    tail = torch.randn(200, k, generator=gen, device='cuda')
+    x[-200:] = tail
+    w = torch.randn(k, n, generator=gen, device='cuda')
+    y = spmm_cpp.linear(x, w)
+    assert torch.equal(y[-200:], spmm_cpp.linear(tail, w)) and not bool(y[:-200].any())
+    p = torch.zeros(m, n, device='cuda')
+    p[-200:] = 1.0
+    dw = spmm_cpp.linear_grad_weight(x, p)
+    want = _d(tail).sum(0).unsqueeze(1).expand(k, n)
+    assert bool(((_d(dw) - want).abs() <= _sum_bound(200, 'f32') * _d(tail).abs().sum(0).unsqueeze(1) + U * want.abs()).all())
+
+
+def test_a_training_run_of_both_operators():
+    """Layers and optimiser as they are used together: two layers, three steps, against the same in 64 bits. Each step moves a
+    weight by at most about lr and gradients agree to 1e-5, so weights agree to 1e-4 lr; where a gradient is within rounding
+    of zero its step's direction is noise, which is why weights with tiny gradients are left out."""
+    gen = torch.Generator(device='cuda').manual_seed(3)
+    x = torch.randn(500, 30, generator=gen, device='cuda')
+    target = torch.randn(500, 6, generator=gen, device='cuda')
+    shapes = [(30, 30), (30,), (30, 6), (6,)]
+    ps = [torch.nn.Parameter(0.2 * torch.randn(*s, generator=gen, device='cuda')) for s in shapes]
+    qs = [p.detach().double().cpu().requires_grad_(True) for p in ps]
+    opt = spmm_cpp.AdamW(ps, lr=0.01, weight_decay=0.1, eps=1e-4)
+    ref = torch.optim.AdamW(qs, lr=0.01, weight_decay=0.1, eps=1e-4)
+    xd, td = x.double().cpu(), target.double().cpu()
+    for _ in range(3):
+        h = spmm_cpp.linear(x, ps[0], ps[1], 'gelu', residual=x)
+        y = spmm_cpp.linear(h, ps[2], ps[3])
+        loss = (y - target).square().mean()
+        opt.zero_grad()
+        loss.backward()
+        opt.step()
+        hd = torch.nn.functional.gelu(xd @ qs[0] + qs[1]) + xd
+        ld = (hd @ qs[2] + qs[3] - td).square().mean()
+        ref.zero_grad()
+        ld.backward()
+        ref.step()
+        assert abs(float(loss) - float(ld)) < 1e-5 * float(ld)
+    for p, q in zip(ps, qs):
+        # a step is lr g / (|g| + eps)-like: its slope in g is at most lr / eps = 100, gradients are off by < 1e-7
+        assert float((p.double().cpu() - q).abs().max()) < 3 * 100 * 1e-7 + 1e-6
