@@ -262,20 +262,22 @@ int dgnn_linear_slope(const void* dy, int64_t ldd, const void* save, int64_t lds
   return DGNN_OK;
 }
 
-int dgnn_linear_grad_input(const void* p, int64_t ldp, const void* w, int64_t ldw, void* dx, int64_t ldx,
-                           int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+int dgnn_linear_grad_input(const void* p, int64_t ldp, const void* w, int64_t ldw, const void* add, int64_t lda,
+                           void* dx, int64_t ldx, int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!known_type(dtype)) return dgnn_fail(DGNN_E_BADARG, "linear_grad_input: unknown type%s (%lld)", "", dtype);
   if (!sizes_ok(M, K, N)) return dgnn_fail(DGNN_E_BADARG, "linear_grad_input: bad sizes%s");
   if (M == 0 || K == 0) return DGNN_OK;
   const int64_t b = width(dtype);
-  if (!matrix_ok(p, ldp, M, N, b) || !matrix_ok(w, ldw, K, N, b) || !matrix_ok(dx, ldx, M, K, b))
+  if (!matrix_ok(p, ldp, M, N, b) || !matrix_ok(w, ldw, K, N, b) || !matrix_ok(dx, ldx, M, K, b)
+      || (add && !matrix_ok(add, lda, M, K, b)))
     return dgnn_fail(DGNN_E_BADARG, "linear_grad_input: null, misaligned or overlapping rows%s");
-  if (!apart(dx, ldx, M, K, p, ldp, M, N, b) || !apart(dx, ldx, M, K, w, ldw, K, N, b))
+  if (!apart(dx, ldx, M, K, p, ldp, M, N, b) || !apart(dx, ldx, M, K, w, ldw, K, N, b) || !apart(dx, ldx, M, K, add, lda, M, K, b))
     return dgnn_fail(DGNN_E_BADARG, "linear_grad_input: dx overlaps an input%s");
   Gemm g{};
   g.a = p; g.lda = ldp; g.a_along = true;
   g.b = w; g.ldb = ldw; g.b_along = true;
   g.M = M; g.N = K; g.K = N;
+  g.residual = add; g.ld_residual = lda;
   g.c = dx; g.ldc = ldx;
   g.stream = (hipStream_t)stream;
   return run(g, dtype, workspace, workspace_bytes, "linear_grad_input");

@@ -46,9 +46,12 @@ def cross_entropy_mean(outputs, target):
     return -torch.log_softmax(outputs, 1).gather(1, target.unsqueeze(1)).mean()
 
 
-def build_model(g, env, model='GCN', hidden_dim=256, num_layers=3, rep=2):
+def build_model(g, env, model='GCN', hidden_dim=256, num_layers=3, rep=2, bias=False, activation='relu', skip=False):
+    """``bias``, ``activation`` and ``skip`` are options of GCN and GCN15D (models/gcn.py); the others are the reference's."""
     if model == 'GCN':
-        return GCN(g, env, hidden_dim=hidden_dim, num_layers=num_layers)
+        return GCN(g, env, hidden_dim=hidden_dim, num_layers=num_layers, bias=bias, activation=activation, skip=skip)
+    if model in ('CachedGCN', 'AdaptiveGCN') and (bias or skip or activation != 'relu'):
+        raise ValueError(f'{model} has no bias, activation or skip option (GCN | GCN15D do)')
     if model == 'CachedGCN':
         return CachedGCN(g, env, hidden_dim=hidden_dim)
     if model == 'AdaptiveGCN':       # 1D_CAGNET/dist_1d.py: 2 layers, log_softmax output (pair it with nll_loss)
@@ -56,8 +59,20 @@ def build_model(g, env, model='GCN', hidden_dim=256, num_layers=3, rep=2):
         return AdaptiveGCN(g, env, hidden_dim=hidden_dim)
     if model == 'GCN15D':            # 1D_CAGNET/dist_15d.py: g is row block rank // rep of world_size // rep
         from models import GCN15D
-        return GCN15D(g, env, hidden_dim=hidden_dim, num_layers=num_layers, rep=rep)
+        return GCN15D(g, env, hidden_dim=hidden_dim, num_layers=num_layers, rep=rep, bias=bias, activation=activation, skip=skip)
     raise ValueError(f'unknown model {model!r} (GCN | CachedGCN | AdaptiveGCN | GCN15D)')
+
+
+def build_optimizer(params, optimizer='adam', lr=0.01, weight_decay=0.0):
+    """'adam': the reference's torch.optim.Adam (dist_train.py:32); 'adamw' / 'adamw8': spmm_cpp.AdamW, one pass a step, with
+    moments in 32 or 8 bits. Every rank steps its own copy; sums are in a fixed order and the 8-bit rounding depends on element
+    and step alone, so copies stay equal."""
+    if optimizer == 'adam':
+        return torch.optim.Adam(params, lr=lr, weight_decay=weight_decay)
+    if optimizer in ('adamw', 'adamw8'):
+        import spmm_cpp
+        return spmm_cpp.AdamW(params, lr=lr, weight_decay=weight_decay, state_bits=8 if optimizer == 'adamw8' else 32)
+    raise ValueError(f'unknown optimizer {optimizer!r} (adam | adamw | adamw8)')
 
 
 def train_step(model, optimizer, loss_func, g, env):
@@ -82,21 +97,23 @@ def train_step(model, optimizer, loss_func, g, env):
     return outputs, loss
 
 
-def train(g, env, total_epoch, model='GCN', hidden_dim=256, num_layers=3, lr=0.01, eval_every=10):
+def train(g, env, total_epoch, model='GCN', hidden_dim=256, num_layers=3, lr=0.01, eval_every=10, optimizer='adam',
+          weight_decay=0.0, **model_options):
+    """``model_options``: bias, activation, skip (build_model)."""
     # The X W products stay on PyTorch's default BLAS library unless DGNN_TUNE_GEMM=1|library asks for the per-shape
     # choice (dist_utils/gemm.py): a timing race decides it, so the default run reproduces bits like the reference's
     # plain torch.mm. Only with real GPUs per rank (nccl): under the gloo rehearsal the ranks share one card.
     tuned = tune_gemms() if (env.device.type == 'cuda' and getattr(env, 'backend', 'nccl') == 'nccl') else False
     try:
-        return _train(g, env, total_epoch, model, hidden_dim, num_layers, lr, eval_every)
+        return _train(g, env, total_epoch, model, hidden_dim, num_layers, lr, eval_every, optimizer, weight_decay, model_options)
     finally:
         if tuned:
             gemm.restore()           # PyTorch's global BLAS settings as the caller had them
 
 
-def _train(g, env, total_epoch, model, hidden_dim, num_layers, lr, eval_every):
-    net = build_model(g, env, model, hidden_dim, num_layers)
-    optimizer = torch.optim.Adam(net.parameters(), lr=lr)
+def _train(g, env, total_epoch, model, hidden_dim, num_layers, lr, eval_every, optimizer, weight_decay, model_options):
+    net = build_model(g, env, model, hidden_dim, num_layers, **model_options)
+    optimizer = build_optimizer(net.parameters(), optimizer, lr, weight_decay)
     loss_func = cross_entropy_mean if g.labels.dim() == 1 else nn.BCEWithLogitsLoss(reduction='mean')
     losses = []
     for epoch in range(total_epoch):
@@ -115,5 +132,7 @@ def main(env, args):
         g = Parted_COO_Graph(args.dataset, rank=env.rank, num_parts=env.world_size, device=env.device)
         env.logger.log('graph loaded', g)
         train(g, env, total_epoch=args.epoch, model=getattr(args, 'model', 'GCN'),
-              hidden_dim=getattr(args, 'hidden', 256), num_layers=getattr(args, 'layers', 3))
+              hidden_dim=getattr(args, 'hidden', 256), num_layers=getattr(args, 'layers', 3), lr=getattr(args, 'lr', 0.01),
+              optimizer=getattr(args, 'optimizer', 'adam'), weight_decay=getattr(args, 'weight_decay', 0.0), bias=getattr(args, 'bias', False),
+              activation=getattr(args, 'activation', 'relu'), skip=getattr(args, 'skip', False))
     env.logger.log(env.timer.summary_all(), rank=0)

@@ -37,6 +37,12 @@ def parse_args(argv=None):
     ap.add_argument('--model', type=str, default='GCN', choices=['GCN', 'CachedGCN'])
     ap.add_argument('--hidden', type=int, default=256)
     ap.add_argument('--layers', type=int, default=3)
+    ap.add_argument('--lr', type=float, default=0.01)
+    ap.add_argument('--optimizer', type=str, default='adam', choices=['adam', 'adamw', 'adamw8'])
+    ap.add_argument('--weight-decay', type=float, default=0.0)
+    ap.add_argument('--bias', action='store_true')
+    ap.add_argument('--activation', type=str, default='relu', choices=['none', 'relu', 'gelu', 'silu'])
+    ap.add_argument('--skip', action='store_true')
     ap.add_argument('--port', type=int, default=29500)
     return ap.parse_args(argv)
 

@@ -25,15 +25,25 @@ from dist_utils import DistEnv, gemm as _gemm
 
 _spmm_override = None          # tests install the CPU oracle here to exercise the pipeline on gloo
 _gather_override = None
+_dense_override = None
 
 
-def set_spmm_backend(fn, gather=None):
+def set_spmm_backend(fn, gather=None, dense=None):
     """Replace the SpMM used by the pipeline (``fn(A_sparse_coo, B, C)`` doing C += A @ B in place) and,
-    optionally, the row gather of the needed-rows transfer (``gather(src, idx_int32, dst)``).
+    optionally, the row gather of the needed-rows transfer (``gather(src, idx_int32, dst)``) and the layer transform
+    (``dense``: an object with spmm_cpp's linear_forward, linear_slope, linear_grad_input and linear_grad_weight).
     ``None`` restores the HIP operators. Test hook: the product never installs a fallback itself."""
-    global _spmm_override, _gather_override
+    global _spmm_override, _gather_override, _dense_override
     _spmm_override = fn
     _gather_override = gather
+    _dense_override = dense
+
+
+def _dense():
+    if _dense_override is not None:
+        return _dense_override
+    import spmm_cpp
+    return spmm_cpp
 
 
 def _trace(*a):
@@ -999,19 +1009,90 @@ def aggregation_layer(name, aggregate, forward_tag=lambda t: 'Forward' + t, back
     return Layer
 
 
+def epilogue_layer(name, aggregate, reduce_grad=None):
+    """The layer of gcn.py:33-53 with bias, activation and skip connection in its product:
+    ``out = act((A_hat H) W + b) + H`` (the last term only with ``skip``) on the operators of spmm_cpp.linear, one pass over
+    the aggregated features instead of a product and an elementwise pass for each of the others.
+
+    Backward, with G the gradient of out and P = G act'(...): the bias gets P's column sums, and the layer's own formulas
+    hold for P -- aggregate it with the same (or the transposed) blocks, ``ag W^T`` (plus G through the skip connection, in
+    the same product), ``H^T ag``; the sums over the ranks are ``reduce_grad``'s. DGNN_WGRAD_FROM_Z applies as in
+    DistGCNLayer; DGNN_TRANSFORM_FIRST does not (the activation follows the aggregation)."""
+
+    class Layer(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, features, weight, bias, adj_parts, tag, activation, skip):
+            if skip and weight.size(0) != weight.size(1):
+                raise RuntimeError(f'{name}: a skip connection needs a square weight, got {tuple(weight.shape)}')
+            z_local = aggregate(adj_parts, features, 'Forward' + tag)
+            with DistEnv.env.timer.timing_cuda('mm'):
+                out, saved = _dense().linear_forward(z_local, weight, bias, activation, features if skip else None,
+                                                     save=any(ctx.needs_input_grad[:3]))
+            keep_z = wgrad_from_z() and not ctx.needs_input_grad[0]
+            ctx.save_for_backward(features, weight, saved, z_local if keep_z else None)
+            ctx.adj_parts, ctx.tag, ctx.activation, ctx.skip = adj_parts, tag, activation, skip
+            return out
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad_output):
+            features, weight, saved, z_local = ctx.saved_tensors
+            timer, dense, reduce = DistEnv.env.timer, _dense(), reduce_grad or DistEnv.env.all_reduce_sum
+            grad_output = grad_output.contiguous()
+            with timer.timing_cuda('mm'):
+                p, grad_bias = dense.linear_slope(grad_output, saved, ctx.activation, ctx.needs_input_grad[2])
+            if z_local is not None:
+                ag = grad_features = None
+                with timer.timing_cuda('mm'):
+                    grad_weight = dense.linear_grad_weight(z_local, p)
+            else:
+                ag = aggregate(getattr(ctx.adj_parts, 'transposed', None) or ctx.adj_parts, p, 'Backward' + ctx.tag)
+                with timer.timing_cuda('mm'):
+                    grad_features = dense.linear_grad_input(ag, weight, grad_output if ctx.skip else None) if ctx.needs_input_grad[0] else None
+                    grad_weight = dense.linear_grad_weight(features, ag)
+            with timer.timing_cuda('all_reduce'):
+                reduce(grad_weight)
+                if grad_bias is not None:
+                    reduce(grad_bias)
+            return grad_features, grad_weight, grad_bias, None, None, None, None
+
+    Layer.__name__ = Layer.__qualname__ = name
+    return Layer
+
+
+EpilogueGCNLayer = epilogue_layer('EpilogueGCNLayer', lambda parts, feat, tag: broadcast(parts, feat, tag, padded_out=True))
+
+
+def fused_linear():
+    """DGNN_FUSED_LINEAR=1: models without bias or skip connection use the layers with the activation in the product too."""
+    return os.environ.get('DGNN_FUSED_LINEAR', '0') == '1'
+
+
 class GCN(nn.Module):
     """ReLU GCN; ``num_layers=3`` is the reference model (gcn.py:56-72): weights drawn with
-    torch.rand after torch.manual_seed(0) on the CPU, in layer order, then moved to the device."""
+    torch.rand after torch.manual_seed(0) on the CPU, in layer order, then moved to the device.
+
+    ``bias`` (zeros at first), ``activation`` of the hidden layers ('none', 'relu', 'gelu', 'silu') and ``skip`` (a skip
+    connection around every layer whose input and output have the same width) go through the layers with an epilogue
+    (``epilogue_layer``); the reference's model, the default, keeps its separate product and ReLU and its bits unless
+    DGNN_FUSED_LINEAR=1."""
 
     layer_cls = DistGCNLayer
+    epilogue_cls = EpilogueGCNLayer
 
-    def __init__(self, g, env, hidden_dim=16, num_layers=3):
+    def __init__(self, g, env, hidden_dim=16, num_layers=3, bias=False, activation='relu', skip=False):
         super().__init__()
+        if activation not in ('none', 'relu', 'gelu', 'silu'):
+            raise ValueError(f'unknown activation {activation!r} (none | relu | gelu | silu)')
         self.g, self.env, self.num_layers = g, env, num_layers
+        self.bias, self.activation, self.skip = bool(bias), activation, bool(skip)
+        self.epilogue = self.bias or self.skip or activation != 'relu' or fused_linear()
         dims = [g.features.size(1)] + [hidden_dim] * (num_layers - 1) + [g.num_classes]
         torch.manual_seed(0)
         for i in range(num_layers):
             setattr(self, f'weight{i + 1}', nn.Parameter(torch.rand(dims[i], dims[i + 1]).to(env.device)))
+        for i in range(num_layers if self.bias else 0):
+            setattr(self, f'bias{i + 1}', nn.Parameter(torch.zeros(dims[i + 1], device=env.device)))
         if g.features.is_cuda and g.features.dtype == torch.float32 and _spmm_override is None:
             # the input features are aggregated every epoch and never change: store them at the kernels' row pitch
             # once (same values, a [n, F] view of a zero-padded buffer) instead of copying them there per epoch
@@ -1021,6 +1102,11 @@ class GCN(nn.Module):
     def forward(self, features):
         h = features
         for i in range(self.num_layers):
+            if self.epilogue:
+                w = getattr(self, f'weight{i + 1}')
+                h = self.epilogue_cls.apply(h, w, getattr(self, f'bias{i + 1}', None), self.g.adj_parts, f'L{i + 1}',
+                                            self.activation if i + 1 < self.num_layers else 'none', self.skip and w.size(0) == w.size(1))
+                continue
             h = self.layer_cls.apply(h, getattr(self, f'weight{i + 1}'), self.g.adj_parts, f'L{i + 1}')
             if i + 1 < self.num_layers:
                 h = F.relu(h)

@@ -71,14 +71,18 @@ class _NoCache:
 Dist15DLayer = _gcn.aggregation_layer(
     'Dist15DLayer', lambda adj_parts, feat, tag: broadcast_15d(adj_parts, feat, tag),
     reduce_grad=lambda g: dist.all_reduce(g, op=dist.ReduceOp.SUM, group=_rep.col_group))
+EpilogueDist15DLayer = _gcn.epilogue_layer(
+    'EpilogueDist15DLayer', lambda adj_parts, feat, tag: broadcast_15d(adj_parts, feat, tag),
+    reduce_grad=lambda g: dist.all_reduce(g, op=dist.ReduceOp.SUM, group=_rep.col_group))
 
 
 class GCN15D(_gcn.GCN):
     """Same weights/initialisation as GCN; layers aggregate with the 1.5D schedule. ``g`` must be the
     Parted_COO_Graph of row block ``rank // rep`` out of ``world_size // rep``."""
     layer_cls = Dist15DLayer
+    epilogue_cls = EpilogueDist15DLayer
 
-    def __init__(self, g, env, hidden_dim=16, num_layers=3, rep=2):
+    def __init__(self, g, env, hidden_dim=16, num_layers=3, rep=2, bias=False, activation='relu', skip=False):
         if _rep is None or _rep.rep != rep or _rep.env is not env:
             init_rep(rep)
-        super().__init__(g, env, hidden_dim, num_layers)
+        super().__init__(g, env, hidden_dim, num_layers, bias, activation, skip)

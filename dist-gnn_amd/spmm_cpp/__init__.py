@@ -94,7 +94,7 @@ _TRAIN_SIGNATURES = {                    # argument types, in the order of inclu
     'dgnn_linear_workspace': [_i32, _i64, _i64, _i64, _i32, _pi64],
     'dgnn_linear_forward': [_p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _i32, _p, _i64, _p],
     'dgnn_linear_slope': [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i32, _i32, _p, _i64, _p],
-    'dgnn_linear_grad_input': [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _p, _i64, _p],
+    'dgnn_linear_grad_input': [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _p, _i64, _p],
     'dgnn_linear_grad_weight': [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _p, _i64, _p],
     'dgnn_adamw': [_p, _i32, _i32, _i32, _p, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, _p],
 }

@@ -119,19 +119,20 @@ def linear_slope(dy, saved, activation, need_bias=True):
     return (dy if p is None else p), db
 
 
-def linear_grad_input(p, weight):
-    """dx = p W^T."""
+def linear_grad_input(p, weight, add=None):
+    """dx = p W^T + add; ``add`` is what else reaches x, the gradient of a skip connection."""
     pp, ldp = _rows(p, 'p')
     wp, ldw = _rows(weight, 'weight', p)
     (M, N), K = p.shape, weight.shape[0]
     if weight.shape[1] != N:
         raise RuntimeError(f'spmm_cpp.linear: shape mismatch p{tuple(p.shape)} weight{tuple(weight.shape)}')
+    ap, lda = (None, 0) if add is None else _rows(add, 'add', p, (M, K))
     with torch.cuda.device(p.device):
         dx = torch.empty(M, K, dtype=p.dtype, device=p.device)
         if M and K:
             ws, wsp, nbytes = _workspace(_GRAD_INPUT, M, K, N, p)
-            _check(_lib.dgnn_linear_grad_input(pp, ldp, wp, ldw, dx.data_ptr(), K, M, K, N, _DTYPES[p.dtype], wsp, nbytes, _stream(p)),
-                   'linear_grad_input')
+            _check(_lib.dgnn_linear_grad_input(pp, ldp, wp, ldw, ap, lda, dx.data_ptr(), K, M, K, N, _DTYPES[p.dtype], wsp, nbytes,
+                                               _stream(p)), 'linear_grad_input')
     return dx
 
 

@@ -28,7 +28,7 @@ extern "C" {
  * With a gradient dy of y:
  *   dgnn_linear_slope         p = dy act'(x W + b) (p may be NULL), dbias[n] = sum over m of p[m][n] (may be NULL); p may be
  *                             dy itself. act DGNN_ACT_NONE: p is a copy of dy
- *   dgnn_linear_grad_input    dx = p W^T
+ *   dgnn_linear_grad_input    dx = p W^T + add    (add [M x K] or NULL: what else reaches x, a skip connection's gradient)
  *   dgnn_linear_grad_weight   dw = x^T p      (M = 0: zeros)
  * workspace: device memory of dgnn_linear_workspace(pass, ...) bytes, 4-byte aligned (0 bytes: may be NULL), free to be used
  * again once the call's kernels have run. Sums over many rows are cut by a rule of the sizes alone and joined in a fixed
@@ -49,8 +49,8 @@ int dgnn_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, 
                         void* workspace, int64_t workspace_bytes, void* stream);
 int dgnn_linear_slope(const void* dy, int64_t ldd, const void* save, int64_t lds, void* p, int64_t ldp, void* dbias,
                       int64_t M, int64_t N, int32_t dtype, int32_t act, void* workspace, int64_t workspace_bytes, void* stream);
-int dgnn_linear_grad_input(const void* p, int64_t ldp, const void* w, int64_t ldw, void* dx, int64_t ldx,
-                           int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int dgnn_linear_grad_input(const void* p, int64_t ldp, const void* w, int64_t ldw, const void* add, int64_t lda,
+                           void* dx, int64_t ldx, int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
 int dgnn_linear_grad_weight(const void* x, int64_t ldx, const void* p, int64_t ldp, void* dw, int64_t ldw,
                             int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
 

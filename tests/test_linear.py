@@ -18,8 +18,8 @@ def _slope(dy=A, ldd=8, save=B, lds=8, p=C, ldp=8, db=None, M=4, N=8, dtype=0, a
     return lib.dgnn_linear_slope(dy, ldd, save, lds, p, ldp, db, M, N, dtype, act, ws, n, None)
 
 
-def _grad_input(p=A, ldp=8, w=B, ldw=8, dx=C, ldx=8, M=4, K=8, N=8, dtype=0, ws=None, n=0):
-    return lib.dgnn_linear_grad_input(p, ldp, w, ldw, dx, ldx, M, K, N, dtype, ws, n, None)
+def _grad_input(p=A, ldp=8, w=B, ldw=8, add=None, lda=8, dx=C, ldx=8, M=4, K=8, N=8, dtype=0, ws=None, n=0):
+    return lib.dgnn_linear_grad_input(p, ldp, w, ldw, add, lda, dx, ldx, M, K, N, dtype, ws, n, None)
 
 
 def _grad_weight(x=A, ldx=8, p=B, ldp=8, dw=C, ldw=8, M=4, K=8, N=8, dtype=0, ws=None, n=0):
@@ -34,7 +34,7 @@ def _grad_weight(x=A, ldx=8, p=B, ldp=8, dw=C, ldw=8, M=4, K=8, N=8, dtype=0, ws
     (_forward, dict(act=2, save=D, lds=7)), (_forward, dict(M=1, K=4096, N=64, ldx=4096, ldw=64, ldy=64)),      # cut, no workspace
     (_slope, dict(dtype=-1)), (_slope, dict(act=9)), (_slope, dict(save=None)), (_slope, dict(lds=7)), (_slope, dict(dy=None)),
     (_slope, dict(ldp=7)), (_slope, dict(act=1, lds=0)), (_slope, dict(db=D)), (_slope, dict(db=D, ws=D, n=4)), (_slope, dict(db=D + 2)),
-    (_grad_input, dict(dtype=5)), (_grad_input, dict(p=None)), (_grad_input, dict(ldx=7)), (_grad_input, dict(dx=A)), (_grad_input, dict(N=-2)),
+    (_grad_input, dict(dtype=5)), (_grad_input, dict(p=None)), (_grad_input, dict(ldx=7)), (_grad_input, dict(dx=A)), (_grad_input, dict(add=D, lda=7)), (_grad_input, dict(add=C)), (_grad_input, dict(N=-2)),
     (_grad_weight, dict(dtype=5)), (_grad_weight, dict(x=None)), (_grad_weight, dict(ldw=7)), (_grad_weight, dict(dw=B)),
     (_grad_weight, dict(M=1 << 31)), (_grad_weight, dict(M=100000, dw=1 << 40)),                                # cut, no workspace
 ])

@@ -243,6 +243,16 @@ def test_gradients_that_are_expanded_or_transposed():
     assert torch.equal(c, d)
 
 
+def test_a_skip_connections_gradient_joins_the_product():
+    for dtype in DT:
+        x, w, _, _, dy = _inputs(300, 70, 40, dtype, False, False, 15)
+        want = _d(dy) @ _d(w).t() + _d(x)
+        bound = _sum_bound(40, dtype) * (_d(dy).abs() @ _d(w).abs().t()) + (U + HALF[dtype]) * want.abs() + 2.0 ** -24
+        _near(spmm_cpp.linear_grad_input(dy, w, add=x), want, bound, dtype)
+    with pytest.raises(RuntimeError, match='add'):
+        spmm_cpp.linear_grad_input(dy, w, add=x[:, :3])
+
+
 def test_columns_between_rows_are_left_alone():
     """The C entries write rows of any distance and nothing between them."""
     x, w, b, r, dy = _inputs(100, 40, 70, 'f32', True, True, 9)
@@ -258,7 +268,7 @@ def test_columns_between_rows_are_left_alone():
     assert lib.dgnn_linear_forward(x.data_ptr(), 40, w.data_ptr(), 70, b.data_ptr(), r.data_ptr(), 70, Y.data_ptr(), 75, None, 0,
                                    100, 40, 70, 0, 3, ws.data_ptr(), ws.numel() * 4, s) == 0
     assert lib.dgnn_linear_slope(dy.data_ptr(), 70, saved.data_ptr(), 70, P.data_ptr(), 75, None, 100, 70, 0, 3, None, 0, s) == 0
-    assert lib.dgnn_linear_grad_input(p.data_ptr(), 70, w.data_ptr(), 70, X.data_ptr(), 45, 100, 40, 70, 0, ws.data_ptr(), ws.numel() * 4, s) == 0
+    assert lib.dgnn_linear_grad_input(p.data_ptr(), 70, w.data_ptr(), 70, None, 0, X.data_ptr(), 45, 100, 40, 70, 0, ws.data_ptr(), ws.numel() * 4, s) == 0
     assert lib.dgnn_linear_grad_weight(x.data_ptr(), 40, p.data_ptr(), 70, W.data_ptr(), 75, 100, 40, 70, 0, ws.data_ptr(), ws.numel() * 4, s) == 0
     for big, small in ((Y, y), (P, p), (X, dx), (W, dw)):
         m, n = small.shape
