@@ -205,13 +205,121 @@ __device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c, _Float16) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, y.h, c, 0, 0, 0);
 }
 
-// what one output element becomes: bias, saved slope data (not relu's, which is one bit), activation, residual
+template <typename T> struct Four { typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T) == 4 ? 4 : 2))); };
+
+// `have` (0..4) elements at p; the others are zero
+template <typename T> __device__ __forceinline__ void load4(const T* p, int have, float (&v)[4]) {
+  if (have == 4) {
+    const typename Four<T>::type q = *reinterpret_cast<const typename Four<T>::type*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (float)q[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < have ? (float)p[i] : 0.f;
+  }
+}
+
+template <typename T> __device__ __forceinline__ void store4(T* p, int have, const float (&v)[4]) {
+  if (have == 4) {
+    typename Four<T>::type q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = (T)v[i];
+    *reinterpret_cast<typename Four<T>::type*>(p) = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < have) p[i] = (T)v[i];
+  }
+}
+
+// What 4 neighbouring sums of a row become: bias, saved slope data, activation, residual, one rounding. Lanes of a wave hold
+// neighbouring fours (8 lanes make relu's word of 32 bits), `have` of the 4 exist (0: none, but the lane still takes part).
 template <typename T>
-__device__ __forceinline__ void finish(const Gemm& g, int64_t row, int64_t col, float t) {
-  if (g.save && g.act > ACT_RELU) ((T*)g.save)[row * g.ld_save + col] = (T)t;
-  t = act_of(g.act, t);
-  if (g.residual) t += (float)((const T*)g.residual)[row * g.ld_residual + col];
-  ((T*)g.c)[row * g.ldc + col] = (T)t;
+__device__ __forceinline__ void finish(const Gemm& g, int64_t row, int64_t col, int have, float (&v)[4], const float (&bias)[4], const float (&res)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] += bias[i];
+  if (g.save && g.act == ACT_RELU) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bits |= (i < have && !(v[i] <= 0.f) ? 1u : 0u) << i;
+    const int lane = threadIdx.x & 7;
+    bits <<= 4 * lane;
+    bits |= __shfl_xor(bits, 1);
+    bits |= __shfl_xor(bits, 2);
+    bits |= __shfl_xor(bits, 4);
+    if (lane == 0 && have > 0) ((uint32_t*)g.save)[row * g.ld_save + col / 32] = bits;
+  } else if (g.save) {
+    store4((T*)g.save + row * g.ld_save + col, have, v);
+  }
+  switch (g.act) {
+    case ACT_NONE: break;
+    case ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = act_of(ACT_RELU, v[i]);
+      break;
+    case ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = act_of(ACT_GELU, v[i]);
+      break;
+    default:
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = act_of(ACT_SILU, v[i]);
+  }
+  if (g.residual) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += res[i];
+  }
+  store4((T*)g.c + row * g.ldc + col, have, v);
+}
+
+// A wave's TM x TN tiles of 32 x 32 from its accumulators to memory, 32 rows at a time through its own part of LDS: the
+// matrix cores leave a column's rows in a lane, memory wants a row's columns side by side (16 bytes of fp32 a lane). The
+// residual's rows are fetched before the turn, so that nothing waits for them one by one.
+template <typename T, int TM, int TN, bool AA, bool BA>
+__device__ __forceinline__ void epilogue(const Gemm& g, f16v (&acc)[TM][TN], float* room, int64_t row0, int64_t col0, int64_t k0, int64_t kend) {
+  constexpr int PITCH = TN * 32 + 4, LANES = TN * 8, STEP = 64 / LANES, TURNS = 32 / STEP;
+  const int lane = threadIdx.x & 63;
+  const int64_t col = col0 + (lane % LANES) * 4;
+  const int have_n = g.N - col >= 4 ? 4 : (g.N > col ? (int)(g.N - col) : 0);
+  const bool whole = g.slices == 1;
+  float bias[4] = {0.f, 0.f, 0.f, 0.f};
+  if (whole && g.bias) load4((const T*)g.bias + col, have_n, bias);
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int64_t first = row0 + i * 32 + lane / LANES;
+    float res[TURNS][4];
+    if (whole && g.residual) {
+#pragma unroll
+      for (int q = 0; q < TURNS; ++q) {
+        const int64_t row = first + q * STEP;
+        load4((const T*)g.residual + row * g.ld_residual + col, row < g.M ? have_n : 0, res[q]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)              // element e of a lane: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32
+        room[(8 * (e / 4) + 4 * (lane >> 5) + e % 4) * PITCH + j * 32 + (lane & 31)] = acc[i][j][e];
+#pragma unroll
+    for (int q = 0; q < TURNS; ++q) {
+      const int64_t row = first + q * STEP;
+      const int have = row < g.M ? have_n : 0;
+      const float4 t = *reinterpret_cast<const float4*>(room + (lane / LANES + q * STEP) * PITCH + (lane % LANES) * 4);
+      float v[4] = {t.x, t.y, t.z, t.w};
+      if constexpr (Unit<T>::PLANES == 3) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (c < have && !(fabsf(v[c]) < __builtin_huge_valf())) {
+            const T* a = (const T*)g.a + (AA ? row * g.lda : row);
+            const T* b = (const T*)g.b + (BA ? (col + c) * g.ldb : col + c);
+            v[c] = 0.f;
+            for (int64_t k = k0; k < kend; ++k) v[c] = fmaf((float)a[AA ? k : k * g.lda], (float)b[BA ? k : k * g.ldb], v[c]);
+          }
+      }
+      if (whole) finish<T>(g, row, col, have, v, bias, res[q]);
+      else store4(g.partial + ((int64_t)blockIdx.y * g.M + row) * g.N + col, have, v);
+    }
+  }
 }
 
 template <typename T, bool AA, bool BA, int BM, int BN, int WM, int WN>
@@ -290,61 +398,39 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm g) {
     buf ^= 1;
   }
 
-  // element i of a lane's 16: row 8 (i / 4) + 4 (lane / 32) + i % 4, column lane % 32 of the 32 x 32 tile
-#pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int64_t col = col0 + (wn * TN + j) * 32 + (lane & 31);
-    const bool in_n = col < g.N;
-    const float bias = g.bias && in_n && g.slices == 1 ? (float)((const T*)g.bias)[col] : 0.f;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t row = row0 + (wm * TM + i) * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
-        const bool in = in_n && row < g.M;
-        float t = acc[i][j][e];
-        if constexpr (PL == 3) {
-          if (in && !(fabsf(t) < __builtin_huge_valf())) {
-            t = 0.f;
-            for (int64_t k = k0; k < kend; ++k)
-              t = fmaf((float)a[AA ? row * g.lda + k : k * g.lda + row], (float)b[BA ? col * g.ldb + k : k * g.ldb + col], t);
-          }
-        }
-        if (g.slices > 1) {
-          if (in) g.partial[((int64_t)blockIdx.y * g.M + row) * g.N + col] = t;
-          continue;
-        }
-        t += bias;
-        if (g.save && g.act == ACT_RELU) {
-          const uint64_t bits = __ballot(in && !(t <= 0.f));
-          if (row < g.M && (lane & 31) == 0 && in_n)
-            ((uint32_t*)g.save)[row * g.ld_save + col / 32] = (uint32_t)(bits >> (lane & 32));
-        }
-        if (in) finish<T>(g, row, col, t);
-      }
-    }
-  }
+  static_assert(WM * WN * 32 * (TN * 32 + 4) * 4 <= 2 * (TA::BYTES + TB::BYTES), "the epilogue's rows fit the tiles' LDS");
+  epilogue<T, TM, TN, AA, BA>(g, acc, reinterpret_cast<float*>(&lds[0][0]) + wave * 32 * (TN * 32 + 4), row0 + wm * TM * 32,
+                              col0 + wn * TN * 32, k0, kend);
 }
 
-// Joins the slices of a product that was cut along its contraction, in their order, and finishes it. A wave takes 64
-// consecutive columns of a row, so relu's bits are whole words.
+// Joins the slices of a product that was cut along its contraction, in their order, and finishes it: 4 columns of a row a
+// lane, 8 slices' loads in flight. A row takes a multiple of 8 lanes, so that relu's bits are whole words.
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_join_kernel(const Gemm g) {
-  const int lane = threadIdx.x & 63;
-  const int64_t wide = (g.N + 63) / 64;
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= g.M * wide) return;
-  const int64_t row = at / wide, col = at % wide * 64 + lane;
-  const bool in = col < g.N;
-  float t = 0.f;
-  if (in)
-    for (int s = 0; s < g.slices; ++s) t += g.partial[((int64_t)s * g.M + row) * g.N + col];
-  if (in && g.bias) t += (float)((const T*)g.bias)[col];
-  if (g.save && g.act == ACT_RELU) {
-    const uint64_t bits = __ballot(in && !(t <= 0.f));
-    if ((lane & 31) == 0 && in) ((uint32_t*)g.save)[row * g.ld_save + col / 32] = (uint32_t)(bits >> (lane & 32));
+  const int64_t wide = (g.N + 31) / 32 * 8;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = at / wide, col = at % wide * 4;
+  const int have = row < g.M && col < g.N ? (g.N - col >= 4 ? 4 : (int)(g.N - col)) : 0;
+  float v[4] = {0.f, 0.f, 0.f, 0.f}, bias[4] = {0.f, 0.f, 0.f, 0.f}, res[4] = {0.f, 0.f, 0.f, 0.f};
+  if (have) {
+    const float* p = g.partial + row * g.N + col;
+    const int64_t step = g.M * g.N;
+    for (int s = 0; s < g.slices; s += 8) {
+      float t[8][4];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (s + u < g.slices) load4(p + (s + u) * step, have, t[u]);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (s + u < g.slices) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] += t[u][i];
+        }
+    }
+    if (g.bias) load4((const T*)g.bias + col, have, bias);
+    if (g.residual) load4((const T*)g.residual + row * g.ld_residual + col, have, res);
   }
-  if (in) finish<T>(g, row, col, t);
+  finish<T>(g, row, col, have, v, bias, res);
 }
 
 struct Shape { int bm, bn; };
@@ -376,8 +462,8 @@ int gemm_launch(const Gemm& g) {
   }
   DGNN_LAUNCHED();
   if (g.slices > 1) {
-    const int64_t waves = g.M * ((g.N + 63) / 64);
-    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, g.stream, g);
+    const int64_t lanes = g.M * ((g.N + 31) / 32 * 8);
+    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((uint32_t)((lanes + 255) / 256)), dim3(256), 0, g.stream, g);
     DGNN_LAUNCHED();
   }
   return DGNN_OK;

@@ -100,8 +100,15 @@ __global__ __launch_bounds__(256) void slab_join_kernel(const float* __restrict_
   const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
   const int64_t col = (int64_t)blockIdx.x * 16 + c;
   float t = 0.f;
-  if (col < N)
-    for (int64_t s = k; s < slabs; s += 16) t += partial[s * N + col];
+  if (col < N) {
+    for (int64_t s = k; s < slabs; s += 128) {               // 8 loads in flight, added in their order
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = s + 16 * u < slabs ? partial[(s + 16 * u) * N + col] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) t += v[u];
+    }
+  }
   sums[k][c] = t;
   __syncthreads();
   if (k == 0 && col < N) {
@@ -136,7 +143,7 @@ int64_t slope_lanes(int64_t N) {
 
 int64_t slope_slab(int64_t M, int64_t N) {
   const int64_t groups = 256 / slope_lanes(N), across = ceil_div(N, 4 * slope_lanes(N));
-  const int64_t blocks = 2048 / (across < 2048 ? across : 2048);
+  const int64_t blocks = 1024 / (across < 1024 ? across : 1024);
   return ceil_div(ceil_div(M, blocks < 1 ? 1 : blocks), groups) * groups;
 }
 
