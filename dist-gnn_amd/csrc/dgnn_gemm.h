@@ -17,6 +17,8 @@
 #pragma once
 #include "dgnn_internal.h"
 
+#include <type_traits>
+
 namespace dgnn {
 
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
@@ -39,6 +41,7 @@ struct Gemm {
   float* partial;          // slices x M x N when slices > 1
   int slices;
   int64_t slice_k;         // contraction elements a slice takes, a multiple of 64
+  char* image;             // room for W's image where the product runs on rows_kernel, else null
   hipStream_t stream;
 };
 
@@ -48,6 +51,14 @@ __device__ __forceinline__ float act_of(int act, float t) {
     case ACT_GELU: return 0.5f * t * (1.f + erff(t * 0.70710678118654752f));
     case ACT_SILU: return t / (1.f + expf(-t));
     default: return t;
+  }
+}
+
+// f(0), f(1), ... f(N - 1) with constant arguments: register arrays that f indexes stay in registers whatever its size
+template <int I, int N, typename F> __device__ __forceinline__ void each(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    each<I + 1, N>(f);
   }
 }
 
@@ -433,6 +444,298 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const Gemm g) {
   finish<T>(g, row, col, have, v, bias, res);
 }
 
+// ---------------------------------------------------------------------------------------
+// Many rows (forward and input gradient of whole graphs or batches). W is laid out first, once a call: zero-padded chunks in the
+// order in which a workgroup's stages read them (split into its three pieces where T is float), so that a stage is one
+// contiguous copy into LDS and the main kernel spends no instruction on W's layout or split. A's rows are not shared by
+// waves -- a wave owns 32 rows and all BN columns -- so they go from memory straight to the lanes that multiply them, and an
+// element is split once. The product is taken transposed, W^T's piece as the first operand: a lane then holds one row's
+// columns in fours and writes them itself, without a turn through LDS.
+// ---------------------------------------------------------------------------------------
+template <typename T> struct Rows;                          // BK: contraction elements a stage
+template <> struct Rows<float> { static constexpr int BK = 16; };
+template <> struct Rows<__bf16> { static constexpr int BK = 64; };
+template <> struct Rows<_Float16> { static constexpr int BK = 64; };
+
+struct Layout {
+  const void* w;
+  int64_t ld, N, K;
+  bool along;
+  int64_t ktiles, ntiles;
+  char* image;              // [ntiles][ktiles][PLANES][BK / 8][BN] chunks
+};
+
+template <typename T, int BN>
+__global__ __launch_bounds__(256) void lay_out_kernel(const Layout g) {
+  constexpr int CH = Rows<T>::BK / 8, PL = Unit<T>::PLANES;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;         // chunk (column tile, stage, chunk, column)
+  const int64_t n = at % BN, c = at / BN % CH, kt = at / BN / CH % g.ktiles, nt = at / BN / CH / g.ktiles;
+  if (nt >= g.ntiles) return;
+  const int64_t col = nt * BN + n, k = (kt * CH + c) * 8;
+  const T* w = (const T*)g.w + (g.along ? col * g.ld + k : k * g.ld + col);
+  const int64_t step = g.along ? 1 : g.ld;
+  T v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = col < g.N && k + i < g.K ? w[i * step] : (T)0.f;
+  u4* out = reinterpret_cast<u4*>(g.image) + ((nt * g.ktiles + kt) * PL * CH + c) * BN + n;
+  if constexpr (PL == 3) {
+    float f[8];
+    u4 h[3];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (float)v[i];
+    split8(f, h);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) out[(int64_t)p * CH * BN] = h[p];
+  } else {
+    union { T e[8]; u4 u; } r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.e[i] = v[i];
+    *out = r.u;
+  }
+}
+
+// 8 consecutive elements of a row, `left` of which exist
+template <typename T> struct Eight { u4 q[8 / Unit<T>::W]; };
+template <typename T> __device__ __forceinline__ void load8(const T* p, int64_t left, Eight<T>& v) {
+  constexpr int W = Unit<T>::W;
+  if (left >= 8) {
+#pragma unroll
+    for (int i = 0; i < 8 / W; ++i) v.q[i] = load16(p + i * W);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8 / W; ++i) v.q[i] = load_some(p + i * W, left - i * W);
+  }
+}
+
+// A lane's columns of its row: saved slope data, activation, residual, one rounding.
+template <typename T, int TN, int ACT>
+__device__ __forceinline__ void rows_out(const Gemm& g, const f16v (&acc)[TN], int64_t row, int64_t col0, int half, bool in) {
+  each<0, TN>([&](auto j) __attribute__((always_inline)) {
+    const int64_t base = col0 + j * 32 + 4 * half;
+    int have[4];
+    float res[4][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t left = g.N - base - 8 * q;
+      have[q] = !in || left <= 0 ? 0 : left >= 4 ? 4 : (int)left;
+    }
+    if (g.residual) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) load4((const T*)g.residual + row * g.ld_residual + base + 8 * q, have[q], res[q]);
+    }
+    uint32_t bits = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = acc[j][4 * q + i];
+      if (g.save) {
+        if constexpr (ACT == ACT_RELU) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) bits |= (i < have[q] && !(v[i] <= 0.f) ? 1u : 0u) << (8 * q + 4 * half + i);
+        } else {
+          store4((T*)g.save + row * g.ld_save + base + 8 * q, have[q], v);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = act_of(ACT, v[i]);
+      if (g.residual) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += res[q][i];
+      }
+      store4((T*)g.c + row * g.ldc + base + 8 * q, have[q], v);
+    }
+    if constexpr (ACT == ACT_RELU) {
+      if (g.save) {
+        bits |= __shfl_xor(bits, 32);
+        if (half == 0 && have[0] > 0) ((uint32_t*)g.save)[row * g.ld_save + (col0 / 32 + j)] = bits;
+      }
+    }
+  });
+}
+
+// TN: column tiles of 32 a wave; RESIDENT: all of W's image stays in LDS and a wave walks over row blocks.
+template <typename T, int TN, int WAVES, bool RESIDENT>
+__global__ __launch_bounds__(WAVES * 64, 2) void rows_kernel(const Gemm g, const char* image, int ktiles) {
+  constexpr int BK = Rows<T>::BK, CH = BK / 8, PL = Unit<T>::PLANES, BN = TN * 32, THREADS = WAVES * 64, S = BK / 16;
+  constexpr int STAGE = PL * CH * BN * 16;                            // bytes
+  constexpr int PER = (STAGE / 16 + THREADS - 1) / THREADS;
+  extern __shared__ __attribute__((aligned(16))) char lds[];          // 2 stages, or all of them
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  // consecutive workgroups go round the 8 XCDs: the column tiles of a row block stay on one of them, one after the other
+  const int64_t ntiles = (g.N + BN - 1) / BN, turn = blockIdx.x / 8;
+  const int64_t nt = turn % ntiles, group = turn / ntiles * 8 + blockIdx.x % 8;
+  const int64_t col0 = nt * BN;
+  const u4* w = reinterpret_cast<const u4*>(image) + nt * ktiles * (STAGE / 16);
+  const T* a = (const T*)g.a;
+
+  u4 stage[PER];
+  auto fetch_w = [&](int kt) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if ((STAGE / 16) % THREADS == 0 || tid + i * THREADS < STAGE / 16) stage[i] = w[(int64_t)kt * (STAGE / 16) + tid + i * THREADS];
+  };
+  auto store_w = [&](char* to) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if ((STAGE / 16) % THREADS == 0 || tid + i * THREADS < STAGE / 16) reinterpret_cast<u4*>(to)[tid + i * THREADS] = stage[i];
+  };
+  Eight<T> cur[S], next[S];
+  auto fetch_a = [&](int64_t block, int kt, Eight<T> (&to)[S]) {
+    int64_t row = block * 32 + (lane & 31);
+    row = row < g.M ? row : g.M - 1;
+    const T* p = a + row * g.lda + (int64_t)kt * BK + 8 * half;
+#pragma unroll
+    for (int s = 0; s < S; ++s) load8(p + 16 * s, g.K - (int64_t)kt * BK - 8 * half - 16 * s, to[s]);
+  };
+
+  const int64_t blocks = (g.M + 31) / 32;
+  int64_t block = group * WAVES + wave;
+  if (!RESIDENT && group * WAVES >= blocks) return;
+  if constexpr (RESIDENT) {
+    for (int kt = 0; kt < ktiles; ++kt) { fetch_w(kt); store_w(lds + kt * STAGE); }
+  } else {
+    fetch_w(0);
+    store_w(lds);
+  }
+  fetch_a(block < blocks ? block : blocks - 1, 0, cur);
+  __syncthreads();
+  if (RESIDENT && block >= blocks) return;
+
+  for (;;) {
+    asm volatile("" ::: "memory");                            // the bias is loaded for each block, not held in 16 TN registers
+    // sums start at the bias: element e of a lane is column 8 (e / 4) + 4 half + e % 4 of the tile, row lane % 32
+    f16v acc[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        float b[4] = {0.f, 0.f, 0.f, 0.f};
+        const int64_t col = col0 + j * 32 + 2 * e + 4 * half;
+        if (g.bias) load4((const T*)g.bias + col, g.N - col >= 4 ? 4 : (g.N > col ? (int)(g.N - col) : 0), b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][e + i] = b[i];
+      }
+    for (int kt = 0; kt < ktiles; ++kt) {
+      const char* from = lds + (RESIDENT ? kt : kt & 1) * STAGE;
+      if constexpr (RESIDENT) {
+        const int64_t after = block + (int64_t)gridDim.x * WAVES;
+        if (kt + 1 < ktiles) fetch_a(block, kt + 1, next);
+        else if (after < blocks) fetch_a(after, 0, next);
+      } else if (kt + 1 < ktiles) {
+        fetch_w(kt + 1);
+        fetch_a(block < blocks ? block : blocks - 1, kt + 1, next);
+      }
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        u4 x[PL];
+        if constexpr (PL == 3) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(cur[s].q[i / 4][i % 4]);
+          split8(v, x);
+        } else {
+          x[0] = cur[s].q[0];
+        }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          u4 y[PL];
+#pragma unroll
+          for (int p = 0; p < PL; ++p)
+            y[p] = *reinterpret_cast<const u4*>(from + (((p * CH + 2 * s + half) * BN) + j * 32 + (lane & 31)) * 16);
+          if constexpr (PL == 3) {                             // small products first
+            acc[j] = mfma(y[0], x[2], acc[j], T());
+            acc[j] = mfma(y[2], x[0], acc[j], T());
+            acc[j] = mfma(y[1], x[1], acc[j], T());
+            acc[j] = mfma(y[0], x[1], acc[j], T());
+            acc[j] = mfma(y[1], x[0], acc[j], T());
+          }
+          acc[j] = mfma(y[0], x[0], acc[j], T());
+        }
+      }
+      if constexpr (!RESIDENT) {
+        if (kt + 1 < ktiles) store_w(lds + ((kt + 1) & 1) * STAGE);
+        __syncthreads();
+      }
+#pragma unroll
+      for (int s = 0; s < S; ++s) cur[s] = next[s];
+    }
+
+    const int64_t row = block * 32 + (lane & 31);
+    const bool in = row < g.M;
+    if constexpr (PL == 3) {
+      float seen = 0.f;                                       // 0, or NaN where a sum is not finite
+      each<0, TN>([&](auto j) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) seen = fmaf(acc[j][e], 0.f, seen);
+      });
+      if (__ballot(!(seen == 0.f))) {
+        each<0, TN>([&](auto j) __attribute__((always_inline)) {
+#pragma unroll 1
+          for (int e = 0; e < 16; ++e) {
+            const int64_t col = col0 + j * 32 + 8 * (e / 4) + 4 * half + e % 4;
+            float t = acc[j][e];
+            if (in && col < g.N && !(fabsf(t) < __builtin_huge_valf())) {
+              const T* x = a + row * g.lda;
+              const T* y = (const T*)g.b + (g.b_along ? col * g.ldb : col);
+              t = 0.f;
+              for (int64_t k = 0; k < g.K; ++k) t = fmaf((float)x[k], (float)y[g.b_along ? k : k * g.ldb], t);
+              if (g.bias) t += (float)((const T*)g.bias)[col];
+            }
+            acc[j][e] = t;
+          }
+        });
+      }
+    }
+    switch (g.act) {
+      case ACT_RELU: rows_out<T, TN, ACT_RELU>(g, acc, row, col0, half, in); break;
+      case ACT_GELU: rows_out<T, TN, ACT_GELU>(g, acc, row, col0, half, in); break;
+      case ACT_SILU: rows_out<T, TN, ACT_SILU>(g, acc, row, col0, half, in); break;
+      default: rows_out<T, TN, ACT_NONE>(g, acc, row, col0, half, in);
+    }
+    if constexpr (!RESIDENT) break;
+    block += (int64_t)gridDim.x * WAVES;
+    if (block >= blocks) break;
+  }
+}
+
+// Columns a wave takes: all of a narrow output, else 256.
+inline int rows_bn(int64_t N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }
+
+// Bytes of W's image, and whether this product runs on rows_kernel: from 1024 rows up, where laying W out is paid back.
+template <typename T> int64_t rows_image(const Gemm& g) {
+  const int64_t bn = rows_bn(g.N), bk = Rows<T>::BK;
+  return ((g.N + bn - 1) / bn) * bn * ((g.K + bk - 1) / bk) * bk * Unit<T>::PLANES * 2;
+}
+inline bool rows_fit(const Gemm& g) {
+  const int64_t bn = rows_bn(g.N), groups = (g.M + 127) / 128 * ((g.N + bn - 1) / bn);
+  return g.a_along && g.K > 0 && groups >= 512 && groups < (1 << 28);
+}
+
+template <typename T, int TN>
+int rows_launch(const Gemm& g, char* image) {
+  constexpr int BN = TN * 32, BK = Rows<T>::BK, CH = BK / 8, STAGE = Unit<T>::PLANES * CH * BN * 16;
+  const int64_t ktiles = (g.K + BK - 1) / BK, ntiles = (g.N + BN - 1) / BN;
+  const Layout l{g.b, g.ldb, g.N, g.K, g.b_along, ktiles, ntiles, image};
+  const int64_t chunks = ntiles * ktiles * CH * BN;
+  hipLaunchKernelGGL((lay_out_kernel<T, BN>), dim3((uint32_t)((chunks + 255) / 256)), dim3(256), 0, g.stream, l);
+  DGNN_LAUNCHED();
+  const int64_t blocks = (g.M + 31) / 32;
+  if (ntiles == 1 && ktiles * STAGE <= 128 * 1024) {
+    constexpr int WAVES = 8;
+    const int64_t per = ktiles * STAGE <= 64 * 1024 ? 2 : 1;          // workgroups a compute unit
+    const int64_t want = (blocks + WAVES - 1) / WAVES, most = 256 * per;
+    hipLaunchKernelGGL((rows_kernel<T, TN, WAVES, true>), dim3((uint32_t)(want < most ? (want + 7) / 8 * 8 : most), 1), dim3(WAVES * 64), (uint32_t)(ktiles * STAGE),
+                       g.stream, g, image, (int)ktiles);
+  } else {
+    constexpr int WAVES = 4;
+    hipLaunchKernelGGL((rows_kernel<T, TN, WAVES, false>), dim3((uint32_t)(((blocks + WAVES - 1) / WAVES + 7) / 8 * 8 * ntiles)), dim3(WAVES * 64), 2 * STAGE,
+                       g.stream, g, image, (int)ktiles);
+  }
+  DGNN_LAUNCHED();
+  return DGNN_OK;
+}
+
 struct Shape { int bm, bn; };
 
 // Tile by the sides of the output: the narrowest that covers it once, else 128 x 256 (the operand with fewer bytes a
@@ -471,6 +774,13 @@ int gemm_launch(const Gemm& g) {
 
 template <typename T>
 int gemm_typed(const Gemm& g) {
+  if (g.image) {
+    switch (rows_bn(g.N)) {
+      case 32: return rows_launch<T, 1>(g, g.image);
+      case 64: return rows_launch<T, 2>(g, g.image);
+      default: return rows_launch<T, 4>(g, g.image);
+    }
+  }
   if (g.a_along && !g.b_along) return gemm_launch<T, true, false>(g);
   if (g.a_along && g.b_along) return gemm_launch<T, true, true>(g);
   return gemm_launch<T, false, false>(g);

@@ -168,14 +168,24 @@ bool apart(const void* a, int64_t lda, int64_t ra, int64_t ca, const void* b, in
   return a1 <= b0 || b1 <= a0;
 }
 
+// How a product runs, by its sizes: over W's laid-out image where there are many rows, else by tiles, cut along the
+// contraction where those are few. Returns the bytes of workspace that takes.
+int64_t plan(Gemm& g, int32_t dtype) {
+  if (rows_fit(g)) {
+    g.slices = 1;
+    return dtype == DGNN_F32 ? rows_image<float>(g) : rows_image<_Float16>(g);
+  }
+  cut(g);
+  return g.slices > 1 ? (int64_t)g.slices * g.M * g.N * 4 : 0;
+}
+
 int run(const Gemm& g, int32_t dtype, void* workspace, int64_t bytes, const char* who) {
   Gemm h = g;
-  cut(h);
-  if (h.slices > 1) {
-    if (!workspace || bytes < (int64_t)h.slices * h.M * h.N * 4 || (uintptr_t)workspace % 4)
-      return dgnn_fail(DGNN_E_BADARG, "%s: workspace too small (%lld bytes wanted)", who, (long long)h.slices * h.M * h.N * 4);
-    h.partial = (float*)workspace;
-  }
+  const int64_t need = plan(h, dtype);
+  if (need && (!workspace || bytes < need || (uintptr_t)workspace % 16))
+    return dgnn_fail(DGNN_E_BADARG, "%s: workspace too small or misaligned (%lld bytes wanted)", who, (long long)need);
+  if (h.slices > 1) h.partial = (float*)workspace;
+  else if (need) h.image = (char*)workspace;
   if (dtype == DGNN_F32) return gemm_f32(h);
   if (dtype == DGNN_BF16) return gemm_bf16(h);
   return gemm_f16(h);
@@ -190,8 +200,8 @@ int dgnn_linear_workspace(int32_t pass, int64_t M, int64_t K, int64_t N, int32_t
   *bytes = 0;
   Gemm g{};
   switch (pass) {
-    case DGNN_LINEAR_FORWARD: g.M = M; g.N = N; g.K = K; break;
-    case DGNN_LINEAR_GRAD_INPUT: g.M = M; g.N = K; g.K = N; break;
+    case DGNN_LINEAR_FORWARD: g.M = M; g.N = N; g.K = K; g.a_along = true; break;
+    case DGNN_LINEAR_GRAD_INPUT: g.M = M; g.N = K; g.K = N; g.a_along = true; break;
     case DGNN_LINEAR_GRAD_WEIGHT: g.M = K; g.N = N; g.K = M; break;
     case DGNN_LINEAR_SLOPE:
       if (M > 0 && N > 0) *bytes = ceil_div(M, slope_slab(M, N)) * N * 4;
@@ -199,8 +209,7 @@ int dgnn_linear_workspace(int32_t pass, int64_t M, int64_t K, int64_t N, int32_t
     default: return dgnn_fail(DGNN_E_BADARG, "linear_workspace: unknown pass%s (%lld)", "", pass);
   }
   if (g.M == 0 || g.N == 0) return DGNN_OK;
-  cut(g);
-  if (g.slices > 1) *bytes = (int64_t)g.slices * g.M * g.N * 4;
+  *bytes = plan(g, dtype);
   return DGNN_OK;
 }
 

@@ -30,7 +30,7 @@ extern "C" {
  *                             dy itself. act DGNN_ACT_NONE: p is a copy of dy
  *   dgnn_linear_grad_input    dx = p W^T + add    (add [M x K] or NULL: what else reaches x, a skip connection's gradient)
  *   dgnn_linear_grad_weight   dw = x^T p      (M = 0: zeros)
- * workspace: device memory of dgnn_linear_workspace(pass, ...) bytes, 4-byte aligned (0 bytes: may be NULL), free to be used
+ * workspace: device memory of dgnn_linear_workspace(pass, ...) bytes, 16-byte aligned (0 bytes: may be NULL), free to be used
  * again once the call's kernels have run. Sums over many rows are cut by a rule of the sizes alone and joined in a fixed
  * order: the same bits every run. Outputs must not overlap inputs (but p may be dy).
  */
