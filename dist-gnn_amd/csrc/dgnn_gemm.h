@@ -453,7 +453,7 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const Gemm g) {
 // columns in fours and writes them itself, without a turn through LDS.
 // ---------------------------------------------------------------------------------------
 template <typename T> struct Rows;                          // BK: contraction elements a stage
-template <> struct Rows<float> { static constexpr int BK = 16; };
+template <> struct Rows<float> { static constexpr int BK = 32; };
 template <> struct Rows<__bf16> { static constexpr int BK = 64; };
 template <> struct Rows<_Float16> { static constexpr int BK = 64; };
 
@@ -507,105 +507,136 @@ template <typename T> __device__ __forceinline__ void load8(const T* p, int64_t 
   }
 }
 
-// A lane's columns of its row: saved slope data, activation, residual, one rounding.
+// A lane of a transposed tile holds its row's columns 8 q + 4 half .. + 3, q = 0..3. Memory takes them as 16 bytes a lane:
+// fp32 fours as they are; two fours of 16-bit values after the halves of the wave have exchanged them, so that a lane of the
+// lower half has columns 16 u .. + 7 and its partner columns 16 u + 8 .. + 15 (u = 0, 1).
+template <typename T> struct Out16;
+template <typename T> struct Out : Out16<T> {};
+template <> struct Out<float> {
+  static constexpr int PIECES = 4, WIDE = 4;                  // 16-byte pieces of a tile's row a lane, elements in one
+  static __device__ __forceinline__ int column(int piece, int half) { return 8 * piece + 4 * half; }
+  static __device__ __forceinline__ void pack(const float (&v)[16], u4 (&out)[4]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[q][i] = __float_as_uint(v[4 * q + i]);
+  }
+  static __device__ __forceinline__ void unpack(const u4 (&in)[4], float (&v)[16]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * q + i] = __uint_as_float(in[q][i]);
+  }
+};
+template <typename T> struct Out16 {
+  static constexpr int PIECES = 2, WIDE = 8;
+  static __device__ __forceinline__ int column(int piece, int half) { return 16 * piece + 8 * half; }
+  static __device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b) {       // a's upper half and b's lower half
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    const u2 r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+  }
+  static __device__ __forceinline__ void pack(const float (&v)[16], u4 (&out)[2]) {
+    union { T e[16]; uint32_t u[8]; } r;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r.e[i] = (T)v[i];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int d = 0; d < 2; ++d) exchange(r.u[4 * u + d], r.u[4 * u + 2 + d]);
+#pragma unroll
+      for (int d = 0; d < 2; ++d) { out[u][d] = r.u[4 * u + d]; out[u][2 + d] = r.u[4 * u + 2 + d]; }
+    }
+  }
+  static __device__ __forceinline__ void unpack(const u4 (&in)[2], float (&v)[16]) {
+    union { T e[16]; uint32_t u[8]; } r;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        r.u[4 * u + d] = in[u][d];
+        r.u[4 * u + 2 + d] = in[u][2 + d];
+        exchange(r.u[4 * u + d], r.u[4 * u + 2 + d]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = (float)r.e[i];
+  }
+};
+
+// the first `have` elements of a 16-byte piece at p
+template <typename T> __device__ __forceinline__ void store_piece(T* p, int have, u4 v) {
+  constexpr int W = Unit<T>::W;
+  if (have >= W) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<u4_at4*>(p) = v;
+    else *reinterpret_cast<u4_at2*>(p) = v;
+  } else {
+    union { u4 u; T e[W]; } r;
+    r.u = v;
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      if (i < have) p[i] = r.e[i];
+  }
+}
+template <typename T> __device__ __forceinline__ u4 load_piece(const T* p, int have) {
+  return have >= Unit<T>::W ? load16(p) : load_some(p, have);
+}
+
+// A lane's columns of its row: saved slope data, activation, residual, one rounding. `res` holds the residual's pieces.
 template <typename T, int TN, int ACT>
-__device__ __forceinline__ void rows_out(const Gemm& g, const f16v (&acc)[TN], int64_t row, int64_t col0, int half, bool in) {
+__device__ __forceinline__ void rows_out(const Gemm& g, const f16v (&acc)[TN], const u4 (&res)[TN][Out<T>::PIECES], int64_t row, int64_t col0, int half, bool in) {
+  constexpr int PIECES = Out<T>::PIECES, WIDE = Out<T>::WIDE;
+  T* const c = (T*)g.c + row * g.ldc;
   each<0, TN>([&](auto j) __attribute__((always_inline)) {
-    const int64_t base = col0 + j * 32 + 4 * half;
-    int have[4];
-    float res[4][4];
+    const int64_t base = col0 + j * 32, left = in ? g.N - base : 0;
+    auto have = [&](int piece) __attribute__((always_inline)) {
+      const int64_t n = left - Out<T>::column(piece, half);
+      return n >= WIDE ? WIDE : n > 0 ? (int)n : 0;
+    };
+    float v[16];
+    u4 out[PIECES];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t left = g.N - base - 8 * q;
-      have[q] = !in || left <= 0 ? 0 : left >= 4 ? 4 : (int)left;
-    }
-    if (g.residual) {
+    for (int e = 0; e < 16; ++e) v[e] = acc[j][e];
+    if (ACT != ACT_NONE && g.save) {
+      if constexpr (ACT == ACT_RELU) {
+        uint32_t bits = 0;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) load4((const T*)g.residual + row * g.ld_residual + base + 8 * q, have[q], res[q]);
-    }
-    uint32_t bits = 0;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = acc[j][4 * q + i];
-      if (g.save) {
-        if constexpr (ACT == ACT_RELU) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) bits |= (i < have[q] && !(v[i] <= 0.f) ? 1u : 0u) << (8 * q + 4 * half + i);
-        } else {
-          store4((T*)g.save + row * g.ld_save + base + 8 * q, have[q], v);
+        for (int e = 0; e < 16; ++e) {
+          const int n = 8 * (e / 4) + 4 * half + e % 4;
+          bits |= (n < left && !(v[e] <= 0.f) ? 1u : 0u) << n;
         }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = act_of(ACT, v[i]);
-      if (g.residual) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += res[q][i];
-      }
-      store4((T*)g.c + row * g.ldc + base + 8 * q, have[q], v);
-    }
-    if constexpr (ACT == ACT_RELU) {
-      if (g.save) {
         bits |= __shfl_xor(bits, 32);
-        if (half == 0 && have[0] > 0) ((uint32_t*)g.save)[row * g.ld_save + (col0 / 32 + j)] = bits;
+        if (half == 0 && left > 0) ((uint32_t*)g.save)[row * g.ld_save + (col0 / 32 + j)] = bits;
+      } else {
+        Out<T>::pack(v, out);
+#pragma unroll
+        for (int q = 0; q < PIECES; ++q) store_piece((T*)g.save + row * g.ld_save + base + Out<T>::column(q, half), have(q), out[q]);
       }
     }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = act_of(ACT, v[e]);
+    if (g.residual) {
+      float r[16];
+      Out<T>::unpack(res[j], r);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] += r[e];
+    }
+    Out<T>::pack(v, out);
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) store_piece(c + base + Out<T>::column(q, half), have(q), out[q]);
   });
 }
 
-// TN: column tiles of 32 a wave; RESIDENT: all of W's image stays in LDS and a wave walks over row blocks.
-template <typename T, int TN, int WAVES, bool RESIDENT>
-__global__ __launch_bounds__(WAVES * 64, 2) void rows_kernel(const Gemm g, const char* image, int ktiles) {
-  constexpr int BK = Rows<T>::BK, CH = BK / 8, PL = Unit<T>::PLANES, BN = TN * 32, THREADS = WAVES * 64, S = BK / 16;
-  constexpr int STAGE = PL * CH * BN * 16;                            // bytes
-  constexpr int PER = (STAGE / 16 + THREADS - 1) / THREADS;
-  extern __shared__ __attribute__((aligned(16))) char lds[];          // 2 stages, or all of them
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  // consecutive workgroups go round the 8 XCDs: the column tiles of a row block stay on one of them, one after the other
-  const int64_t ntiles = (g.N + BN - 1) / BN, turn = blockIdx.x / 8;
-  const int64_t nt = turn % ntiles, group = turn / ntiles * 8 + blockIdx.x % 8;
-  const int64_t col0 = nt * BN;
-  const u4* w = reinterpret_cast<const u4*>(image) + nt * ktiles * (STAGE / 16);
-  const T* a = (const T*)g.a;
+// What a wave of the two kernels below does: TN column tiles of 32 rows.
+template <typename T, int TN> struct Wave {
+  static constexpr int BK = Rows<T>::BK, CH = BK / 8, PL = Unit<T>::PLANES, BN = TN * 32, S = BK / 16;
+  static constexpr int STAGE = PL * CH * BN * 16;             // bytes of a stage of W's image
+  f16v acc[TN];
+  Eight<T> a[S];                                              // this lane's part of its row: 8 elements of each 16
 
-  u4 stage[PER];
-  auto fetch_w = [&](int kt) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if ((STAGE / 16) % THREADS == 0 || tid + i * THREADS < STAGE / 16) stage[i] = w[(int64_t)kt * (STAGE / 16) + tid + i * THREADS];
-  };
-  auto store_w = [&](char* to) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if ((STAGE / 16) % THREADS == 0 || tid + i * THREADS < STAGE / 16) reinterpret_cast<u4*>(to)[tid + i * THREADS] = stage[i];
-  };
-  Eight<T> cur[S], next[S];
-  auto fetch_a = [&](int64_t block, int kt, Eight<T> (&to)[S]) {
-    int64_t row = block * 32 + (lane & 31);
-    row = row < g.M ? row : g.M - 1;
-    const T* p = a + row * g.lda + (int64_t)kt * BK + 8 * half;
-#pragma unroll
-    for (int s = 0; s < S; ++s) load8(p + 16 * s, g.K - (int64_t)kt * BK - 8 * half - 16 * s, to[s]);
-  };
-
-  const int64_t blocks = (g.M + 31) / 32;
-  int64_t block = group * WAVES + wave;
-  if (!RESIDENT && group * WAVES >= blocks) return;
-  if constexpr (RESIDENT) {
-    for (int kt = 0; kt < ktiles; ++kt) { fetch_w(kt); store_w(lds + kt * STAGE); }
-  } else {
-    fetch_w(0);
-    store_w(lds);
-  }
-  fetch_a(block < blocks ? block : blocks - 1, 0, cur);
-  __syncthreads();
-  if (RESIDENT && block >= blocks) return;
-
-  for (;;) {
-    asm volatile("" ::: "memory");                            // the bias is loaded for each block, not held in 16 TN registers
-    // sums start at the bias: element e of a lane is column 8 (e / 4) + 4 half + e % 4 of the tile, row lane % 32
-    f16v acc[TN];
+  // sums start at the bias: element e of a lane is column 8 (e / 4) + 4 half + e % 4 of the tile, row lane % 32
+  __device__ __forceinline__ void begin(const Gemm& g, int64_t col0, int half) {
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -616,52 +647,62 @@ __global__ __launch_bounds__(WAVES * 64, 2) void rows_kernel(const Gemm g, const
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[j][e + i] = b[i];
       }
-    for (int kt = 0; kt < ktiles; ++kt) {
-      const char* from = lds + (RESIDENT ? kt : kt & 1) * STAGE;
-      if constexpr (RESIDENT) {
-        const int64_t after = block + (int64_t)gridDim.x * WAVES;
-        if (kt + 1 < ktiles) fetch_a(block, kt + 1, next);
-        else if (after < blocks) fetch_a(after, 0, next);
-      } else if (kt + 1 < ktiles) {
-        fetch_w(kt + 1);
-        fetch_a(block < blocks ? block : blocks - 1, kt + 1, next);
-      }
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        u4 x[PL];
-        if constexpr (PL == 3) {
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(cur[s].q[i / 4][i % 4]);
-          split8(v, x);
-        } else {
-          x[0] = cur[s].q[0];
-        }
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          u4 y[PL];
-#pragma unroll
-          for (int p = 0; p < PL; ++p)
-            y[p] = *reinterpret_cast<const u4*>(from + (((p * CH + 2 * s + half) * BN) + j * 32 + (lane & 31)) * 16);
-          if constexpr (PL == 3) {                             // small products first
-            acc[j] = mfma(y[0], x[2], acc[j], T());
-            acc[j] = mfma(y[2], x[0], acc[j], T());
-            acc[j] = mfma(y[1], x[1], acc[j], T());
-            acc[j] = mfma(y[0], x[1], acc[j], T());
-            acc[j] = mfma(y[1], x[0], acc[j], T());
-          }
-          acc[j] = mfma(y[0], x[0], acc[j], T());
-        }
-      }
-      if constexpr (!RESIDENT) {
-        if (kt + 1 < ktiles) store_w(lds + ((kt + 1) & 1) * STAGE);
-        __syncthreads();
-      }
-#pragma unroll
-      for (int s = 0; s < S; ++s) cur[s] = next[s];
-    }
+  }
 
-    const int64_t row = block * 32 + (lane & 31);
+  // stage kt of the row whose lane part begins at p; `to` may be another wave state's
+  static __device__ __forceinline__ void fetch(const T* p, int64_t K, int kt, int half, Eight<T> (&to)[S]) {
+    const T* q = p + (int64_t)kt * BK;
+    const int64_t left = K - (int64_t)kt * BK;
+    if (left >= BK) {
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int i = 0; i < 8 / Unit<T>::W; ++i) to[s].q[i] = load16(q + 16 * s + i * Unit<T>::W);
+    } else {
+#pragma unroll
+      for (int s = 0; s < S; ++s) load8(q + 16 * s, left - 8 * half - 16 * s, to[s]);
+    }
+  }
+
+  // `from` points at this lane's chunks: stage + ((lane / 32) BN + lane % 32) chunks. The next tile's chunks are read before
+  // a tile's products are issued.
+  __device__ __forceinline__ void multiply(const char* from) {
+    u4 y[2][PL];
+    auto read = [&](int s, int j, u4 (&to)[PL]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int p = 0; p < PL; ++p) to[p] = *reinterpret_cast<const u4*>(from + ((p * CH + 2 * s) * BN + j * 32) * 16);
+    };
+    read(0, 0, y[0]);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      u4 x[PL];
+      if constexpr (PL == 3) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(a[s].q[i / 4][i % 4]);
+        split8(v, x);
+      } else {
+        x[0] = a[s].q[0];
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int t = (s * TN + j) & 1;
+        if (j + 1 < TN) read(s, j + 1, y[t ^ 1]);
+        else if (s + 1 < S) read(s + 1, 0, y[t ^ 1]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (PL == 3) {                               // small products first
+          acc[j] = mfma(y[t][0], x[2], acc[j], T());
+          acc[j] = mfma(y[t][2], x[0], acc[j], T());
+          acc[j] = mfma(y[t][1], x[1], acc[j], T());
+          acc[j] = mfma(y[t][0], x[1], acc[j], T());
+          acc[j] = mfma(y[t][1], x[0], acc[j], T());
+        }
+        acc[j] = mfma(y[t][0], x[0], acc[j], T());
+      }
+    }
+  }
+
+  __device__ __forceinline__ void finish(const Gemm& g, int64_t row, int64_t col0, int half) {
     const bool in = row < g.M;
     if constexpr (PL == 3) {
       float seen = 0.f;                                       // 0, or NaN where a sum is not finite
@@ -676,7 +717,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void rows_kernel(const Gemm g, const
             const int64_t col = col0 + j * 32 + 8 * (e / 4) + 4 * half + e % 4;
             float t = acc[j][e];
             if (in && col < g.N && !(fabsf(t) < __builtin_huge_valf())) {
-              const T* x = a + row * g.lda;
+              const T* x = (const T*)g.a + row * g.lda;
               const T* y = (const T*)g.b + (g.b_along ? col * g.ldb : col);
               t = 0.f;
               for (int64_t k = 0; k < g.K; ++k) t = fmaf((float)x[k], (float)y[g.b_along ? k : k * g.ldb], t);
@@ -687,15 +728,114 @@ __global__ __launch_bounds__(WAVES * 64, 2) void rows_kernel(const Gemm g, const
         });
       }
     }
-    switch (g.act) {
-      case ACT_RELU: rows_out<T, TN, ACT_RELU>(g, acc, row, col0, half, in); break;
-      case ACT_GELU: rows_out<T, TN, ACT_GELU>(g, acc, row, col0, half, in); break;
-      case ACT_SILU: rows_out<T, TN, ACT_SILU>(g, acc, row, col0, half, in); break;
-      default: rows_out<T, TN, ACT_NONE>(g, acc, row, col0, half, in);
+    // all of the residual is on its way before the first store: the compiler may not move a load over one
+    u4 res[TN][Out<T>::PIECES];
+    if (g.residual) {
+      const T* r = (const T*)g.residual + row * g.ld_residual + col0;
+      each<0, TN>([&](auto j) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < Out<T>::PIECES; ++q) {
+          const int64_t col = j * 32 + Out<T>::column(q, half), left = in ? g.N - col0 - col : 0;
+          res[j][q] = load_piece(r + col, left >= Out<T>::WIDE ? Out<T>::WIDE : left > 0 ? (int)left : 0);
+        }
+      });
     }
-    if constexpr (!RESIDENT) break;
-    block += (int64_t)gridDim.x * WAVES;
-    if (block >= blocks) break;
+    switch (g.act) {
+      case ACT_RELU: rows_out<T, TN, ACT_RELU>(g, acc, res, row, col0, half, in); break;
+      case ACT_GELU: rows_out<T, TN, ACT_GELU>(g, acc, res, row, col0, half, in); break;
+      case ACT_SILU: rows_out<T, TN, ACT_SILU>(g, acc, res, row, col0, half, in); break;
+      default: rows_out<T, TN, ACT_NONE>(g, acc, res, row, col0, half, in);
+    }
+  }
+};
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+// W's stages go round two buffers in LDS, copied there by the memory unit itself while the stage before is multiplied; each
+// buffer is an array of its own, so that the compiler sees that a copy into one does not touch the reads of the other.
+template <typename T, int TN, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 3) void rows_kernel(const Gemm g, const char* image, int ktiles) {
+  using V = Wave<T, TN>;
+  constexpr int STAGE = V::STAGE, PIECES = STAGE / 1024, PER = (PIECES + WAVES - 1) / WAVES;
+  __shared__ __attribute__((aligned(16))) char even[STAGE];
+  __shared__ __attribute__((aligned(16))) char odd[STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  // consecutive workgroups go round the 8 XCDs: the column tiles of a row block stay on one of them, one after the other
+  const int64_t ntiles = (g.N + V::BN - 1) / V::BN, turn = blockIdx.x / 8;
+  const int64_t nt = turn % ntiles, group = turn / ntiles * 8 + blockIdx.x % 8;
+  const int64_t row = (group * WAVES + wave) * 32 + (lane & 31);
+  if (group * WAVES * 32 >= g.M) return;
+  const char* w = image + nt * ktiles * STAGE + lane * 16;
+  const T* p = (const T*)g.a + (row < g.M ? row : g.M - 1) * g.lda + 8 * half;
+  auto send = [&](int kt, char* to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      int piece = i * WAVES + wave;
+      piece = PIECES % WAVES == 0 || piece < PIECES ? piece : PIECES - 1;
+      __builtin_amdgcn_global_load_lds((const void*)(w + (int64_t)kt * STAGE + piece * 1024), (lds_ptr)(to + piece * 1024), 16, 0, 0);
+    }
+  };
+  // everything on its way has arrived, and every wave is done with what it read
+  auto meet = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+
+  V v;
+  Eight<T> next[V::S];
+  send(0, even);
+  V::fetch(p, g.K, 0, half, v.a);
+  v.begin(g, nt * V::BN, half);
+  meet();
+  auto step = [&](int kt, const char* from, char* to) __attribute__((always_inline)) {
+    if (kt + 1 < ktiles) {
+      send(kt + 1, to);
+      V::fetch(p, g.K, kt + 1, half, next);
+    }
+    v.multiply(from + ((lane >> 5) * V::BN + (lane & 31)) * 16);
+    meet();
+#pragma unroll
+    for (int s = 0; s < V::S; ++s) v.a[s] = next[s];
+  };
+  for (int kt = 0; kt < ktiles; kt += 2) {
+    step(kt, even, odd);
+    if (kt + 1 < ktiles) step(kt + 1, odd, even);
+  }
+  v.finish(g, row, nt * V::BN, half);
+}
+
+// The same where the whole image of W fits LDS: it is copied there once, and the waves walk over row blocks on their own,
+// the next stage of rows (the next block's first one at the end) always on its way.
+template <typename T, int TN, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void rows_resident_kernel(const Gemm g, const char* image, int ktiles) {
+  using V = Wave<T, TN>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  for (int i = tid; i < ktiles * (V::STAGE / 16); i += WAVES * 64) reinterpret_cast<u4*>(lds)[i] = reinterpret_cast<const u4*>(image)[i];
+  __syncthreads();
+  const int64_t blocks = (g.M + 31) / 32, stride = (int64_t)gridDim.x * WAVES;
+  int64_t block = (int64_t)blockIdx.x * WAVES + wave;
+  if (block >= blocks) return;
+  auto part = [&](int64_t at) __attribute__((always_inline)) {
+    const int64_t row = at * 32 + (lane & 31);
+    return (const T*)g.a + (row < g.M ? row : g.M - 1) * g.lda + 8 * half;
+  };
+  V v;
+  Eight<T> next[V::S];
+  const T* p = part(block);
+  V::fetch(p, g.K, 0, half, v.a);
+  for (; block < blocks; block += stride) {
+    asm volatile("" ::: "memory");                            // the bias is loaded for each block, not held in 16 TN registers
+    v.begin(g, 0, half);
+    for (int kt = 0; kt < ktiles; ++kt) {
+      if (kt + 1 < ktiles) {
+        V::fetch(p, g.K, kt + 1, half, next);
+      } else if (block + stride < blocks) {
+        p = part(block + stride);
+        V::fetch(p, g.K, 0, half, next);
+      }
+      v.multiply(lds + kt * V::STAGE + ((lane >> 5) * V::BN + (lane & 31)) * 16);
+#pragma unroll
+      for (int s = 0; s < V::S; ++s) v.a[s] = next[s];
+    }
+    v.finish(g, block * 32 + (lane & 31), 0, half);
   }
 }
 
@@ -725,11 +865,11 @@ int rows_launch(const Gemm& g, char* image) {
     constexpr int WAVES = 8;
     const int64_t per = ktiles * STAGE <= 64 * 1024 ? 2 : 1;          // workgroups a compute unit
     const int64_t want = (blocks + WAVES - 1) / WAVES, most = 256 * per;
-    hipLaunchKernelGGL((rows_kernel<T, TN, WAVES, true>), dim3((uint32_t)(want < most ? (want + 7) / 8 * 8 : most), 1), dim3(WAVES * 64), (uint32_t)(ktiles * STAGE),
+    hipLaunchKernelGGL((rows_resident_kernel<T, TN, WAVES>), dim3((uint32_t)(want < most ? want : most)), dim3(WAVES * 64), (uint32_t)(ktiles * STAGE),
                        g.stream, g, image, (int)ktiles);
   } else {
     constexpr int WAVES = 4;
-    hipLaunchKernelGGL((rows_kernel<T, TN, WAVES, false>), dim3((uint32_t)(((blocks + WAVES - 1) / WAVES + 7) / 8 * 8 * ntiles)), dim3(WAVES * 64), 2 * STAGE,
+    hipLaunchKernelGGL((rows_kernel<T, TN, WAVES>), dim3((uint32_t)(((blocks + WAVES - 1) / WAVES + 7) / 8 * 8 * ntiles)), dim3(WAVES * 64), 0,
                        g.stream, g, image, (int)ktiles);
   }
   DGNN_LAUNCHED();
