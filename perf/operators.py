@@ -180,6 +180,8 @@ def prepare(case, seed):
                              master_weights=case["master"])
         given = opt.state_dict()
         opt.load_state_dict({"state": _state_dict(s), "param_groups": given["param_groups"]})
+        for name, t in opt.state_buffers().items():
+            t.copy_(s[name])     # what lies between the tensors too: it comes back with the buffers
         for name in STATE[case["bits"]] + ("master", "place"):
             s[name] = None       # the optimiser has its own now
         s["opt"], s["params"] = opt, params
