@@ -318,4 +318,52 @@ int dgnn_linear_grad_weight(const void* x, int64_t ldx, const void* p, int64_t l
   return run(g, dtype, workspace, workspace_bytes, "linear_grad_weight");
 }
 
+// Everything a gradient dy of y gives, in one call: what the three entries above compute, in the same order on the stream, so
+// that one workspace serves them one after the other behind p's part of it.
+static int64_t backward_parts(int64_t M, int64_t K, int64_t N, int32_t dtype, int32_t act, int64_t* p_bytes) {
+  int64_t most = 0;
+  for (int32_t pass = DGNN_LINEAR_SLOPE; pass <= DGNN_LINEAR_GRAD_WEIGHT; ++pass) {
+    int64_t n = 0;
+    (void)dgnn_linear_workspace(pass, M, K, N, dtype, &n);
+    if (n > most) most = n;
+  }
+  *p_bytes = act == ACT_NONE ? 0 : ceil_div(M * N * width(dtype), 256) * 256;
+  return *p_bytes + most;
+}
+
+int dgnn_linear_backward_workspace(int64_t M, int64_t K, int64_t N, int32_t dtype, int32_t act, int64_t* bytes) {
+  if (!bytes || !known_type(dtype) || !sizes_ok(M, K, N) || act < ACT_NONE || act > ACT_SILU)
+    return dgnn_fail(DGNN_E_BADARG, "linear_backward_workspace: bad argument%s");
+  int64_t p;
+  *bytes = backward_parts(M, K, N, dtype, act, &p);
+  return DGNN_OK;
+}
+
+int dgnn_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* dy, int64_t ldd,
+                         const void* save, int64_t lds, void* dx, int64_t lddx, void* dw, int64_t lddw, void* dbias,
+                         int64_t M, int64_t K, int64_t N, int32_t dtype, int32_t act,
+                         void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!known_type(dtype)) return dgnn_fail(DGNN_E_BADARG, "linear_backward: unknown type%s (%lld)", "", dtype);
+  if (act < ACT_NONE || act > ACT_SILU) return dgnn_fail(DGNN_E_BADARG, "linear_backward: unknown activation%s (%lld)", "", act);
+  if (!sizes_ok(M, K, N)) return dgnn_fail(DGNN_E_BADARG, "linear_backward: bad sizes%s");
+  int64_t p_bytes;
+  const int64_t need = backward_parts(M, K, N, dtype, act, &p_bytes);
+  if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+    return dgnn_fail(DGNN_E_BADARG, "linear_backward: workspace too small or misaligned%s (%lld bytes wanted)", "", need);
+  char* rest = (char*)workspace + p_bytes;
+  const void* p = dy;
+  int64_t ldp = ldd;
+  if (act != ACT_NONE || dbias) {
+    void* to = act != ACT_NONE && M > 0 && N > 0 ? workspace : nullptr;
+    const int rc = dgnn_linear_slope(dy, ldd, save, lds, to, N, dbias, M, N, dtype, act, rest, need - p_bytes, stream);
+    if (rc != DGNN_OK) return rc;
+    if (act != ACT_NONE) { p = workspace; ldp = N; }
+  }
+  if (dx) {
+    const int rc = dgnn_linear_grad_input(p, ldp, w, ldw, nullptr, 0, dx, lddx, M, K, N, dtype, rest, need - p_bytes, stream);
+    if (rc != DGNN_OK) return rc;
+  }
+  return dw ? dgnn_linear_grad_weight(x, ldx, p, ldp, dw, lddw, M, K, N, dtype, rest, need - p_bytes, stream) : DGNN_OK;
+}
+
 }  // extern "C"

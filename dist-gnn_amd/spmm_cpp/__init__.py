@@ -96,6 +96,8 @@ _TRAIN_SIGNATURES = {                    # argument types, in the order of inclu
     'dgnn_linear_slope': [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i32, _i32, _p, _i64, _p],
     'dgnn_linear_grad_input': [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _p, _i64, _p],
     'dgnn_linear_grad_weight': [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _p, _i64, _p],
+    'dgnn_linear_backward_workspace': [_i64, _i64, _i64, _i32, _i32, _pi64],
+    'dgnn_linear_backward': [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _i32, _p, _i64, _p],
     'dgnn_adamw': [_p, _i32, _i32, _i32, _p, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, _p],
 }
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}         # DGNN_F32, DGNN_BF16, DGNN_F16

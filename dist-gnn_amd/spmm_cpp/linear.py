@@ -158,7 +158,7 @@ class _Linear(torch.autograd.Function):
         wanted = ctx.needs_input_grad
         y, saved = linear_forward(x, weight, bias, activation, residual, save=any(wanted[:3]))
         ctx.save_for_backward(x if wanted[1] else None, weight if wanted[0] else None, saved)
-        ctx.activation = activation
+        ctx.act, ctx.K = ACTIVATIONS[activation], x.shape[1]
         return y
 
     @staticmethod
@@ -168,13 +168,33 @@ class _Linear(torch.autograd.Function):
         want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if want_x or want_w or want_b:
-            if dy.dim() == 2 and (dy.stride(1) != 1 and dy.size(1) > 1 or dy.stride(0) < dy.size(1) and dy.size(0) > 1):
-                dy = dy.contiguous()                                  # an expanded or transposed gradient
-            p, db = linear_slope(dy, saved, ctx.activation, want_b)
-            if want_x:
-                dx = linear_grad_input(p, weight)
-            if want_w:
-                dw = linear_grad_weight(x, p)
+            # one call for all of them (x, weight and saved were checked when they were saved; dy is of y's shape and type)
+            (M, N), K, act = dy.shape, ctx.K, ctx.act
+            ldd, s1 = dy.stride()
+            if s1 != 1 and N > 1 or ldd < N and M > 1:                # an expanded or transposed gradient
+                dy = dy.contiguous()
+                ldd = N
+            dtype, dev = dy.dtype, dy.device
+            code = _DTYPES[dtype]
+            with torch.cuda.device(dev):
+                need = ctypes.c_int64()
+                _check(_lib.dgnn_linear_backward_workspace(M, K, N, code, act, ctypes.byref(need)), 'linear_backward')
+                ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+                xp = wp = dxp = dwp = dbp = sp = None
+                ldx = ldw = lds = 0
+                if want_x:
+                    dx = torch.empty((M, K), dtype=dtype, device=dev)
+                    dxp, wp, ldw = dx.data_ptr(), weight.data_ptr(), weight.stride(0) if K > 1 else max(N, 1)
+                if want_w:
+                    dw = torch.empty((K, N), dtype=dtype, device=dev)
+                    dwp, xp, ldx = dw.data_ptr(), x.data_ptr(), x.stride(0) if M > 1 else max(K, 1)
+                if want_b:
+                    db = torch.empty(N, dtype=dtype, device=dev)
+                    dbp = db.data_ptr()
+                if saved is not None:
+                    sp, lds = saved.data_ptr(), max(saved.shape[1], 1)
+                _check(_lib.dgnn_linear_backward(xp, ldx, wp, ldw, dy.data_ptr(), max(ldd, N) if M > 1 else max(N, 1), sp, lds, dxp, max(K, 1), dwp,
+                                                 max(N, 1), dbp, M, K, N, code, act, ws.data_ptr(), need.value, _stream(dy)), 'linear_backward')
         return dx, dw, db, dy if want_r else None, None
 
 

@@ -30,6 +30,8 @@ extern "C" {
  *                             dy itself. act DGNN_ACT_NONE: p is a copy of dy
  *   dgnn_linear_grad_input    dx = p W^T + add    (add [M x K] or NULL: what else reaches x, a skip connection's gradient)
  *   dgnn_linear_grad_weight   dw = x^T p      (M = 0: zeros)
+ *   dgnn_linear_backward      all of them in one call, p in the workspace; dx, dw and dbias may be NULL (x, w and save are then
+ *                             only needed for what is asked for). Its workspace: dgnn_linear_backward_workspace
  * workspace: device memory of dgnn_linear_workspace(pass, ...) bytes, 16-byte aligned (0 bytes: may be NULL), free to be used
  * again once the call's kernels have run. Sums over many rows are cut by a rule of the sizes alone and joined in a fixed
  * order: the same bits every run. Outputs must not overlap inputs (but p may be dy).
@@ -53,6 +55,11 @@ int dgnn_linear_grad_input(const void* p, int64_t ldp, const void* w, int64_t ld
                            void* dx, int64_t ldx, int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
 int dgnn_linear_grad_weight(const void* x, int64_t ldx, const void* p, int64_t ldp, void* dw, int64_t ldw,
                             int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int dgnn_linear_backward_workspace(int64_t M, int64_t K, int64_t N, int32_t dtype, int32_t act, int64_t* bytes);
+int dgnn_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* dy, int64_t ldd,
+                         const void* save, int64_t lds, void* dx, int64_t lddx, void* dw, int64_t lddw, void* dbias,
+                         int64_t M, int64_t K, int64_t N, int32_t dtype, int32_t act,
+                         void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * One AdamW step over `count` tensors (a handful of launches for hundreds of them). With g a tensor's gradient, t the

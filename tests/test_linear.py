@@ -26,6 +26,11 @@ def _grad_weight(x=A, ldx=8, p=B, ldp=8, dw=C, ldw=8, M=4, K=8, N=8, dtype=0, ws
     return lib.dgnn_linear_grad_weight(x, ldx, p, ldp, dw, ldw, M, K, N, dtype, ws, n, None)
 
 
+def _backward(x=A, ldx=8, w=B, ldw=8, dy=C, ldd=8, save=D, lds=8, dx=5 << 22, lddx=8, dw=6 << 22, lddw=8, db=7 << 22, M=4, K=8, N=8, dtype=0, act=2,
+              ws=8 << 22, n=1 << 20):
+    return lib.dgnn_linear_backward(x, ldx, w, ldw, dy, ldd, save, lds, dx, lddx, dw, lddw, db, M, K, N, dtype, act, ws, n, None)
+
+
 @pytest.mark.parametrize('call,kw', [
     (_forward, dict(dtype=3)), (_forward, dict(act=4)), (_forward, dict(act=-1)), (_forward, dict(M=-1)), (_forward, dict(K=1 << 31)),
     (_forward, dict(x=None)), (_forward, dict(w=None)), (_forward, dict(y=None)), (_forward, dict(ldx=7)), (_forward, dict(ldw=7)),
@@ -35,6 +40,8 @@ def _grad_weight(x=A, ldx=8, p=B, ldp=8, dw=C, ldw=8, M=4, K=8, N=8, dtype=0, ws
     (_slope, dict(dtype=-1)), (_slope, dict(act=9)), (_slope, dict(save=None)), (_slope, dict(lds=7)), (_slope, dict(dy=None)),
     (_slope, dict(ldp=7)), (_slope, dict(act=1, lds=0)), (_slope, dict(db=D)), (_slope, dict(db=D, ws=D, n=4)), (_slope, dict(db=D + 2)),
     (_grad_input, dict(dtype=5)), (_grad_input, dict(p=None)), (_grad_input, dict(ldx=7)), (_grad_input, dict(dx=A)), (_grad_input, dict(add=D, lda=7)), (_grad_input, dict(add=C)), (_grad_input, dict(N=-2)),
+    (_backward, dict(dtype=5)), (_backward, dict(act=4)), (_backward, dict(M=-1)), (_backward, dict(ws=None)), (_backward, dict(n=100)),
+    (_backward, dict(ws=(8 << 22) + 8)), (_backward, dict(dy=None)), (_backward, dict(save=None)),
     (_grad_weight, dict(dtype=5)), (_grad_weight, dict(x=None)), (_grad_weight, dict(ldw=7)), (_grad_weight, dict(dw=B)),
     (_grad_weight, dict(M=1 << 31)), (_grad_weight, dict(M=100000, dw=1 << 40)),                                # cut, no workspace
 ])
