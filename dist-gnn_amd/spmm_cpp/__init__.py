@@ -1465,5 +1465,22 @@ def _dense_for(A):
 
 
 # --------------------------------------------------------------------------- what a training step computes beside the aggregation
+def _load_torch_binding():
+    """lib/_dgnn_torch.so: the host side of the training operators over the same library."""
+    import importlib.util
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), '..', 'lib', '_dgnn_torch.so')
+    if not os.path.exists(path):
+        raise RuntimeError(f'spmm_cpp: {os.path.normpath(path)} is missing -- build it with '
+                           '`python -c "import __graft_entry__ as g; g.build()"`. There is no fallback.')
+    spec = importlib.util.spec_from_file_location('_dgnn_torch', path)
+    ext = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ext)
+    ext.bind([ctypes.cast(getattr(_lib, n), ctypes.c_void_p).value for n in
+              ('dgnn_last_error', 'dgnn_linear_workspace', 'dgnn_linear_forward', 'dgnn_linear_slope', 'dgnn_linear_grad_input',
+               'dgnn_linear_grad_weight', 'dgnn_linear_backward_workspace', 'dgnn_linear_backward', 'dgnn_adamw')])
+    return ext
+
+
+_ext = _load_torch_binding()
 from .adamw import AdamW  # noqa: E402,F401
 from .linear import ACTIVATIONS, linear, linear_forward, linear_grad_input, linear_grad_weight, linear_slope  # noqa: E402,F401

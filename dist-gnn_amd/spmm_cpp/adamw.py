@@ -4,27 +4,14 @@ The reference's training loop steps ``torch.optim.Adam`` (light_dist_gnn/dist_tr
 parameter. Here a step is one pass over parameter, gradient and moments, for up to 64 tensors a launch, with the moments
 in 32 or in 8 bits.
 """
-import ctypes
 import math
-import operator
 
 import numpy as np
 import torch
 
-from . import _check, _lib, _stream, _DTYPES
-
-_T, _NONE = torch.Tensor, type(None)
-_grad_of, _dtype_of, _layout_of = operator.attrgetter('grad'), operator.attrgetter('dtype'), operator.attrgetter('is_sparse')
+from . import _DTYPES, _ext
 
 BLOCK = 256                       # elements that share a scale; a tensor starts at a multiple of it in the state buffers
-
-_TENSOR = np.dtype([('param', np.uint64), ('grad', np.uint64), ('numel', np.int64), ('start', np.int64), ('decay', np.float32),
-                    ('rate', np.float32), ('root', np.float32), ('turn', np.uint32), ('index', np.int32), ('reserved', np.int32)])
-
-
-class _CState(ctypes.Structure):          # struct dgnn_adamw_state (include/dgnn_train.h)
-    _fields_ = [(n, ctypes.c_void_p) for n in ('exp_avg', 'exp_avg_sq', 'exp_avg_scale', 'exp_avg_sq_scale', 'master',
-                                               'steps', 'factors')]
 
 
 def _kinds(bits, master):
@@ -41,7 +28,7 @@ def _kinds(bits, master):
 
 class _Segment:
     """The parameters of one group that share a device and a type, and their state: one flat buffer per kind, every tensor's
-    part starting at a multiple of 256 elements. What the kernel's table needs of them and does not change is kept filled."""
+    part starting at a multiple of 256 elements."""
 
     def __init__(self, params, bits, master, capturable):
         self.params, self.bits, self.has_master, self.capturable = params, bits, master, capturable
@@ -49,7 +36,6 @@ class _Segment:
         sizes = np.array([p.numel() for p in params], dtype=np.int64)
         blocks = -(-sizes // BLOCK)
         self.starts = (np.cumsum(blocks) - blocks) * BLOCK
-        self.size_list, self.where = sizes.tolist(), None
         self.sizes, total = sizes, int(blocks.sum()) * BLOCK
         self.kinds = _kinds(bits, master)
         self.flat = {}
@@ -60,21 +46,11 @@ class _Segment:
             self.steps = torch.zeros(len(params), dtype=torch.int64, device=self.device)
             self.factors = torch.zeros(len(params), 4, dtype=torch.float32, device=self.device)
         else:
-            self.host_steps = np.zeros(len(params), dtype=np.int64)
-            self.steps = torch.from_numpy(self.host_steps)
-        self.table = np.zeros(len(params), dtype=_TENSOR)
-        self.table['numel'], self.table['start'] = sizes, self.starts
-        self.table['index'] = np.arange(len(params))
-        st = self.cstate = _CState()
+            self.steps = torch.zeros(len(params), dtype=torch.int64)
         f = self.flat
-        st.exp_avg = f['exp_avg'].data_ptr()
-        st.exp_avg_sq = f['exp_avg_sq' if bits == 32 else 'exp_avg_rms'].data_ptr()
-        if bits == 8:
-            st.exp_avg_scale, st.exp_avg_sq_scale = f['exp_avg_scale'].data_ptr(), f['exp_avg_rms_scale'].data_ptr()
-        if master:
-            st.master = f['master'].data_ptr()
-        if capturable:
-            st.steps, st.factors = self.steps.data_ptr(), self.factors.data_ptr()
+        self.table = _ext.AdamTable(params, self.starts.tolist(), bits, f['exp_avg'], f['exp_avg_sq' if bits == 32 else 'exp_avg_rms'],
+                                    f.get('exp_avg_scale'), f.get('exp_avg_rms_scale'), f.get('master'), self.steps,
+                                    self.factors if capturable else None)
 
     def views(self, i):
         """The state dict entry of parameter i: views of the flat buffers."""
@@ -234,55 +210,11 @@ class AdamW(torch.optim.Optimizer):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError('AdamW: take a step or call init_state() before capturing one in a graph')
             self.init_state()
+        capturing = not self.capturable and torch.cuda.is_current_stream_capturing()
         for group, segments in zip(self.param_groups, self._segments):
-            for seg in segments:
-                self._step_segment(group, seg)
-        return loss
-
-    def _step_segment(self, group, seg):
-        # The host's time a step is what a few attributes of every tensor cost (0.14 us each): they are read column by column
-        # in C loops. A parameter at the address that it had in the last step is the tensor that was checked then.
-        params, table, sizes = seg.params, seg.table, seg.size_list
-        grads = list(map(_grad_of, params))
-        live = slice(None)
-        if _NONE in set(map(type, grads)):
-            live = [i for i, g in enumerate(grads) if g is not None]
-            if not live:
-                return
-            params, grads, sizes, table = [params[i] for i in live], [grads[i] for i in live], [sizes[i] for i in live], table[live]
-        dev, dtype, n = seg.device, seg.dtype, len(params)
-        where = list(map(_T.data_ptr, params))
-        if where != seg.where:
-            if any(p.device != dev or p.dtype is not dtype or not p.is_contiguous() for p in params):
-                raise RuntimeError(f'AdamW: a parameter is not a contiguous {dtype} tensor on {dev} any more')
-        if list(map(_dtype_of, grads)).count(dtype) != n or list(map(_T.get_device, grads)).count(dev.index) != n:
-            raise RuntimeError(f'AdamW: a gradient is not {dtype} on {dev}, as its parameter is')
-        if any(map(_layout_of, grads)):
-            raise RuntimeError('AdamW: a gradient is sparse')
-        if list(map(_T.numel, params)) != sizes or list(map(_T.numel, grads)) != sizes:
-            raise RuntimeError('AdamW: a parameter or its gradient changed its size')
-        if list(map(_T.is_contiguous, grads)).count(True) != n:
-            grads = [g.contiguous() for g in grads]
-        with torch.cuda.device(dev):
-            if not seg.capturable and torch.cuda.is_current_stream_capturing():
+            if capturing and any(p.grad is not None for p in group['params']):
                 raise RuntimeError('AdamW: a step is captured in a graph, but the optimiser was made without capturable=True')
             b1, b2 = group['betas']
-            lr = float(group['lr'])
-            table['param'] = where
-            table['grad'] = list(map(_T.data_ptr, grads))
-            table['decay'] = 1.0 - lr * group['weight_decay']
-            if not seg.capturable:
-                steps = seg.host_steps[live] + 1
-                first = int(steps[0])
-                if (steps == first).all():
-                    table['rate'], table['root'] = lr / (1.0 - b1 ** first), 1.0 / math.sqrt(1.0 - b2 ** first)
-                else:
-                    table['rate'], table['root'] = lr / (1.0 - b1 ** steps.astype(np.float64)), 1.0 / np.sqrt(1.0 - b2 ** steps.astype(np.float64))
-                table['turn'] = steps & 0xFFFFFFFF
-            _check(_lib.dgnn_adamw(table.ctypes.data, n, _DTYPES[dtype], seg.bits, ctypes.byref(seg.cstate), lr, b1, b2,
-                                   float(group['eps']), _stream(params[0])), 'adamw')
-        seg.where = where
-        if not seg.capturable:
-            seg.host_steps[live] += 1
-        # the kernel writes behind autograd's back: a graph that saved a parameter has to notice
-        torch.autograd.graph.increment_version(params)
+            for seg in segments:
+                seg.table.step(float(group['lr']), b1, b2, float(group['eps']), float(group['weight_decay']))
+        return loss
