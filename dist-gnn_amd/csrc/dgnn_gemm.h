@@ -414,35 +414,49 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm g) {
                               col0 + wn * TN * 32, k0, kend);
 }
 
-// Joins the slices of a product that was cut along its contraction, in their order, and finishes it: 4 columns of a row a
-// lane, 8 slices' loads in flight. A row takes a multiple of 8 lanes, so that relu's bits are whole words.
+// Joins the slices of a product that was cut along its contraction and finishes it: 32 fours of columns a workgroup, 8 lanes
+// to a four, each adding every 8th slice with up to 8 loads in flight; the 8 sums meet in their order. A row takes a multiple of
+// 8 fours, so that relu's bits are whole words.
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_join_kernel(const Gemm g) {
+  __shared__ __attribute__((aligned(16))) float sums[8][32][4];
+  const int four = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int64_t wide = (g.N + 31) / 32 * 8;
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t at = (int64_t)blockIdx.x * 32 + four;
   const int64_t row = at / wide, col = at % wide * 4;
   const int have = row < g.M && col < g.N ? (g.N - col >= 4 ? 4 : (int)(g.N - col)) : 0;
-  float v[4] = {0.f, 0.f, 0.f, 0.f}, bias[4] = {0.f, 0.f, 0.f, 0.f}, res[4] = {0.f, 0.f, 0.f, 0.f};
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
   if (have) {
     const float* p = g.partial + row * g.N + col;
     const int64_t step = g.M * g.N;
-    for (int s = 0; s < g.slices; s += 8) {
+    for (int s = part; s < g.slices; s += 64) {
       float t[8][4];
 #pragma unroll
       for (int u = 0; u < 8; ++u)
-        if (s + u < g.slices) load4(p + (s + u) * step, have, t[u]);
+        if (s + 8 * u < g.slices) load4(p + (s + 8 * u) * step, have, t[u]);
 #pragma unroll
       for (int u = 0; u < 8; ++u)
-        if (s + u < g.slices) {
+        if (s + 8 * u < g.slices) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[i] += t[u][i];
         }
     }
-    if (g.bias) load4((const T*)g.bias + col, have, bias);
-    if (g.residual) load4((const T*)g.residual + row * g.ld_residual + col, have, res);
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sums[part][four][i] = v[i];
+  __syncthreads();
+  if (part) return;
+  float bias[4] = {0.f, 0.f, 0.f, 0.f}, res[4] = {0.f, 0.f, 0.f, 0.f};
+  if (have && g.bias) load4((const T*)g.bias + col, have, bias);
+  if (have && g.residual) load4((const T*)g.residual + row * g.ld_residual + col, have, res);
+#pragma unroll
+  for (int k = 1; k < 8; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += sums[k][four][i];
   finish<T>(g, row, col, have, v, bias, res);
 }
+
+inline uint32_t join_blocks(const Gemm& g) { return (uint32_t)((g.M * ((g.N + 31) / 32 * 8) + 31) / 32); }
 
 // ---------------------------------------------------------------------------------------
 // Many rows (forward and input gradient of whole graphs or batches). W is laid out first, once a call: zero-padded chunks in the
@@ -876,6 +890,198 @@ int rows_launch(const Gemm& g, char* image) {
   return DGNN_OK;
 }
 
+// ---------------------------------------------------------------------------------------
+// A handful of rows (1..8): W's bytes are all there is, each is used once a row, so plain fused multiply-adds in fp32 keep up
+// and no sum is split over workgroups -- one launch. thin_across: W[k][n] with n contiguous; LANES lanes take 16 bytes each
+// of a row of W, the others and the 16 waves further rows, all loads of a lane are on their way together, and the rows'
+// sums meet by exchanges in the wave and through LDS. LANES is as small as it takes to have a workgroup for every compute unit;
+// neighbouring column blocks, which share cache lines, run on one XCD. thin_along: W[n][k] with the contraction contiguous; a
+// wave takes COLS outputs and all lanes their contraction.
+// ---------------------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ void thin_out(const Gemm& g, int64_t row, int64_t col, float t) {
+  if (g.save && g.act > ACT_RELU) ((T*)g.save)[row * g.ld_save + col] = (T)t;
+  t = act_of(g.act, t);
+  if (g.residual) t += (float)((const T*)g.residual)[row * g.ld_residual + col];
+  ((T*)g.c)[row * g.ldc + col] = (T)t;
+}
+
+template <typename T> __device__ __forceinline__ void widen16(u4 v, float (&out)[Unit<T>::W]) {
+  union { u4 u; T e[Unit<T>::W]; } r;
+  r.u = v;
+#pragma unroll
+  for (int i = 0; i < Unit<T>::W; ++i) out[i] = (float)r.e[i];
+}
+
+template <typename T, int ROWS, int WAVES, int U, int LEAST, int MOST>      // LEAST <= lanes <= MOST
+__global__ __launch_bounds__(WAVES * 64) void thin_across_kernel(const Gemm g, int lanes) {
+  constexpr int W = Unit<T>::W, WIDE = MOST * W, STAGED = 64 / LEAST * WAVES * U;
+  __shared__ __attribute__((aligned(16))) float room[ROWS * (STAGED > WAVES * WIDE ? STAGED : WAVES * WIDE)];
+  const int64_t kbeg = (int64_t)blockIdx.y * g.slice_k, kend = kbeg + g.slice_k < g.K ? kbeg + g.slice_k : g.K;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t each_xcd = (gridDim.x + 7) / 8, block = (int64_t)(blockIdx.x % 8) * each_xcd + blockIdx.x / 8;
+  const int64_t col = (block * lanes + lane % lanes) * W, left = g.N - col;
+  const int per = 64 / lanes * WAVES, mine = wave * (64 / lanes) + lane / lanes;      // rows of W a pass, this lane's among them
+  const T* w = (const T*)g.b + col;
+  const T* x = (const T*)g.a;
+  float acc[ROWS][W];
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+    for (int i = 0; i < W; ++i) acc[m][i] = 0.f;
+  for (int64_t base = kbeg; base < kend; base += (int64_t)per * U) {
+    u4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = base + u * per + mine;
+      v[u] = u4{0, 0, 0, 0};
+      if (k < kend && left > 0) v[u] = left >= W ? load16(w + k * g.ldb) : load_some(w + k * g.ldb, left);
+    }
+    __syncthreads();
+    for (int at = threadIdx.x; at < per * U * ROWS; at += WAVES * 64) {          // x's part, widened, the rows of a k side by side
+      const int k = at % (per * U), m = at / (per * U);
+      room[k * ROWS + m] = m < g.M && base + k < kend ? (float)x[m * g.lda + base + k] : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (base + u * per + mine >= kend) continue;
+      float f[W];
+      widen16<T>(v[u], f);
+      const float* s = room + (u * per + mine) * ROWS;
+#pragma unroll
+      for (int m = 0; m < ROWS; ++m) {
+        const float sm = s[m];
+#pragma unroll
+        for (int i = 0; i < W; ++i) acc[m][i] = fmaf(sm, f[i], acc[m][i]);
+      }
+    }
+  }
+  __syncthreads();
+  for (int d = lanes; d < 64; d <<= 1)
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+      for (int i = 0; i < W; ++i) acc[m][i] += __shfl_xor(acc[m][i], d);
+  if (lane < lanes)
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+      for (int i = 0; i < W; ++i) room[(wave * ROWS + m) * WIDE + lane * W + i] = acc[m][i];
+  __syncthreads();
+  const int wide = lanes * W;
+  for (int at = threadIdx.x; at < (ROWS * wide + 63) / 64 * 64; at += WAVES * 64) {      // whole waves: relu's bits are gathered below
+    const int m = at / wide, c = at % wide;
+    const int64_t n = block * wide + c;
+    const bool in = m < ROWS && m < g.M && n < g.N;
+    float t = 0.f;
+    if (in) {
+#pragma unroll
+      for (int k = 0; k < WAVES; ++k) t += room[(k * ROWS + m) * WIDE + c];
+      if (g.slices > 1) g.partial[((int64_t)blockIdx.y * g.M + m) * g.N + n] = t;
+      else if (g.bias) t += (float)((const T*)g.bias)[n];
+    }
+    if (g.slices > 1) continue;
+    if (g.save && g.act == ACT_RELU) {                         // a byte for 8 columns, up to the end of the row's last word
+      const uint64_t bits = __ballot(in && !(t <= 0.f));
+      if ((c & 7) == 0 && m < ROWS && m < g.M && n < (g.N + 31) / 32 * 32)
+        ((uint8_t*)((uint32_t*)g.save + m * g.ld_save))[n / 8] = (uint8_t)(bits >> (lane & 56));
+    }
+    if (in) thin_out<T>(g, m, n, t);
+  }
+}
+
+template <typename T, int ROWS, int COLS>
+__global__ __launch_bounds__(256) void thin_along_kernel(const Gemm g) {
+  constexpr int W = Unit<T>::W;
+  const int lane = threadIdx.x & 63;
+  const int64_t col = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * COLS;
+  if (col >= g.N) return;
+  const T* x = (const T*)g.a;
+  float acc[ROWS][COLS];
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) acc[m][c] = 0.f;
+  for (int64_t k = lane * W; k < g.K; k += 64 * W) {
+    const int64_t left = g.K - k;
+    u4 v[COLS], s[ROWS];
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+      const T* w = (const T*)g.b + (col + c < g.N ? col + c : g.N - 1) * g.ldb + k;
+      v[c] = left >= W ? load16(w) : load_some(w, left);
+    }
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) {
+      const T* p = x + (m < g.M ? m : g.M - 1) * g.lda + k;
+      s[m] = left >= W ? load16(p) : load_some(p, left);
+    }
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+      float f[W];
+      widen16<T>(v[c], f);
+#pragma unroll
+      for (int m = 0; m < ROWS; ++m) {
+        float e[W];
+        widen16<T>(s[m], e);
+#pragma unroll
+        for (int i = 0; i < W; ++i) acc[m][c] = fmaf(e[i], f[i], acc[m][c]);
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1)
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) acc[m][c] += __shfl_xor(acc[m][c], d);
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+    for (int c = 0; c < COLS; ++c)
+      if (lane == m * COLS + c && m < g.M && col + c < g.N)
+        thin_out<T>(g, m, col + c, g.bias ? acc[m][c] + (float)((const T*)g.bias)[col + c] : acc[m][c]);
+}
+
+inline bool thin_fit(const Gemm& g) { return g.a_along && g.M <= 8; }
+
+// Slices of W's rows: one while W is so small that the launch is what it costs; else as many as give 256 workgroups, which
+// then read 1 KiB of a row at a time (16-byte columns of a long matrix all lie in a few of the memory's channels).
+template <typename T> void thin_cut(Gemm& g) {
+  g.slices = 1;
+  g.slice_k = g.K > 0 ? g.K : 1;
+  if (g.b_along || g.K * g.N * (int64_t)sizeof(T) <= (4 << 20)) return;
+  const int64_t blocks = (g.N + 64 * Unit<T>::W - 1) / (64 * Unit<T>::W);
+  int64_t want = 256 / (blocks < 256 ? blocks : 256);
+  const int64_t most = (g.K + 31) / 32;
+  want = want < 2 ? 2 : want > most ? most : want;
+  g.slice_k = ((g.K + want - 1) / want + 31) / 32 * 32;
+  g.slices = (int)((g.K + g.slice_k - 1) / g.slice_k);
+}
+
+template <typename T, int ROWS>
+int thin_launch(const Gemm& g) {
+  constexpr int W = Unit<T>::W;
+  if (g.b_along) {
+    if (g.N >= 4096) hipLaunchKernelGGL((thin_along_kernel<T, ROWS, 4>), dim3((uint32_t)((g.N + 15) / 16)), dim3(256), 0, g.stream, g);
+    else hipLaunchKernelGGL((thin_along_kernel<T, ROWS, 1>), dim3((uint32_t)((g.N + 3) / 4)), dim3(256), 0, g.stream, g);
+  } else {
+    const int64_t cols = (g.N + 31) / 32 * 32;
+    if (g.slices == 1) {
+      int lanes = 8;
+      while (lanes > 2 && (g.N + lanes * W - 1) / (lanes * W) < 256) lanes /= 2;
+      const int64_t blocks = (cols + lanes * W - 1) / (lanes * W);
+      hipLaunchKernelGGL((thin_across_kernel<T, ROWS, 16, 4, 2, 8>), dim3((uint32_t)((blocks + 7) / 8 * 8)), dim3(1024), 0, g.stream, g, lanes);
+    } else {
+      const int64_t blocks = (cols + 64 * W - 1) / (64 * W);
+      hipLaunchKernelGGL((thin_across_kernel<T, ROWS, 8, 16, 64, 64>), dim3((uint32_t)((blocks + 7) / 8 * 8), (uint32_t)g.slices), dim3(512), 0, g.stream, g, 64);
+      DGNN_LAUNCHED();
+      hipLaunchKernelGGL((gemm_join_kernel<T>), dim3(join_blocks(g)), dim3(256), 0, g.stream, g);
+    }
+  }
+  DGNN_LAUNCHED();
+  return DGNN_OK;
+}
+
 struct Shape { int bm, bn; };
 
 // Tile by the sides of the output: the narrowest that covers it once, else 128 x 256 (the operand with fewer bytes a
@@ -905,8 +1111,7 @@ int gemm_launch(const Gemm& g) {
   }
   DGNN_LAUNCHED();
   if (g.slices > 1) {
-    const int64_t lanes = g.M * ((g.N + 31) / 32 * 8);
-    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((uint32_t)((lanes + 255) / 256)), dim3(256), 0, g.stream, g);
+    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3(join_blocks(g)), dim3(256), 0, g.stream, g);
     DGNN_LAUNCHED();
   }
   return DGNN_OK;
@@ -914,6 +1119,15 @@ int gemm_launch(const Gemm& g) {
 
 template <typename T>
 int gemm_typed(const Gemm& g) {
+  if (thin_fit(g)) {
+    switch (g.M) {
+      case 1: return thin_launch<T, 1>(g);
+      case 2: return thin_launch<T, 2>(g);
+      case 3: case 4: return thin_launch<T, 4>(g);
+      case 5: case 6: return thin_launch<T, 6>(g);
+      default: return thin_launch<T, 8>(g);
+    }
+  }
   if (g.image) {
     switch (rows_bn(g.N)) {
       case 32: return rows_launch<T, 1>(g, g.image);

@@ -168,9 +168,13 @@ bool apart(const void* a, int64_t lda, int64_t ra, int64_t ca, const void* b, in
   return a1 <= b0 || b1 <= a0;
 }
 
-// How a product runs, by its sizes: over W's laid-out image where there are many rows, else by tiles, cut along the
+// How a product runs, by its sizes: a handful of rows on plain multiply-adds, over W's laid-out image where there are many rows, else by tiles, cut along the
 // contraction where those are few. Returns the bytes of workspace that takes.
 int64_t plan(Gemm& g, int32_t dtype) {
+  if (thin_fit(g)) {
+    if (dtype == DGNN_F32) thin_cut<float>(g); else thin_cut<_Float16>(g);
+    return g.slices > 1 ? (int64_t)g.slices * g.M * g.N * 4 : 0;
+  }
   if (rows_fit(g)) {
     g.slices = 1;
     return dtype == DGNN_F32 ? rows_image<float>(g) : rows_image<_Float16>(g);

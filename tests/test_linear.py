@@ -36,7 +36,7 @@ def _backward(x=A, ldx=8, w=B, ldw=8, dy=C, ldd=8, save=D, lds=8, dx=5 << 22, ld
     (_forward, dict(x=None)), (_forward, dict(w=None)), (_forward, dict(y=None)), (_forward, dict(ldx=7)), (_forward, dict(ldw=7)),
     (_forward, dict(ldy=7)), (_forward, dict(x=A + 2)), (_forward, dict(bias=A + 1)), (_forward, dict(res=D, ldr=7)),
     (_forward, dict(y=A + 64)), (_forward, dict(y=B)), (_forward, dict(res=C + 32, ldr=8)), (_forward, dict(act=1, save=D, lds=0)),
-    (_forward, dict(act=2, save=D, lds=7)), (_forward, dict(M=1, K=4096, N=64, ldx=4096, ldw=64, ldy=64)),      # cut, no workspace
+    (_forward, dict(act=2, save=D, lds=7)), (_forward, dict(M=9, K=4096, N=64, ldx=4096, ldw=64, ldy=64, x=1 << 30)),      # cut, no workspace
     (_slope, dict(dtype=-1)), (_slope, dict(act=9)), (_slope, dict(save=None)), (_slope, dict(lds=7)), (_slope, dict(dy=None)),
     (_slope, dict(ldp=7)), (_slope, dict(act=1, lds=0)), (_slope, dict(db=D)), (_slope, dict(db=D, ws=D, n=4)), (_slope, dict(db=D + 2)),
     (_grad_input, dict(dtype=5)), (_grad_input, dict(p=None)), (_grad_input, dict(ldx=7)), (_grad_input, dict(dx=A)), (_grad_input, dict(add=D, lda=7)), (_grad_input, dict(add=C)), (_grad_input, dict(N=-2)),

@@ -21,7 +21,7 @@ pytestmark = pytest.mark.gpu
 DT = {'f32': torch.float32, 'bf16': torch.bfloat16, 'f16': torch.float16}
 HALF = {k: torch.finfo(t).eps / 2 for k, t in DT.items()}
 U = 2.0 ** -24
-SIZES = [(1, 1, 1), (1, 602, 256), (2, 3, 5), (7, 4096, 130), (33, 17, 31), (31, 64, 32), (64, 1433, 16), (129, 40, 41), (257, 602, 256),
+SIZES = [(1, 1, 1), (3, 300, 4099), (8, 4100, 129), (4, 40, 8), (1, 602, 256), (2, 3, 5), (7, 4096, 130), (33, 17, 31), (31, 64, 32), (64, 1433, 16), (129, 40, 41), (257, 602, 256),
          (128, 256, 257), (300, 33, 300), (1000, 7, 64), (4099, 100, 47), (20000, 31, 129)]
 
 
