@@ -891,6 +891,204 @@ int rows_launch(const Gemm& g, char* image) {
 }
 
 // ---------------------------------------------------------------------------------------
+// x^T p of fp32 matrices, the weight gradient over many rows: both operands keep the contraction across rows, and it is long
+// (every node) while the output is small. A wave owns 32 columns of x and all the workgroup's columns of p; x goes from memory
+// straight to the lanes (8 rows' values of a column each), p is turned and split once a workgroup on its way to LDS. The rows
+// are cut into slices for 3 workgroups a compute unit, the tiles of a slice stay on one XCD, and a join adds the slices.
+// (16-bit values would come 2 or 4 bytes a load here; the tiles of gemm_kernel load 16, which is worth more.)
+// ---------------------------------------------------------------------------------------
+template <int BN> struct Turn {                               // BN columns of 32 rows by 256 lanes: 8 rows of 2 columns a lane
+  static constexpr int BK = 32, CH = BK / 8, GROUPS = BN / 2, UNITS = GROUPS * CH, STAGE = 3 * CH * BN * 16;
+  typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+  typedef uint32_t u2_at4 __attribute__((ext_vector_type(2), aligned(4)));
+  u2 r[8];
+
+  static __device__ __forceinline__ int place(int col) { return col ^ ((col >> 4) & 7); }
+
+  // p: the tile's first column of row 0. A lane's distance from its row's start is 32 bits, the rows' starts are the
+  // workgroup's: addresses cost scalar registers
+  __device__ __forceinline__ void fetch(const float* p, int64_t ld, int64_t cols, int64_t k0, int64_t kend, int tid) {
+    if (UNITS < 256 && tid >= UNITS) return;
+    const int col = tid % GROUPS * 2, chunk = tid / GROUPS;
+    const uint32_t off = (uint32_t)((8 * chunk * ld + col) * 4);
+    if (k0 + BK <= kend && cols >= BN) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = *reinterpret_cast<const u2_at4*>(reinterpret_cast<const char*>(p + (k0 + i) * ld) + off);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(p + (k0 + i) * ld) + off);
+        r[i] = u2{0, 0};
+        if (k0 + 8 * chunk + i < kend) {
+          if (col < cols) r[i][0] = q[0];
+          if (col + 1 < cols) r[i][1] = q[1];
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void store(char* lds, int tid) const {
+    if (UNITS < 256 && tid >= UNITS) return;
+    char* const at = lds + (tid / GROUPS) * BN * 16;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      char* const to = at + place(tid % GROUPS * 2 + c) * 16;
+      float v[8];
+      u4 h[3];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i][c]);
+      split8(v, h);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<u4*>(to + p * CH * BN * 16) = h[p];
+    }
+  }
+};
+
+template <int TN>
+__global__ __launch_bounds__(256, 3) void columns_kernel(const Gemm g) {
+  constexpr int BN = TN * 32, BK = 32, S = BK / 16, CH = BK / 8, BM = 128;
+  using B = Turn<BN>;
+  __shared__ __attribute__((aligned(16))) char even[B::STAGE];
+  __shared__ __attribute__((aligned(16))) char odd[B::STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int64_t tiles_m = (g.M + BM - 1) / BM, tiles_n = (g.N + BN - 1) / BN, tiles = tiles_m * tiles_n;
+  int64_t tile = blockIdx.x % tiles, slice = blockIdx.x / tiles;
+  if (g.slices >= 8) {                                         // consecutive workgroups go round the 8 XCDs
+    tile = blockIdx.x / 8 % tiles;
+    slice = blockIdx.x / 8 / tiles * 8 + blockIdx.x % 8;
+    if (slice >= g.slices) return;
+  }
+  const int64_t row0 = tile / tiles_n * BM + wave * 32, col0 = tile % tiles_n * BN;           // of the output
+  const int64_t kbeg = slice * g.slice_k, kend = kbeg + g.slice_k < g.K ? kbeg + g.slice_k : g.K;
+  const float* const x = (const float*)g.a;
+  const float* const p = (const float*)g.b;
+  const int64_t mine = row0 + (lane & 31);                     // a lane's column of x; past the end the last one stands in
+  const uint32_t off = (uint32_t)(((mine < g.M ? mine : g.M - 1) + 8 * half * g.lda) * 4);
+
+  f16v acc[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) acc[j] = f16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  float cur[S][8], next[S][8];                                 // a lane's column of 8 rows of each 16
+  auto fetch_x = [&](int64_t k0, float (&to)[S][8]) __attribute__((always_inline)) {
+    const bool whole = k0 + BK <= kend;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float* q = reinterpret_cast<const float*>(reinterpret_cast<const char*>(x + (k0 + 16 * s + i) * g.lda) + off);
+        if (whole) to[s][i] = *q;
+        else to[s][i] = k0 + 16 * s + 8 * half + i < kend ? *q : 0.f;
+      }
+  };
+  B b;
+  if (kbeg < kend) {
+    b.fetch(p + col0, g.ldb, g.N - col0, kbeg, kend, tid);
+    fetch_x(kbeg, cur);
+    b.store(even, tid);
+  }
+  __syncthreads();
+  auto step = [&](int64_t k, const char* from, char* to) __attribute__((always_inline)) {
+    const bool more = k + BK < kend;
+    if (more) {
+      b.fetch(p + col0, g.ldb, g.N - col0, k + BK, kend, tid);
+      fetch_x(k + BK, next);
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      u4 f[3];
+      split8(cur[s], f);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        u4 y[3];
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+          y[q] = *reinterpret_cast<const u4*>(from + ((q * CH + 2 * s + half) * BN + B::place(j * 32 + (lane & 31))) * 16);
+        acc[j] = mfma(f[2], y[0], acc[j], float());            // small products first
+        acc[j] = mfma(f[0], y[2], acc[j], float());
+        acc[j] = mfma(f[1], y[1], acc[j], float());
+        acc[j] = mfma(f[1], y[0], acc[j], float());
+        acc[j] = mfma(f[0], y[1], acc[j], float());
+        acc[j] = mfma(f[0], y[0], acc[j], float());
+      }
+    }
+    if (more) b.store(to, tid);
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) cur[s][i] = next[s][i];
+  };
+  for (int64_t k = kbeg; k < kend; k += 2 * BK) {
+    step(k, even, odd);
+    if (k + BK < kend) step(k + BK, odd, even);
+  }
+
+  each<0, TN>([&](auto j) __attribute__((always_inline)) {
+    const int64_t col = col0 + j * 32 + (lane & 31);
+    float seen = 0.f;                                          // 0, or NaN where a sum is not finite
+#pragma unroll
+    for (int e = 0; e < 16; ++e) seen = fmaf(acc[j][e], 0.f, seen);
+    if (__ballot(!(seen == 0.f))) {
+#pragma unroll 1
+      for (int e = 0; e < 16; ++e) {
+        const int64_t row = row0 + 8 * (e / 4) + 4 * half + e % 4;
+        float t = acc[j][e];
+        if (row < g.M && col < g.N && !(fabsf(t) < __builtin_huge_valf())) {
+          t = 0.f;
+          for (int64_t k = kbeg; k < kend; ++k) t = fmaf(x[k * g.lda + row], p[k * g.ldb + col], t);
+        }
+        acc[j][e] = t;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int64_t row = row0 + 8 * (e / 4) + 4 * half + e % 4;
+      if (row < g.M && col < g.N) {
+        if (g.slices > 1) g.partial[(slice * g.M + row) * g.N + col] = acc[j][e];
+        else ((float*)g.c)[row * g.ldc + col] = acc[j][e];
+      }
+    }
+  });
+}
+
+// From 16384 rows up, while a lane's distance from its row fits 32 bits.
+template <typename T> bool columns_fit(const Gemm& g) {
+  return sizeof(T) == 4 && !g.a_along && g.K >= 16384 && (8 * g.lda + g.M) * 4 <= 0xffffffffLL && 32 * g.ldb * 4 <= 0xffffffffLL;
+}
+
+inline int64_t columns_tiles(const Gemm& g) { return ((g.M + 127) / 128) * ((g.N + rows_bn(g.N) - 1) / rows_bn(g.N)); }
+
+// Slices for 3 workgroups a compute unit, as many for each XCD, 256 rows at least, and no more partial sums than a quarter
+// of what the operands weigh.
+inline void columns_cut(Gemm& g) {
+  const int64_t tiles = columns_tiles(g), most = (g.K + 255) / 256, heavy = g.K * (g.M + g.N) / (4 * g.M * g.N);
+  int64_t want = 768 / (tiles < 768 ? tiles : 768);
+  if (want > most) want = most;
+  if (want > heavy) want = heavy;
+  if (want >= 8) want = want / 8 * 8;
+  if (want < 1) want = 1;
+  g.slice_k = ((g.K + want - 1) / want + 31) / 32 * 32;
+  g.slices = (int)((g.K + g.slice_k - 1) / g.slice_k);
+}
+
+inline int columns_launch(const Gemm& g) {
+  const int64_t blocks = (g.slices >= 8 ? ((int64_t)g.slices + 7) / 8 * 8 : g.slices) * columns_tiles(g);
+  if (blocks > 0x7fffffffLL) return dgnn_fail(DGNN_E_BADARG, "linear_grad_weight: too many tiles%s");
+  const dim3 grid((uint32_t)blocks);
+  switch (rows_bn(g.N)) {
+    case 32: hipLaunchKernelGGL((columns_kernel<1>), grid, dim3(256), 0, g.stream, g); break;
+    case 64: hipLaunchKernelGGL((columns_kernel<2>), grid, dim3(256), 0, g.stream, g); break;
+    default: hipLaunchKernelGGL((columns_kernel<4>), grid, dim3(256), 0, g.stream, g);
+  }
+  DGNN_LAUNCHED();
+  if (g.slices > 1) {
+    hipLaunchKernelGGL((gemm_join_kernel<float>), dim3(join_blocks(g)), dim3(256), 0, g.stream, g);
+    DGNN_LAUNCHED();
+  }
+  return DGNN_OK;
+}
+
+// ---------------------------------------------------------------------------------------
 // A handful of rows (1..8): W's bytes are all there is, each is used once a row, so plain fused multiply-adds in fp32 keep up
 // and no sum is split over workgroups -- one launch. thin_across: W[k][n] with n contiguous; LANES lanes take 16 bytes each
 // of a row of W, the others and the 16 waves further rows, all loads of a lane are on their way together, and the rows'
@@ -1094,6 +1292,9 @@ inline Shape shape_of(int64_t M, int64_t N) {
   return {128, 256};
 }
 
+// Workgroups a compute unit holds at once, by their LDS.
+inline int resident_of(Shape s) { return s.bn == 256 ? 1 : s.bn == 128 && s.bm == 128 ? 2 : 3; }
+
 inline int64_t tiles_of(Shape s, int64_t M, int64_t N) { return ((M + s.bm - 1) / s.bm) * ((N + s.bn - 1) / s.bn); }
 
 template <typename T, bool AA, bool BA>
@@ -1135,9 +1336,11 @@ int gemm_typed(const Gemm& g) {
       default: return rows_launch<T, 4>(g, g.image);
     }
   }
-  if (g.a_along && !g.b_along) return gemm_launch<T, true, false>(g);
-  if (g.a_along && g.b_along) return gemm_launch<T, true, true>(g);
-  return gemm_launch<T, false, false>(g);
+  if constexpr (sizeof(T) == 4) {
+    if (columns_fit<T>(g)) return columns_launch(g);
+  }
+  if (!g.a_along) return gemm_launch<T, false, false>(g);
+  return g.b_along ? gemm_launch<T, true, true>(g) : gemm_launch<T, true, false>(g);
 }
 
 __attribute__((visibility("hidden"))) int gemm_f32(const Gemm& g);

@@ -122,11 +122,13 @@ constexpr int64_t kCompute = 256;              // compute units
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// A product with fewer output tiles than compute units is cut along its contraction, at 128 elements a slice or more.
+// A product whose output tiles do not fill the compute units is cut along its contraction, at 128 elements a slice or more:
+// for one workgroup a unit in any case, for as many as fit while the partial sums weigh less than half the operands.
 void cut(Gemm& g) {
-  const int64_t tiles = tiles_of(shape_of(g.M, g.N), g.M, g.N);
-  int64_t want = kCompute / (tiles > 0 ? tiles : 1);
-  const int64_t most = ceil_div(g.K, 128);
+  const Shape shape = shape_of(g.M, g.N);
+  const int64_t tiles = tiles_of(shape, g.M, g.N), one = kCompute / (tiles > 0 ? tiles : 1);
+  const int64_t most = ceil_div(g.K, 128), light = g.M > 0 && g.N > 0 ? g.K * (g.M + g.N) / (4 * g.M * g.N) : 1;
+  int64_t want = one > light ? one : light < one * resident_of(shape) ? light : one * resident_of(shape);
   if (want > most) want = most;
   if (want < 1) want = 1;
   g.slice_k = ceil_div(ceil_div(g.K, want), 64) * 64;
@@ -173,6 +175,10 @@ bool apart(const void* a, int64_t lda, int64_t ra, int64_t ca, const void* b, in
 int64_t plan(Gemm& g, int32_t dtype) {
   if (thin_fit(g)) {
     if (dtype == DGNN_F32) thin_cut<float>(g); else thin_cut<_Float16>(g);
+    return g.slices > 1 ? (int64_t)g.slices * g.M * g.N * 4 : 0;
+  }
+  if (dtype == DGNN_F32 && columns_fit<float>(g)) {
+    columns_cut(g);
     return g.slices > 1 ? (int64_t)g.slices * g.M * g.N * 4 : 0;
   }
   if (rows_fit(g)) {

@@ -56,7 +56,8 @@ def test_c_entries_with_nothing_to_do():
 
 def test_workspace_is_bounded():
     """Only products with fewer tiles than compute units are cut, so the partial sums stay under 256 tiles of 128 x 256 floats;
-    where W is laid out, its image has at most 6 bytes an element, both sides rounded up (to 256 and 64)."""
+    where W is laid out, its image has at most 6 bytes an element, both sides rounded up (to 256 and 64); the weight gradient's
+    partial sums weigh at most a quarter of its operands, and one output at least."""
     n = ctypes.c_int64()
     for kind in range(4):
         for M in (0, 1, 7, 33, 2708, 232965, 2449029):
@@ -64,7 +65,7 @@ def test_workspace_is_bounded():
                 for N in (0, 1, 16, 41, 256, 4096):
                     for dtype in range(3):
                         assert lib.dgnn_linear_workspace(kind, M, K, N, dtype, ctypes.byref(n)) == 0
-                        assert 0 <= n.value <= (max(256 * 128 * 256 * 4, 6 * (K + 256) * (N + 256)) if kind != 1 else 4096 * max(N, 1) * 4)
+                        assert 0 <= n.value <= (max(256 * 128 * 256 * 4, 6 * (K + 256) * (N + 256), M * (K + N), 4 * K * N) if kind != 1 else 4096 * max(N, 1) * 4)
     assert lib.dgnn_linear_workspace(4, 1, 1, 1, 0, ctypes.byref(n)) == 1
     assert lib.dgnn_linear_workspace(0, -1, 1, 1, 0, ctypes.byref(n)) == 1
     assert lib.dgnn_linear_workspace(0, 1, 1, 1, 0, None) == 1
