@@ -93,6 +93,17 @@ template <typename T> __device__ __forceinline__ u4 load_some(const T* p, int64_
   return r.v;
 }
 
+// W elements of which only the first `n` exist where reading all of them is safe (what lies behind a row's end is the next row)
+template <typename T> __device__ __forceinline__ u4 load_masked(const T* p, int64_t n) {
+  u4 v = load16(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) v[i] = i < n ? v[i] : 0u;
+    else v[i] = 2 * i + 1 < n ? v[i] : 2 * i < n ? v[i] & 0xffffu : 0u;
+  }
+  return v;
+}
+
 __device__ __forceinline__ uint32_t pack_bf(float x, float y) {
   union { bf2 h; uint32_t u; } r;
   r.h = __builtin_convertvector(f2{x, y}, bf2);
@@ -128,32 +139,45 @@ template <typename T, bool ALONG, int ROWS, int THREADS> struct Tile {
   // whose lanes are W rows apart, over the banks
   static __device__ __forceinline__ int place(int row) { return row ^ ((row >> 4) & 7); }
 
-  __device__ __forceinline__ void fetch(const T* base, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int64_t kend, int tid) {
+  // `kall`: the whole contraction, kend the slice's. Loads may run over a row's end wherever another row follows: rows (or
+  // columns) past the operand's give sums that nobody keeps, contraction elements past kend are made zero.
+  __device__ __forceinline__ void fetch(const T* base, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int64_t kend, int64_t kall, int tid) {
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       const int id = tid + u * THREADS;
       if (UNITS % THREADS != 0 && id >= UNITS) break;
       if constexpr (ALONG) {
-        const int64_t row = row0 + id / CH;
-        const T* p = base + (row < rows ? row : rows - 1) * ld + k0 + 8 * (id % CH);
+        int64_t row = row0 + id / CH;
+        row = row < rows ? row : rows - 1;
+        const T* p = base + row * ld + k0 + 8 * (id % CH);
         const int64_t left = kend - k0 - 8 * (id % CH);
         if (left >= 8) {
 #pragma unroll
           for (int q = 0; q < QUADS; ++q) r[u][q] = load16(p + q * W);
+        } else if (left > 0 && row + 1 < rows && ld >= 8) {
+#pragma unroll
+          for (int q = 0; q < QUADS; ++q) r[u][q] = load_masked(p + q * W, left - q * W);
         } else {
 #pragma unroll
           for (int q = 0; q < QUADS; ++q) r[u][q] = load_some(p + q * W, left - q * W);
         }
       } else {
-        const int64_t col = row0 + (id % (ROWS / W)) * W;
         const int64_t k = k0 + 8 * (id / (ROWS / W));
-        const T* p = base + k * ld + col;
-        const int64_t left = rows - col;
+        int64_t col = row0 + (id % (ROWS / W)) * W;
+        if (k0 + BK <= kend && k0 + BK < kall && ld >= W) {
+          col = col < rows ? col : row0;
+          const T* p = base + k * ld + col;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          if (k + q >= kend) r[u][q] = u4{0, 0, 0, 0};
-          else if (left >= W) r[u][q] = load16(p + q * ld);
-          else r[u][q] = load_some(p + q * ld, left);
+          for (int q = 0; q < 8; ++q) r[u][q] = load16(p + q * ld);
+        } else {
+          const T* p = base + k * ld + col;
+          const int64_t left = rows - col;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            if (k + q >= kend) r[u][q] = u4{0, 0, 0, 0};
+            else if (left >= W) r[u][q] = load16(p + q * ld);
+            else r[u][q] = load_some(p + q * ld, left);
+          }
         }
       }
     }
@@ -358,8 +382,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm g) {
   TA ta;
   TB tb;
   if (k0 < kend) {
-    ta.fetch(a, g.lda, row0, g.M, k0, kend, tid);
-    tb.fetch(b, g.ldb, col0, g.N, k0, kend, tid);
+    ta.fetch(a, g.lda, row0, g.M, k0, kend, g.K, tid);
+    tb.fetch(b, g.ldb, col0, g.N, k0, kend, g.K, tid);
     ta.store(lds[0], tid);
     tb.store(lds[0] + TA::BYTES, tid);
   }
@@ -368,8 +392,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm g) {
   for (int64_t k = k0; k < kend; k += BK) {
     const bool more = k + BK < kend;
     if (more) {
-      ta.fetch(a, g.lda, row0, g.M, k + BK, kend, tid);
-      tb.fetch(b, g.ldb, col0, g.N, k + BK, kend, tid);
+      ta.fetch(a, g.lda, row0, g.M, k + BK, kend, g.K, tid);
+      tb.fetch(b, g.ldb, col0, g.N, k + BK, kend, g.K, tid);
     }
     const char* la = lds[buf];
     const char* lb = lds[buf] + TA::BYTES;
@@ -508,13 +532,16 @@ __global__ __launch_bounds__(256) void lay_out_kernel(const Layout g) {
   }
 }
 
-// 8 consecutive elements of a row, `left` of which exist
+// 8 consecutive elements of a row, `left` of which exist; `over`: a load may run over the row's end
 template <typename T> struct Eight { u4 q[8 / Unit<T>::W]; };
-template <typename T> __device__ __forceinline__ void load8(const T* p, int64_t left, Eight<T>& v) {
+template <typename T> __device__ __forceinline__ void load8(const T* p, int64_t left, bool over, Eight<T>& v) {
   constexpr int W = Unit<T>::W;
   if (left >= 8) {
 #pragma unroll
     for (int i = 0; i < 8 / W; ++i) v.q[i] = load16(p + i * W);
+  } else if (left > 0 && over) {
+#pragma unroll
+    for (int i = 0; i < 8 / W; ++i) v.q[i] = load_masked(p + i * W, left - i * W);
   } else {
 #pragma unroll
     for (int i = 0; i < 8 / W; ++i) v.q[i] = load_some(p + i * W, left - i * W);
@@ -664,7 +691,7 @@ template <typename T, int TN> struct Wave {
   }
 
   // stage kt of the row whose lane part begins at p; `to` may be another wave state's
-  static __device__ __forceinline__ void fetch(const T* p, int64_t K, int kt, int half, Eight<T> (&to)[S]) {
+  static __device__ __forceinline__ void fetch(const T* p, int64_t K, int kt, int half, bool over, Eight<T> (&to)[S]) {
     const T* q = p + (int64_t)kt * BK;
     const int64_t left = K - (int64_t)kt * BK;
     if (left >= BK) {
@@ -674,7 +701,7 @@ template <typename T, int TN> struct Wave {
         for (int i = 0; i < 8 / Unit<T>::W; ++i) to[s].q[i] = load16(q + 16 * s + i * Unit<T>::W);
     } else {
 #pragma unroll
-      for (int s = 0; s < S; ++s) load8(q + 16 * s, left - 8 * half - 16 * s, to[s]);
+      for (int s = 0; s < S; ++s) load8(q + 16 * s, left - 8 * half - 16 * s, over, to[s]);
     }
   }
 
@@ -781,6 +808,7 @@ __global__ __launch_bounds__(WAVES * 64, 3) void rows_kernel(const Gemm g, const
   if (group * WAVES * 32 >= g.M) return;
   const char* w = image + nt * ktiles * STAGE + lane * 16;
   const T* p = (const T*)g.a + (row < g.M ? row : g.M - 1) * g.lda + 8 * half;
+  const bool over = row + 1 < g.M && g.lda >= 8;
   auto send = [&](int kt, char* to) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -795,13 +823,13 @@ __global__ __launch_bounds__(WAVES * 64, 3) void rows_kernel(const Gemm g, const
   V v;
   Eight<T> next[V::S];
   send(0, even);
-  V::fetch(p, g.K, 0, half, v.a);
+  V::fetch(p, g.K, 0, half, over, v.a);
   v.begin(g, nt * V::BN, half);
   meet();
   auto step = [&](int kt, const char* from, char* to) __attribute__((always_inline)) {
     if (kt + 1 < ktiles) {
       send(kt + 1, to);
-      V::fetch(p, g.K, kt + 1, half, next);
+      V::fetch(p, g.K, kt + 1, half, over, next);
     }
     v.multiply(from + ((lane >> 5) * V::BN + (lane & 31)) * 16);
     meet();
@@ -827,23 +855,25 @@ __global__ __launch_bounds__(WAVES * 64, 2) void rows_resident_kernel(const Gemm
   const int64_t blocks = (g.M + 31) / 32, stride = (int64_t)gridDim.x * WAVES;
   int64_t block = (int64_t)blockIdx.x * WAVES + wave;
   if (block >= blocks) return;
+  bool over = false;
   auto part = [&](int64_t at) __attribute__((always_inline)) {
     const int64_t row = at * 32 + (lane & 31);
+    over = row + 1 < g.M && g.lda >= 8;
     return (const T*)g.a + (row < g.M ? row : g.M - 1) * g.lda + 8 * half;
   };
   V v;
   Eight<T> next[V::S];
   const T* p = part(block);
-  V::fetch(p, g.K, 0, half, v.a);
+  V::fetch(p, g.K, 0, half, over, v.a);
   for (; block < blocks; block += stride) {
     asm volatile("" ::: "memory");                            // the bias is loaded for each block, not held in 16 TN registers
     v.begin(g, 0, half);
     for (int kt = 0; kt < ktiles; ++kt) {
       if (kt + 1 < ktiles) {
-        V::fetch(p, g.K, kt + 1, half, next);
+        V::fetch(p, g.K, kt + 1, half, over, next);
       } else if (block + stride < blocks) {
         p = part(block + stride);
-        V::fetch(p, g.K, 0, half, next);
+        V::fetch(p, g.K, 0, half, over, next);
       }
       v.multiply(lds + kt * V::STAGE + ((lane >> 5) * V::BN + (lane & 31)) * 16);
 #pragma unroll
@@ -905,13 +935,23 @@ template <int BN> struct Turn {                               // BN columns of 3
 
   static __device__ __forceinline__ int place(int col) { return col ^ ((col >> 4) & 7); }
 
-  // p: the tile's first column of row 0. A lane's distance from its row's start is 32 bits, the rows' starts are the
-  // workgroup's: addresses cost scalar registers
-  __device__ __forceinline__ void fetch(const float* p, int64_t ld, int64_t cols, int64_t k0, int64_t kend, int tid) {
+  uint32_t off;
+  int col;
+  bool pair;
+
+  // p: the tile's first column of row 0, `cols` columns from there on. A lane's distance from its row's start is 32 bits, the
+  // rows' starts are the workgroup's: addresses cost scalar registers. A lane past the columns reads the first ones (its sums
+  // are not kept); a pair that ends past them reads on into the next row, or is two loads where none follows
+  __device__ __forceinline__ void begin(int64_t ld, int64_t cols, int tid) {
+    col = tid % GROUPS * 2;
+    col = col < cols ? col : 0;
+    pair = col + 1 < cols;
+    off = (uint32_t)((8 * (tid / GROUPS) * ld + col) * 4);
+  }
+
+  __device__ __forceinline__ void fetch(const float* p, int64_t ld, int64_t k0, int64_t kend, int64_t kall, int tid) {
     if (UNITS < 256 && tid >= UNITS) return;
-    const int col = tid % GROUPS * 2, chunk = tid / GROUPS;
-    const uint32_t off = (uint32_t)((8 * chunk * ld + col) * 4);
-    if (k0 + BK <= kend && cols >= BN) {
+    if (k0 + BK <= kend && k0 + BK < kall && ld >= 2) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) r[i] = *reinterpret_cast<const u2_at4*>(reinterpret_cast<const char*>(p + (k0 + i) * ld) + off);
     } else {
@@ -919,9 +959,9 @@ template <int BN> struct Turn {                               // BN columns of 3
       for (int i = 0; i < 8; ++i) {
         const uint32_t* q = reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(p + (k0 + i) * ld) + off);
         r[i] = u2{0, 0};
-        if (k0 + 8 * chunk + i < kend) {
-          if (col < cols) r[i][0] = q[0];
-          if (col + 1 < cols) r[i][1] = q[1];
+        if (k0 + 8 * (tid / GROUPS) + i < kend) {
+          r[i][0] = q[0];
+          if (pair) r[i][1] = q[1];
         }
       }
     }
@@ -981,8 +1021,9 @@ __global__ __launch_bounds__(256, 3) void columns_kernel(const Gemm g) {
       }
   };
   B b;
+  b.begin(g.ldb, g.N - col0, tid);
   if (kbeg < kend) {
-    b.fetch(p + col0, g.ldb, g.N - col0, kbeg, kend, tid);
+    b.fetch(p + col0, g.ldb, kbeg, kend, g.K, tid);
     fetch_x(kbeg, cur);
     b.store(even, tid);
   }
@@ -990,7 +1031,7 @@ __global__ __launch_bounds__(256, 3) void columns_kernel(const Gemm g) {
   auto step = [&](int64_t k, const char* from, char* to) __attribute__((always_inline)) {
     const bool more = k + BK < kend;
     if (more) {
-      b.fetch(p + col0, g.ldb, g.N - col0, k + BK, kend, tid);
+      b.fetch(p + col0, g.ldb, k + BK, kend, g.K, tid);
       fetch_x(k + BK, next);
     }
 #pragma unroll
@@ -1284,11 +1325,12 @@ struct Shape { int bm, bn; };
 
 // Tile by the sides of the output: the narrowest that covers it once, else 128 x 256 (the operand with fewer bytes a
 // multiply-add to move; 8 waves of 64 x 64).
-inline Shape shape_of(int64_t M, int64_t N) {
+inline Shape shape_of(const Gemm& g) {
+  const int64_t M = g.M, N = g.N;
   if (M <= 32) return {32, 128};
   if (N <= 32) return {128, 32};
   if (N <= 64) return {128, 64};
-  if (N <= 128) return {128, 128};
+  if (N <= 128 || (!g.a_along && g.K >= 16384)) return {128, 128};
   return {128, 256};
 }
 
@@ -1299,7 +1341,7 @@ inline int64_t tiles_of(Shape s, int64_t M, int64_t N) { return ((M + s.bm - 1) 
 
 template <typename T, bool AA, bool BA>
 int gemm_launch(const Gemm& g) {
-  const Shape s = shape_of(g.M, g.N);
+  const Shape s = shape_of(g);
   const int64_t tiles = tiles_of(s, g.M, g.N);
   if (tiles > 0x7fffffffLL) return dgnn_fail(DGNN_E_BADARG, "linear: too many tiles%s (%lld)", "", tiles);
   const dim3 grid((uint32_t)tiles, (uint32_t)g.slices);

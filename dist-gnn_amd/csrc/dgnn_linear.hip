@@ -125,7 +125,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // A product whose output tiles do not fill the compute units is cut along its contraction, at 128 elements a slice or more:
 // for one workgroup a unit in any case, for as many as fit while the partial sums weigh less than half the operands.
 void cut(Gemm& g) {
-  const Shape shape = shape_of(g.M, g.N);
+  const Shape shape = shape_of(g);
   const int64_t tiles = tiles_of(shape, g.M, g.N), one = kCompute / (tiles > 0 ? tiles : 1);
   const int64_t most = ceil_div(g.K, 128), light = g.M > 0 && g.N > 0 ? g.K * (g.M + g.N) / (4 * g.M * g.N) : 1;
   int64_t want = one > light ? one : light < one * resident_of(shape) ? light : one * resident_of(shape);
