@@ -29,7 +29,8 @@ struct Gemm {
   int64_t lda, ldb;
   bool a_along, b_along;
   int64_t M, N, K;
-  // epilogue: c = act(acc + bias) + residual; save receives acc + bias (or, for relu, a bit per value that is > 0)
+  // epilogue: c = act(acc + bias) + residual; save receives acc + bias in fp32 (or, for relu, a bit per value that is > 0): in 16
+  // bits its rounding would be the largest error of the gradients' column sums
   const void* bias;
   const void* residual;
   int64_t ld_residual;
@@ -284,7 +285,7 @@ __device__ __forceinline__ void finish(const Gemm& g, int64_t row, int64_t col, 
     bits |= __shfl_xor(bits, 4);
     if (lane == 0 && have > 0) ((uint32_t*)g.save)[row * g.ld_save + col / 32] = bits;
   } else if (g.save) {
-    store4((T*)g.save + row * g.ld_save + col, have, v);
+    store4((float*)g.save + row * g.ld_save + col, have, v);
   }
   switch (g.act) {
     case ACT_NONE: break;
@@ -439,17 +440,17 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm g) {
 }
 
 // Joins the slices of a product that was cut along its contraction and finishes it: 32 fours of columns a workgroup, 8 lanes
-// to a four, each adding every 8th slice with up to 8 loads in flight; the 8 sums meet in their order. A row takes a multiple of
+// to a four, each adding every 8th slice with up to 8 loads in flight, in 64 bits; the 8 sums meet in their order. A row takes a multiple of
 // 8 fours, so that relu's bits are whole words.
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_join_kernel(const Gemm g) {
-  __shared__ __attribute__((aligned(16))) float sums[8][32][4];
+  __shared__ double sums[8][32][4];
   const int four = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int64_t wide = (g.N + 31) / 32 * 8;
   const int64_t at = (int64_t)blockIdx.x * 32 + four;
   const int64_t row = at / wide, col = at % wide * 4;
   const int have = row < g.M && col < g.N ? (g.N - col >= 4 ? 4 : (int)(g.N - col)) : 0;
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
   if (have) {
     const float* p = g.partial + row * g.N + col;
     const int64_t step = g.M * g.N;
@@ -462,12 +463,12 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const Gemm g) {
       for (int u = 0; u < 8; ++u)
         if (s + 8 * u < g.slices) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] += t[u][i];
+          for (int i = 0; i < 4; ++i) sum[i] += t[u][i];
         }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sums[part][four][i] = v[i];
+  for (int i = 0; i < 4; ++i) sums[part][four][i] = sum[i];
   __syncthreads();
   if (part) return;
   float bias[4] = {0.f, 0.f, 0.f, 0.f}, res[4] = {0.f, 0.f, 0.f, 0.f};
@@ -476,7 +477,10 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const Gemm g) {
 #pragma unroll
   for (int k = 1; k < 8; ++k)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] += sums[k][four][i];
+    for (int i = 0; i < 4; ++i) sum[i] += sums[k][four][i];
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (float)sum[i];
   finish<T>(g, row, col, have, v, bias, res);
 }
 
@@ -650,9 +654,13 @@ __device__ __forceinline__ void rows_out(const Gemm& g, const f16v (&acc)[TN], c
         bits |= __shfl_xor(bits, 32);
         if (half == 0 && left > 0) ((uint32_t*)g.save)[row * g.ld_save + (col0 / 32 + j)] = bits;
       } else {
-        Out<T>::pack(v, out);
+        u4 wide[4];
+        Out<float>::pack(v, wide);
 #pragma unroll
-        for (int q = 0; q < PIECES; ++q) store_piece((T*)g.save + row * g.ld_save + base + Out<T>::column(q, half), have(q), out[q]);
+        for (int q = 0; q < 4; ++q) {
+          const int64_t n = left - Out<float>::column(q, half);
+          store_piece((float*)g.save + row * g.ld_save + base + Out<float>::column(q, half), n >= 4 ? 4 : n > 0 ? (int)n : 0, wide[q]);
+        }
       }
     }
 #pragma unroll
@@ -1138,7 +1146,7 @@ inline int columns_launch(const Gemm& g) {
 // wave takes COLS outputs and all lanes their contraction.
 // ---------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ void thin_out(const Gemm& g, int64_t row, int64_t col, float t) {
-  if (g.save && g.act > ACT_RELU) ((T*)g.save)[row * g.ld_save + col] = (T)t;
+  if (g.save && g.act > ACT_RELU) ((float*)g.save)[row * g.ld_save + col] = t;
   t = act_of(g.act, t);
   if (g.residual) t += (float)((const T*)g.residual)[row * g.ld_residual + col];
   ((T*)g.c)[row * g.ldc + col] = (T)t;

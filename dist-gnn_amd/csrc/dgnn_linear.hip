@@ -11,7 +11,7 @@ using namespace dgnn;
 // ---------------------------------------------------------------------------------------
 // p = dy act'(x W + b) and the sums of p's columns. Reads dy and what the forward pass saved once and writes p once. A row
 // is taken by the fewest lanes (a power of two) that cover it with 4 columns each, 64 at most, so narrow rows fill a
-// wave too; a lane keeps its columns' sums over the block's rows, in fp32, the block adds its lanes in a fixed order and a
+// wave too; a lane keeps its columns' sums over the block's rows, in 64 bits (sums over every node cancel), the block adds its lanes in a fixed order and a
 // second launch adds the blocks': no atomics, the same bits every run.
 // ---------------------------------------------------------------------------------------
 struct Slope {
@@ -19,7 +19,7 @@ struct Slope {
   const void* save;
   void* p;
   int64_t ld_dy, ld_save, ld_p, M, N, slab;      // rows a block takes
-  float* partial;                                // gridDim.y x N, or null
+  double* partial;                               // gridDim.y x N, or null
   int act, lanes;
 };
 
@@ -32,13 +32,13 @@ __device__ __forceinline__ float slope_of(int act, float t) {
 template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(const Slope g) {
   typedef T quad __attribute__((ext_vector_type(4), aligned(sizeof(T) == 4 ? 4 : 2)));
-  __shared__ float sums[256][4];
+  __shared__ double sums[256][4];
   const int lane = threadIdx.x % g.lanes, group = threadIdx.x / g.lanes, groups = 256 / g.lanes;
   const int64_t col = ((int64_t)blockIdx.x * g.lanes + lane) * 4;
   const int64_t first = (int64_t)blockIdx.y * g.slab;
   const int64_t last = first + g.slab < g.M ? first + g.slab : g.M;
   const int have = g.N - col >= 4 ? 4 : (g.N > col ? (int)(g.N - col) : 0);
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
   if (have > 0) {
     for (int64_t row = first + group; row < last; row += groups) {
       const T* dy = (const T*)g.dy + row * g.ld_dy + col;
@@ -57,10 +57,10 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope g) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = (word >> i) & 1 ? v[i] : 0.f;
       } else if (g.act != ACT_NONE) {
-        const T* pre = (const T*)g.save + row * g.ld_save + col;
+        const float* pre = (const float*)g.save + row * g.ld_save + col;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (i < have) v[i] *= slope_of(g.act, (float)pre[i]);
+          if (i < have) v[i] *= slope_of(g.act, pre[i]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[i] += v[i];
@@ -95,16 +95,16 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope g) {
 
 // sums of the slabs' columns: 16 columns a block, 16 lanes each take every 16th slab, added in their order
 template <typename T>
-__global__ __launch_bounds__(256) void slab_join_kernel(const float* __restrict__ partial, int64_t slabs, int64_t N, T* __restrict__ out) {
-  __shared__ float sums[16][17];
+__global__ __launch_bounds__(256) void slab_join_kernel(const double* __restrict__ partial, int64_t slabs, int64_t N, T* __restrict__ out) {
+  __shared__ double sums[16][17];
   const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
   const int64_t col = (int64_t)blockIdx.x * 16 + c;
-  float t = 0.f;
+  double t = 0.0;
   if (col < N) {
     for (int64_t s = k; s < slabs; s += 128) {               // 8 loads in flight, added in their order
-      float v[8];
+      double v[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = s + 16 * u < slabs ? partial[(s + 16 * u) * N + col] : 0.f;
+      for (int u = 0; u < 8; ++u) v[u] = s + 16 * u < slabs ? partial[(s + 16 * u) * N + col] : 0.0;
 #pragma unroll
       for (int u = 0; u < 8; ++u) t += v[u];
     }
@@ -113,9 +113,68 @@ __global__ __launch_bounds__(256) void slab_join_kernel(const float* __restrict_
   __syncthreads();
   if (k == 0 && col < N) {
     for (int i = 1; i < 16; ++i) t += sums[i][c];
-    out[col] = (T)t;
+    out[col] = (T)(float)t;
   }
 }
+
+// ---------------------------------------------------------------------------------------
+// The whole backward pass of a small layer (M N <= 4096) in one launch, where the launches are what it costs: a workgroup
+// computes p = dy act'(x W + b) into LDS, in fp32 and for itself, and gives the gradients of `chunk` columns of x: their rows
+// of dw = x^T p, their columns of dx = p W^T; the first workgroup adds p's columns up. Plain fused multiply-adds in fp32: few
+// products average over few roundings, so p is not rounded to 16 bits here as it is on the way to the matrix cores.
+// ---------------------------------------------------------------------------------------
+constexpr int kSmall = 4096;
+
+struct Small {
+  const void *x, *w, *dy, *save;
+  void *dx, *dw, *db;
+  int64_t ldx, ldw, ldd, lds, lddx, lddw;
+  int M, K, N, act, chunk;
+};
+
+// out(o, sum over l < L of f(o, l)) for o < count by 256 lanes: 1 to 64 lanes (a power of two) share a sum
+template <typename S, typename F, typename G>
+__device__ __forceinline__ void small_sums(int count, int L, F f, G out) {
+  int share = 1;
+  while (share < 64 && count * share * 2 <= 256) share *= 2;
+  const int part = threadIdx.x % share;
+  for (int base = 0; base < count; base += 256 / share) {
+    const int o = base + threadIdx.x / share;
+    S t = 0;
+    if (o < count)
+      for (int l = part; l < L; l += share) t = f(o, l, t);
+    for (int d = 1; d < share; d <<= 1) t += __shfl_xor(t, d);
+    if (o < count && part == 0) out(o, t);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void small_backward_kernel(const Small g) {
+  __shared__ float p[kSmall], xs[kSmall], ws[kSmall + 16];
+  const int M = g.M, N = g.N, k0 = blockIdx.x * g.chunk, KC = g.K - k0 < g.chunk ? g.K - k0 : g.chunk, pitch = N + 1 - (N & 1);
+  for (int i = threadIdx.x; i < M * N; i += 256) {
+    const int m = i / N, n = i % N;
+    float v = (float)((const T*)g.dy)[m * g.ldd + n];
+    if (g.act == ACT_RELU) v = ((const uint32_t*)g.save)[m * g.lds + n / 32] >> (n & 31) & 1 ? v : 0.f;
+    else if (g.act != ACT_NONE) v *= slope_of(g.act, ((const float*)g.save)[m * g.lds + n]);
+    p[i] = v;
+  }
+  if (g.dw)
+    for (int i = threadIdx.x; i < M * KC; i += 256) xs[i] = (float)((const T*)g.x)[i / KC * g.ldx + k0 + i % KC];
+  if (g.dx)
+    for (int i = threadIdx.x; i < KC * N; i += 256) ws[i / N * pitch + i % N] = (float)((const T*)g.w)[(k0 + i / N) * g.ldw + i % N];
+  __syncthreads();
+  if (g.dw)
+    small_sums<float>(KC * N, M, [&](int o, int m, float t) { return fmaf(xs[m * KC + o / N], p[m * N + o % N], t); },
+               [&](int o, float t) { ((T*)g.dw)[(int64_t)(k0 + o / N) * g.lddw + o % N] = (T)t; });
+  if (g.dx)
+    small_sums<float>(M * KC, N, [&](int o, int n, float t) { return fmaf(p[o / KC * N + n], ws[o % KC * pitch + n], t); },
+               [&](int o, float t) { ((T*)g.dx)[(int64_t)(o / KC) * g.lddx + k0 + o % KC] = (T)t; });
+  if (g.db && blockIdx.x == 0)
+    small_sums<double>(N, M, [&](int n, int m, double t) { return t + p[m * N + n]; }, [&](int n, double t) { ((T*)g.db)[n] = (T)(float)t; });
+}
+
+bool small_fit(int64_t M, int64_t K, int64_t N) { return M > 0 && N > 0 && K > 0 && M <= kSmall && N <= kSmall && M * N <= kSmall; }
 
 // ---------------------------------------------------------------------------------------
 constexpr int64_t kCompute = 256;              // compute units
@@ -214,7 +273,7 @@ int dgnn_linear_workspace(int32_t pass, int64_t M, int64_t K, int64_t N, int32_t
     case DGNN_LINEAR_GRAD_INPUT: g.M = M; g.N = K; g.K = N; g.a_along = true; break;
     case DGNN_LINEAR_GRAD_WEIGHT: g.M = K; g.N = N; g.K = M; break;
     case DGNN_LINEAR_SLOPE:
-      if (M > 0 && N > 0) *bytes = ceil_div(M, slope_slab(M, N)) * N * 4;
+      if (M > 0 && N > 0) *bytes = ceil_div(M, slope_slab(M, N)) * N * 8;
       return DGNN_OK;
     default: return dgnn_fail(DGNN_E_BADARG, "linear_workspace: unknown pass%s (%lld)", "", pass);
   }
@@ -236,7 +295,7 @@ int dgnn_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, 
       || (residual && !matrix_ok(residual, ldr, M, N, b)))
     return dgnn_fail(DGNN_E_BADARG, "linear_forward: null, misaligned or overlapping rows%s");
   if (save && act != ACT_NONE) {
-    const bool fits = act == ACT_RELU ? lds >= (N + 31) / 32 && (uintptr_t)save % 4 == 0 : lds >= N && (uintptr_t)save % b == 0;
+    const bool fits = act == ACT_RELU ? lds >= (N + 31) / 32 && (uintptr_t)save % 4 == 0 : lds >= N && (uintptr_t)save % 4 == 0;
     if (!fits) return dgnn_fail(DGNN_E_BADARG, "linear_forward: save is too narrow or misaligned%s");
   }
   if (!apart(y, ldy, M, N, x, ldx, M, K, b) || !apart(y, ldy, M, N, w, ldw, K, N, b) || !apart(y, ldy, M, N, residual, ldr, M, N, b))
@@ -264,14 +323,14 @@ int dgnn_linear_slope(const void* dy, int64_t ldd, const void* save, int64_t lds
   if ((uintptr_t)dbias % b) return dgnn_fail(DGNN_E_BADARG, "linear_slope: misaligned dbias%s");
   if (M > 0) {
     if (!matrix_ok(dy, ldd, M, N, b) || (p && !matrix_ok(p, ldp, M, N, b)) || (act == ACT_RELU && (!save || lds < (N + 31) / 32 || (uintptr_t)save % 4))
-        || (act > ACT_RELU && !matrix_ok(save, lds, M, N, b)))
+        || (act > ACT_RELU && !matrix_ok(save, lds, M, N, 4)))
       return dgnn_fail(DGNN_E_BADARG, "linear_slope: null, misaligned or overlapping rows%s");
   }
   const int64_t lanes = slope_lanes(N), slab = M > 0 ? slope_slab(M, N) : 1, slabs = ceil_div(M, slab);
-  if (dbias && slabs > 0 && (!workspace || workspace_bytes < slabs * N * 4 || (uintptr_t)workspace % 4))
-    return dgnn_fail(DGNN_E_BADARG, "linear_slope: workspace too small%s (%lld bytes wanted)", "", slabs * N * 4);
+  if (dbias && slabs > 0 && (!workspace || workspace_bytes < slabs * N * 8 || (uintptr_t)workspace % 8))
+    return dgnn_fail(DGNN_E_BADARG, "linear_slope: workspace too small%s (%lld bytes wanted)", "", slabs * N * 8);
   if (M > 0 && (p || dbias)) {
-    const Slope g{dy, save, p, ldd, lds, ldp, M, N, slab, dbias ? (float*)workspace : nullptr, act, (int)lanes};
+    const Slope g{dy, save, p, ldd, lds, ldp, M, N, slab, dbias ? (double*)workspace : nullptr, act, (int)lanes};
     const dim3 grid((uint32_t)ceil_div(N, 4 * lanes), (uint32_t)slabs);
     if (dtype == DGNN_F32) hipLaunchKernelGGL((slope_kernel<float>), grid, dim3(256), 0, s, g);
     else if (dtype == DGNN_BF16) hipLaunchKernelGGL((slope_kernel<__bf16>), grid, dim3(256), 0, s, g);
@@ -280,9 +339,9 @@ int dgnn_linear_slope(const void* dy, int64_t ldd, const void* save, int64_t lds
   }
   if (dbias) {
     const dim3 grid((uint32_t)ceil_div(N, 16));
-    if (dtype == DGNN_F32) hipLaunchKernelGGL((slab_join_kernel<float>), grid, dim3(256), 0, s, (const float*)workspace, slabs, N, (float*)dbias);
-    else if (dtype == DGNN_BF16) hipLaunchKernelGGL((slab_join_kernel<__bf16>), grid, dim3(256), 0, s, (const float*)workspace, slabs, N, (__bf16*)dbias);
-    else hipLaunchKernelGGL((slab_join_kernel<_Float16>), grid, dim3(256), 0, s, (const float*)workspace, slabs, N, (_Float16*)dbias);
+    if (dtype == DGNN_F32) hipLaunchKernelGGL((slab_join_kernel<float>), grid, dim3(256), 0, s, (const double*)workspace, slabs, N, (float*)dbias);
+    else if (dtype == DGNN_BF16) hipLaunchKernelGGL((slab_join_kernel<__bf16>), grid, dim3(256), 0, s, (const double*)workspace, slabs, N, (__bf16*)dbias);
+    else hipLaunchKernelGGL((slab_join_kernel<_Float16>), grid, dim3(256), 0, s, (const double*)workspace, slabs, N, (_Float16*)dbias);
     DGNN_LAUNCHED();
   }
   return DGNN_OK;
@@ -337,6 +396,8 @@ static int64_t backward_parts(int64_t M, int64_t K, int64_t N, int32_t dtype, in
     (void)dgnn_linear_workspace(pass, M, K, N, dtype, &n);
     if (n > most) most = n;
   }
+  *p_bytes = 0;
+  if (small_fit(M, K, N)) return 0;
   *p_bytes = act == ACT_NONE ? 0 : ceil_div(M * N * width(dtype), 256) * 256;
   return *p_bytes + most;
 }
@@ -360,6 +421,26 @@ int dgnn_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
   const int64_t need = backward_parts(M, K, N, dtype, act, &p_bytes);
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return dgnn_fail(DGNN_E_BADARG, "linear_backward: workspace too small or misaligned%s (%lld bytes wanted)", "", need);
+  if (small_fit(M, K, N)) {
+    const int64_t b = width(dtype);
+    if (!matrix_ok(dy, ldd, M, N, b) || (dw && (!matrix_ok(x, ldx, M, K, b) || !matrix_ok(dw, lddw, K, N, b)))
+        || (dx && (!matrix_ok(w, ldw, K, N, b) || !matrix_ok(dx, lddx, M, K, b))) || (uintptr_t)dbias % b
+        || (act == ACT_RELU && (!save || lds < (N + 31) / 32 || (uintptr_t)save % 4)) || (act > ACT_RELU && !matrix_ok(save, lds, M, N, 4)))
+      return dgnn_fail(DGNN_E_BADARG, "linear_backward: null, misaligned or overlapping rows%s");
+    if (!apart(dx, lddx, M, K, dy, ldd, M, N, b) || !apart(dx, lddx, M, K, w, ldw, K, N, b) || !apart(dw, lddw, K, N, x, ldx, M, K, b)
+        || !apart(dw, lddw, K, N, dy, ldd, M, N, b))
+      return dgnn_fail(DGNN_E_BADARG, "linear_backward: an output overlaps an input%s");
+    if (!dx && !dw && !dbias) return DGNN_OK;
+    const int64_t side = M > N ? M : N, chunk = kSmall / side < 1 ? 1 : kSmall / side < 16 ? kSmall / side : 16;
+    const Small g{x, w, dy, save, dx, dw, dbias, ldx, ldw, ldd, lds, lddx, lddw, (int)M, (int)K, (int)N, (int)act, (int)chunk};
+    const dim3 grid(dx || dw ? (uint32_t)ceil_div(K, chunk) : 1);
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == DGNN_F32) hipLaunchKernelGGL((small_backward_kernel<float>), grid, dim3(256), 0, s, g);
+    else if (dtype == DGNN_BF16) hipLaunchKernelGGL((small_backward_kernel<__bf16>), grid, dim3(256), 0, s, g);
+    else hipLaunchKernelGGL((small_backward_kernel<_Float16>), grid, dim3(256), 0, s, g);
+    DGNN_LAUNCHED();
+    return DGNN_OK;
+  }
   char* rest = (char*)workspace + p_bytes;
   const void* p = dy;
   int64_t ldp = ldd;

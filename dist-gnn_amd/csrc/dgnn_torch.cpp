@@ -115,7 +115,7 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const
   const Rows r = rows(residual, "residual", x, M, N);
   const Guard guard(x.device());
   Tensor y = at::empty({M, N}, x.options()), saved;
-  if (save && act) saved = act == DGNN_ACT_RELU ? at::empty({M, (N + 31) / 32}, x.options().dtype(at::kInt)) : at::empty({M, N}, x.options());
+  if (save && act) saved = act == DGNN_ACT_RELU ? at::empty({M, (N + 31) / 32}, x.options().dtype(at::kInt)) : at::empty({M, N}, x.options().dtype(at::kFloat));
   if (M && N) {
     int64_t bytes;
     const Tensor ws = workspace(DGNN_LINEAR_FORWARD, M, K, N, x, &bytes);
@@ -130,7 +130,7 @@ std::pair<Tensor, Tensor> linear_slope(const Tensor& dy, const MaybeTensor& save
   const int64_t M = dy.size(0), N = dy.size(1);
   if (act) {
     const int64_t wide = act == DGNN_ACT_RELU ? (N + 31) / 32 : N;
-    const auto type = act == DGNN_ACT_RELU ? at::kInt : dy.scalar_type();
+    const auto type = act == DGNN_ACT_RELU ? at::kInt : at::kFloat;
     if (!saved || !saved->defined() || saved->dim() != 2 || saved->size(0) != M || saved->size(1) != wide || saved->scalar_type() != type
         || saved->device() != dy.device() || !saved->is_contiguous())
       refuse("spmm_cpp.linear: saved must be what linear_forward returned for this activation and shape");

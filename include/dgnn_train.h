@@ -24,7 +24,7 @@ extern "C" {
  * the exact sum as a chain of fp32 operations), one rounding at the end. relu(NaN) is NaN.
  *   act    DGNN_ACT_*: none, relu, gelu (0.5 t (1 + erf(t / sqrt 2))), silu (t / (1 + e^-t))
  *   save   NULL, or what dgnn_linear_slope needs: for relu uint32 [M][lds], bit n % 32 of word n / 32 set where x W + b is
- *          not <= 0 (lds >= ceil(N / 32), bits past N zero); for gelu and silu x W + b in the matrices' type (lds >= N)
+ *          not <= 0 (lds >= ceil(N / 32), bits past N zero); for gelu and silu x W + b as float (lds >= N)
  * With a gradient dy of y:
  *   dgnn_linear_slope         p = dy act'(x W + b) (p may be NULL), dbias[n] = sum over m of p[m][n] (may be NULL); p may be
  *                             dy itself. act DGNN_ACT_NONE: p is a copy of dy

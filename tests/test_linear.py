@@ -40,8 +40,9 @@ def _backward(x=A, ldx=8, w=B, ldw=8, dy=C, ldd=8, save=D, lds=8, dx=5 << 22, ld
     (_slope, dict(dtype=-1)), (_slope, dict(act=9)), (_slope, dict(save=None)), (_slope, dict(lds=7)), (_slope, dict(dy=None)),
     (_slope, dict(ldp=7)), (_slope, dict(act=1, lds=0)), (_slope, dict(db=D)), (_slope, dict(db=D, ws=D, n=4)), (_slope, dict(db=D + 2)),
     (_grad_input, dict(dtype=5)), (_grad_input, dict(p=None)), (_grad_input, dict(ldx=7)), (_grad_input, dict(dx=A)), (_grad_input, dict(add=D, lda=7)), (_grad_input, dict(add=C)), (_grad_input, dict(N=-2)),
-    (_backward, dict(dtype=5)), (_backward, dict(act=4)), (_backward, dict(M=-1)), (_backward, dict(ws=None)), (_backward, dict(n=100)),
-    (_backward, dict(ws=(8 << 22) + 8)), (_backward, dict(dy=None)), (_backward, dict(save=None)),
+    (_backward, dict(dtype=5)), (_backward, dict(act=4)), (_backward, dict(M=-1)), (_backward, dict(M=600, ws=None)), (_backward, dict(M=600, n=100)),
+    (_backward, dict(M=600, ws=(8 << 22) + 8)), (_backward, dict(ldx=7)), (_backward, dict(w=None)), (_backward, dict(M=600, dy=None)), (_backward, dict(lddw=3)),
+    (_backward, dict(db=(7 << 22) + 2)), (_backward, dict(dx=B)), (_backward, dict(dw=C)), (_backward, dict(act=1, lds=0)), (_backward, dict(dy=None)), (_backward, dict(save=None)),
     (_grad_weight, dict(dtype=5)), (_grad_weight, dict(x=None)), (_grad_weight, dict(ldw=7)), (_grad_weight, dict(dw=B)),
     (_grad_weight, dict(M=1 << 31)), (_grad_weight, dict(M=100000, dw=1 << 40)),                                # cut, no workspace
 ])
@@ -65,7 +66,7 @@ def test_workspace_is_bounded():
                 for N in (0, 1, 16, 41, 256, 4096):
                     for dtype in range(3):
                         assert lib.dgnn_linear_workspace(kind, M, K, N, dtype, ctypes.byref(n)) == 0
-                        assert 0 <= n.value <= (max(256 * 128 * 256 * 4, 6 * (K + 256) * (N + 256), M * (K + N), 4 * K * N) if kind != 1 else 4096 * max(N, 1) * 4)
+                        assert 0 <= n.value <= (max(256 * 128 * 256 * 4, 6 * (K + 256) * (N + 256), M * (K + N), 4 * K * N) if kind != 1 else 4096 * max(N, 1) * 8)
     assert lib.dgnn_linear_workspace(4, 1, 1, 1, 0, ctypes.byref(n)) == 1
     assert lib.dgnn_linear_workspace(0, -1, 1, 1, 0, ctypes.byref(n)) == 1
     assert lib.dgnn_linear_workspace(0, 1, 1, 1, 0, None) == 1

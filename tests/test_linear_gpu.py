@@ -2,11 +2,11 @@
 
 Bounds, with h = eps / 2 of the type (2^-24, bf16 2^-8, fp16 2^-11) and S = sum of |products|:
   sums        the fp32 accumulation of K products in 16s: at most (10 + 12 K / 16) 2^-24 S (six products an fp32 pair, each
-              addition rounded once or truncated), a sixth of the K part for 16-bit operands; n additions of a column sum: n 2^-24 S
+              addition rounded once or truncated), a sixth of the K part for 16-bit operands; column sums are added in 64 bits: 4 2^-24 S
   result      h |result| on top
   activation  |act'| <= 1.13, |act''| <= 0.8; its own evaluation 16 2^-24 (|act| + |argument|)
-  slope       what is saved of x W + b is rounded once: 0.8 (h |pre| + its error) |dy|, and relu's bit may be either where
-              |pre| is within its error; p is rounded once more (h |p|) before the products
+  slope       x W + b is saved in fp32: 0.8 (2^-24 |pre| + its error) |dy|, and relu's bit may be either where |pre| is within
+              its error; p is rounded once (h |p|) before the products
 """
 import itertools
 
@@ -21,7 +21,7 @@ pytestmark = pytest.mark.gpu
 DT = {'f32': torch.float32, 'bf16': torch.bfloat16, 'f16': torch.float16}
 HALF = {k: torch.finfo(t).eps / 2 for k, t in DT.items()}
 U = 2.0 ** -24
-SIZES = [(1, 1, 1), (3, 300, 4099), (8, 4100, 129), (4, 40, 8), (1, 602, 256), (2, 3, 5), (7, 4096, 130), (33, 17, 31), (31, 64, 32), (64, 1433, 16), (129, 40, 41), (257, 602, 256),
+SIZES = [(1, 1, 1), (4096, 3, 1), (1, 20, 4096), (63, 1433, 65), (64, 100, 65), (900, 5, 4), (3, 300, 4099), (8, 4100, 129), (4, 40, 8), (1, 602, 256), (2, 3, 5), (7, 4096, 130), (33, 17, 31), (31, 64, 32), (64, 1433, 16), (129, 40, 41), (257, 602, 256),
          (128, 256, 257), (300, 33, 300), (1000, 7, 64), (4099, 100, 47), (20000, 31, 129)]
 
 
@@ -83,7 +83,7 @@ def _definition(x, w, b, r, dy, dtype, act):
     elif act == 'relu':
         e_p = dy.abs() * (pre.abs() <= e_pre)
     else:
-        e_p = dy.abs() * (0.8 * (h * pre.abs() + 2 * e_pre) + 16 * U * (1 + pre.abs()))
+        e_p = dy.abs() * (0.8 * (U * pre.abs() + 2 * e_pre) + 16 * U * (1 + pre.abs()))
     tiny = 2.0 ** -25 if dtype == 'f16' else 0               # fp16's smallest half step
     e_round = e_p + (h * (p.abs() + e_p) + tiny if act in ('gelu', 'silu') else 0)
     for name, a, c, e, count in (('dx', p, w.t(), None, n), ('dw', x.t(), p, None, m)):
@@ -92,7 +92,7 @@ def _definition(x, w, b, r, dy, dtype, act):
         e = e + _sum_bound(count, dtype) * (a.abs() @ c.abs() + e)
         out[name] = (v, e + h * v.abs() + 1e-40 + tiny)
     v = p.sum(0)
-    e = e_p.sum(0) + (m + 2) * U * (p.abs() + e_p).sum(0)
+    e = e_p.sum(0) + 4 * U * (p.abs() + e_p).sum(0)
     out['db'] = (v, e + h * v.abs() + 1e-40 + tiny)
     out['dr'] = (dy, torch.zeros_like(dy))
     return out
