@@ -2,13 +2,16 @@
 //
 // Per element the step reads p, g and two moments and writes p and the moments: there is nothing to reuse, so the kernel
 // is one pass at the memory's rate and everything else is arranged around that. All tensors of a call are cut into chunks
-// of 4096 elements; a workgroup finds its tensor by bisection in a table that travels in the kernel's arguments (no
-// upload, nothing to keep alive, and a captured graph keeps its own copy), 64 tensors a launch.
+// of 1024 to 4096 elements; a workgroup finds its tensor by bisection in a table that travels in the kernel's arguments (no
+// upload, nothing to keep alive, and a captured graph keeps its own copy), 64 tensors a launch. Values that are touched once
+// are loaded and stored past the caches' usual order of replacement (200 M fp32 elements: 1031 us without, 928 us with).
 //
-// A chunk is 16 blocks of 256 elements, the unit that shares a scale where moments are 8 bits wide. 16 lanes own a block:
-// quad j of lane l is elements 64 j + 4 l .. + 3, so every load of 4 elements is contiguous over the lanes (256 B of fp32,
-// 128 B of 16-bit values, 64 B of codes per block) and the block's maximum is four exchanges among 16 lanes instead of
-// six among 64.
+// 256 elements are the unit that shares a scale where moments are 8 bits wide. 16, 32 or 64 lanes own such a block: quad j
+// of lane l of L is elements 4 (L j + l) .. + 3, so every load of 4 elements is contiguous over the lanes, and the block's
+// maximum is a few exchanges among them.
+//
+// Measured on 200 M elements (bytes read and written): fp32 5.4 to 6.0 TB/s, 8-bit moments with a master copy 6.1, without
+// 4.4 (bf16) to 5.9 (fp32); a large copy reaches 4.75.
 //
 // Compiled without contraction: each operation is rounded once, in the order the header states, so results do not depend
 // on how the compiler fuses.
@@ -22,7 +25,6 @@
 namespace {
 
 constexpr int kBlock = 256;        // elements that share a scale
-constexpr int kChunk = 4096;       // elements a workgroup of 256 lanes takes
 constexpr int kTable = 64;         // tensors a launch: 64 * 48 B of kernel arguments stay under 4 KiB
 
 struct Entry {
@@ -54,15 +56,21 @@ struct State {
 template <typename T> struct Quad { using V = T __attribute__((ext_vector_type(4), aligned(sizeof(T)))); };
 typedef float f4 __attribute__((ext_vector_type(4)));
 
+// Elements a lane takes; a workgroup takes 256 times as many. 32-bit moments are bound by memory alone and want many loads in
+// flight (200 M fp32 elements: 16 928 us, 8 969 us). 8-bit ones are bound by the arithmetic as well and want waves, so few
+// registers (bf16 with a master copy, 200 M elements: 16 996 us, 8 652 us, 4 598 us); without a master copy there is less to
+// load and more of the rest, which 8 share better (16 616 us, 8 458 us, 4 488 us).
+constexpr int each(bool bits8, bool master) { return !bits8 ? 16 : master ? 4 : 8; }
+
 template <typename T> __device__ __forceinline__ float widen(T x) { return (float)x; }
 
 // the largest |x| as bits: NaN above infinity above every finite value, so a value that is not finite is not lost
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-__device__ __forceinline__ uint32_t max16(uint32_t a) {
+template <int LANES> __device__ __forceinline__ uint32_t max_over(uint32_t a) {
 #pragma unroll
-  for (int d = 1; d < 16; d <<= 1) {
-    const uint32_t b = (uint32_t)__shfl_xor((int)a, d, 16);
+  for (int d = 1; d < LANES; d <<= 1) {
+    const uint32_t b = (uint32_t)__shfl_xor((int)a, d, LANES);
     a = a > b ? a : b;
   }
   return a;
@@ -79,11 +87,27 @@ __device__ __forceinline__ float at_step(float x, float u) {
 
 __device__ __forceinline__ float dither(uint32_t h) { return (float)(h >> 16) * 0x1p-16f; }
 
+// The same for |x| >= 2^-6 or x = 0, in three integer operations: |x| / s has 3 bits before the 20 that the addition of
+// the 16 bits of u carries into, and where the sum reaches the next power of two its floor is that power either way.
+__device__ __forceinline__ float at_step_above(float x, uint32_t h) {
+  return __uint_as_float((__float_as_uint(x) + ((h >> 16) << 4)) & 0xfff00000u);
+}
+
+// sqrt(x) rounded to nearest for x = 0 and 2^-96 <= x < inf: x rsq(x) is within 2 ulp, its residual is exact in an fma, and
+// one correction by it rounds right (every float of the range was compared with sqrtf). 6 operations where sqrtf, which has
+// to scale small arguments, takes 16.
+__device__ __forceinline__ float root_above(float x) {
+  const float y = __builtin_amdgcn_rsqf(fmaxf(x, 0x1p-126f));
+  const float g = x * y;
+  return __builtin_fmaf(__builtin_fmaf(-g, g, x), 0.5f * y, g);
+}
+
 constexpr uint32_t kMAlong = 0x6A09E667u, kMAhead = 0x9E3779B9u, kRAlong = 0x3C6EF372u, kRAhead = 0xBB67AE85u;
 
 template <typename T, bool MASTER, bool BITS8>
 __global__ __launch_bounds__(256) void adamw_kernel(const Table tab, const State st) {
   using V4 = typename Quad<T>::V;
+  constexpr int EACH = each(BITS8, MASTER), LANES = kBlock / EACH;                          // elements of a lane, lanes of a block
   int lo = 0, hi = tab.count - 1;
   const uint32_t chunk = blockIdx.x;
   while (lo < hi) {
@@ -100,22 +124,22 @@ __global__ __launch_bounds__(256) void adamw_kernel(const Table tab, const State
     const float* f = st.factors + 4 * (int64_t)e.index;
     rate = f[0]; root_c = f[1]; turn = __float_as_uint(f[2]);
   }
-  const int lane = threadIdx.x & 15, blk = threadIdx.x >> 4;
-  const int64_t at = (int64_t)(chunk - tab.first[lo]) * kChunk + blk * kBlock;      // this block's first element
-  if (at >= numel) return;                                                          // whole 16-lane groups
+  const int lane = threadIdx.x % LANES, blk = threadIdx.x / LANES;
+  const int64_t at = (int64_t)(chunk - tab.first[lo]) * (256 * EACH) + blk * kBlock;      // this block's first element
+  if (at >= numel) return;                                                          // whole blocks
   const int64_t sat = (int64_t)e.start * kBlock + at;                               // and its place in the state
   const bool whole = at + kBlock <= numel;
   const int left = whole ? kBlock : (int)(numel - at);
 
-  float pw[16], gw[16], m[16], v[16];                                               // v holds the root where BITS8
+  float pw[EACH], gw[EACH], m[EACH], v[EACH];                                               // v holds the root where BITS8
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int q = 64 * j + 4 * lane;
+  for (int j = 0; j < EACH / 4; ++j) {
+    const int q = 4 * (LANES * j + lane);
     if (whole) {
-      const V4 gv = *reinterpret_cast<const V4*>(g + at + q);
+      const V4 gv = __builtin_nontemporal_load(reinterpret_cast<const V4*>(g + at + q));
 #pragma unroll
       for (int i = 0; i < 4; ++i) gw[4 * j + i] = widen(gv[i]);
-      const V4 pv = *reinterpret_cast<const V4*>(p + at + q);
+      const V4 pv = __builtin_nontemporal_load(reinterpret_cast<const V4*>(p + at + q));
 #pragma unroll
       for (int i = 0; i < 4; ++i) pw[4 * j + i] = widen(pv[i]);
     } else {
@@ -126,7 +150,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const Table tab, const State
       }
     }
     if constexpr (MASTER) {
-      const f4 wide = *reinterpret_cast<const f4*>(st.master + sat + q);
+      const f4 wide = __builtin_nontemporal_load(reinterpret_cast<const f4*>(st.master + sat + q));
 #pragma unroll
       for (int i = 0; i < 4; ++i)                                                   // else p was written by somebody else
         if (__float_as_uint(widen((T)wide[i])) == __float_as_uint(pw[4 * j + i])) pw[4 * j + i] = wide[i];
@@ -143,8 +167,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(const Table tab, const State
       v[4 * j + 2] = __builtin_amdgcn_cvt_f32_fp8((int)vc, 2);
       v[4 * j + 3] = __builtin_amdgcn_cvt_f32_fp8((int)vc, 3);
     } else {
-      const f4 mv = *reinterpret_cast<const f4*>((const float*)st.m + sat + q);
-      const f4 vv = *reinterpret_cast<const f4*>((const float*)st.v + sat + q);
+      const f4 mv = __builtin_nontemporal_load(reinterpret_cast<const f4*>((const float*)st.m + sat + q));
+      const f4 vv = __builtin_nontemporal_load(reinterpret_cast<const f4*>((const float*)st.v + sat + q));
 #pragma unroll
       for (int i = 0; i < 4; ++i) { m[4 * j + i] = mv[i]; v[4 * j + i] = vv[i]; }
     }
@@ -153,9 +177,9 @@ __global__ __launch_bounds__(256) void adamw_kernel(const Table tab, const State
   const int64_t b = sat / kBlock;
   float ms = 0.f, vs = 0.f;
   if constexpr (BITS8) { ms = st.m_scale[b]; vs = st.v_scale[b]; }
-  uint32_t mtop = 0, vtop = 0;
+  uint32_t mtop = 0, vtop = 0, low = 0xffffffffu, high = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < EACH; ++i) {
     float mi = m[i], vi = v[i];
     const float gi = gw[i];
     if constexpr (BITS8) {
@@ -163,46 +187,78 @@ __global__ __launch_bounds__(256) void adamw_kernel(const Table tab, const State
       const float r = vi * vs;
       vi = r * r;
     }
-    mi = mi * st.b1 + gi * st.c1;
-    vi = vi * st.b2 + (gi * gi) * st.c2;
-    const float r = sqrtf(vi);
-    const float step = mi / (r * root_c + st.eps);
-    pw[i] = pw[i] * e.decay - step * rate;
-    m[i] = mi;
-    v[i] = BITS8 ? r : vi;
+    m[i] = mi * st.b1 + gi * st.c1;
+    v[i] = vi * st.b2 + (gi * gi) * st.c2;
     if constexpr (BITS8) {
-      if (whole || 64 * (i >> 2) + 4 * lane + (i & 3) < left) {
-        mtop = max(mtop, magnitude(mi));
+      low = min(low, __float_as_uint(v[i]) - 1);                                    // zero wraps round to the top
+      high = max(high, __float_as_uint(v[i]));
+    }
+  }
+  if constexpr (BITS8) {
+    if (__any(low < 0x0f800000u - 1 || high >= 0x7f800000u)) {
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) v[i] = sqrtf(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) v[i] = root_above(v[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const float r = BITS8 ? v[i] : sqrtf(v[i]);
+    const float step = m[i] / (r * root_c + st.eps);
+    pw[i] = pw[i] * e.decay - step * rate;
+    if constexpr (BITS8) {
+      if (whole || 4 * (LANES * (i >> 2) + lane) + (i & 3) < left) {
+        mtop = max(mtop, magnitude(m[i]));
         vtop = max(vtop, magnitude(r));
       }
     }
   }
 
   if constexpr (BITS8) {
-    mtop = max(max16(mtop), __float_as_uint(0x1p-100f));
-    vtop = max(max16(vtop), __float_as_uint(0x1p-100f));
+    mtop = max(max_over<LANES>(mtop), __float_as_uint(0x1p-100f));
+    vtop = max(max_over<LANES>(vtop), __float_as_uint(0x1p-100f));
     const float mt = __uint_as_float(mtop), vt = __uint_as_float(vtop);
     const float minv = 448.f / mt, vinv = 448.f / vt;
     if (lane == 0) { st.m_scale[b] = mt * (1.f / 448.f); st.v_scale[b] = vt * (1.f / 448.f); }
     const uint32_t hm = (uint32_t)(at + 4 * lane) * kMAlong + turn * kMAhead;
     const uint32_t hr = (uint32_t)(at + 4 * lane) * kRAlong + turn * kRAhead;
+    low = 0xffffffffu;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t k = 64 * (i >> 2) + (i & 3);
-      m[i] = at_step(m[i] * minv, dither(hm + k * kMAlong));
-      const float c = at_step(v[i] * vinv, dither(hr + k * kRAlong));
-      v[i] = v[i] > 0.f && c < 0x1p-9f ? 0x1p-9f : c;
+    for (int i = 0; i < EACH; ++i) {
+      m[i] = m[i] * minv;
+      v[i] = v[i] * vinv;
+      low = min(low, (__float_as_uint(m[i]) << 1) - 2);                             // without the sign
+      low = min(low, (__float_as_uint(v[i]) << 1) - 2);
+    }
+    // A value below 2^-6 of the codes' 448 is one in 10^4 of normally distributed ones, so most waves have none
+    if (__any(low < (0x3c800000u << 1) - 2 || mtop >= 0x7f800000u || vtop >= 0x7f800000u)) {
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const uint32_t k = 4 * LANES * (i >> 2) + (i & 3);
+        m[i] = at_step(m[i], dither(hm + k * kMAlong));
+        const float c = at_step(v[i], dither(hr + k * kRAlong));
+        v[i] = v[i] > 0.f && c < 0x1p-9f ? 0x1p-9f : c;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const uint32_t k = 4 * LANES * (i >> 2) + (i & 3);
+        m[i] = at_step_above(m[i], hm + k * kMAlong);
+        v[i] = at_step_above(v[i], hr + k * kRAlong);
+      }
     }
   }
 
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int q = 64 * j + 4 * lane;
+  for (int j = 0; j < EACH / 4; ++j) {
+    const int q = 4 * (LANES * j + lane);
     if (whole) {
       V4 pv;
 #pragma unroll
       for (int i = 0; i < 4; ++i) pv[i] = (T)pw[4 * j + i];
-      *reinterpret_cast<V4*>(p + at + q) = pv;
+      __builtin_nontemporal_store(pv, reinterpret_cast<V4*>(p + at + q));
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -212,7 +268,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const Table tab, const State
       f4 pv;
 #pragma unroll
       for (int i = 0; i < 4; ++i) pv[i] = whole || q + i < left ? pw[4 * j + i] : 0.f;
-      *reinterpret_cast<f4*>(st.master + sat + q) = pv;
+      __builtin_nontemporal_store(pv, reinterpret_cast<f4*>(st.master + sat + q));
     }
     if constexpr (BITS8) {
       int mc = __builtin_amdgcn_cvt_pk_fp8_f32(m[4 * j], m[4 * j + 1], 0, false);
@@ -225,8 +281,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(const Table tab, const State
       f4 mv, vv;
 #pragma unroll
       for (int i = 0; i < 4; ++i) { mv[i] = m[4 * j + i]; vv[i] = v[4 * j + i]; }
-      *reinterpret_cast<f4*>((float*)st.m + sat + q) = mv;
-      *reinterpret_cast<f4*>((float*)st.v + sat + q) = vv;
+      __builtin_nontemporal_store(mv, reinterpret_cast<f4*>((float*)st.m + sat + q));
+      __builtin_nontemporal_store(vv, reinterpret_cast<f4*>((float*)st.v + sat + q));
     }
   }
 }
@@ -286,6 +342,7 @@ extern "C" int dgnn_adamw(const struct dgnn_adamw_tensor* tensors, int32_t count
   hipStream_t s = (hipStream_t)stream;
   const State st{state->exp_avg, state->exp_avg_sq, state->exp_avg_scale, state->exp_avg_sq_scale, state->master, state->factors,
                  (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
+  const int64_t chunk = 256 * each(state_bits == 8, state->master != nullptr);
   constexpr int64_t most = 1 << 30;                      // chunks a launch
   for (int32_t i = 0; i < count;) {
     Table tab;
@@ -293,7 +350,7 @@ extern "C" int dgnn_adamw(const struct dgnn_adamw_tensor* tensors, int32_t count
     int64_t chunks = 0;
     while (i < count && tab.count < kTable) {
       const struct dgnn_adamw_tensor& t = tensors[i];
-      const int64_t need = (t.numel + kChunk - 1) / kChunk;
+      const int64_t need = (t.numel + chunk - 1) / chunk;
       if (chunks + need > most && tab.count) break;
       if (need || state->steps) {                        // an empty tensor still counts its steps
         tab.first[tab.count] = (uint32_t)chunks;
