@@ -46,11 +46,39 @@ struct Gemm {
   hipStream_t stream;
 };
 
-__device__ __forceinline__ float act_of(int act, float t) {
+// The normal distribution's density e = exp(-t^2/2) (times sqrt(2 pi)) and tail Phi(-|t|), for results of 16 bits: the tail is
+// e u P(u), u = 1 / (1 + 0.36 |t|), P fitted to a relative error below 1e-6 over |t| <= 14, beyond which both are 0 in
+// fp32 -- 2^-9 is what a result's rounding is off by. 15 operations where erff and expf take some 60.
+__device__ __forceinline__ void normal_tail(float t, float& e, float& tail) {
+  const float u = __builtin_amdgcn_rcpf(fmaf(0.36f, fabsf(t), 1.f));
+  e = __builtin_amdgcn_exp2f(t * t * -0.72134752044448170f);
+  float q = 0.04706796788f;
+  q = fmaf(q, u, -0.1798049046f);
+  q = fmaf(q, u, 0.1810091365f);
+  q = fmaf(q, u, 0.02651105193f);
+  q = fmaf(q, u, 0.1397333685f);
+  q = fmaf(q, u, 0.1417698558f);
+  q = fmaf(q, u, 0.1437132311f);
+  tail = e * u * q;
+}
+
+template <typename T> __device__ __forceinline__ float sigmoid_of(float t) {
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t * -1.4426950408889634f));
+  else return 1.f / (1.f + expf(-t));
+}
+
+template <typename T> __device__ __forceinline__ float act_of(int act, float t) {
   switch (act) {
     case ACT_RELU: return t <= 0.f ? 0.f : t;
-    case ACT_GELU: return 0.5f * t * (1.f + erff(t * 0.70710678118654752f));
-    case ACT_SILU: return t / (1.f + expf(-t));
+    case ACT_GELU:
+      if constexpr (sizeof(T) == 2) {
+        float e, tail;
+        normal_tail(t, e, tail);
+        return t * (t < 0.f ? tail : 1.f - tail);
+      } else {
+        return 0.5f * t * (1.f + erff(t * 0.70710678118654752f));
+      }
+    case ACT_SILU: return sizeof(T) == 2 ? t * sigmoid_of<T>(t) : t / (1.f + expf(-t));
     default: return t;
   }
 }
@@ -291,15 +319,15 @@ __device__ __forceinline__ void finish(const Gemm& g, int64_t row, int64_t col, 
     case ACT_NONE: break;
     case ACT_RELU:
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = act_of(ACT_RELU, v[i]);
+      for (int i = 0; i < 4; ++i) v[i] = act_of<T>(ACT_RELU, v[i]);
       break;
     case ACT_GELU:
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = act_of(ACT_GELU, v[i]);
+      for (int i = 0; i < 4; ++i) v[i] = act_of<T>(ACT_GELU, v[i]);
       break;
     default:
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = act_of(ACT_SILU, v[i]);
+      for (int i = 0; i < 4; ++i) v[i] = act_of<T>(ACT_SILU, v[i]);
   }
   if (g.residual) {
 #pragma unroll
@@ -439,52 +467,62 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm g) {
                               col0 + wn * TN * 32, k0, kend);
 }
 
-// Joins the slices of a product that was cut along its contraction and finishes it: 32 fours of columns a workgroup, 8 lanes
-// to a four, each adding every 8th slice with up to 8 loads in flight, in 64 bits; the 8 sums meet in their order. A row takes a multiple of
-// 8 fours, so that relu's bits are whole words.
-template <typename T>
+// Joins the slices of a product that was cut along its contraction and finishes it, in 64 bits: PARTS lanes to a four of
+// columns, each adding every PARTS-th slice with up to 8 loads in flight; the PARTS sums meet in their order. Up to 8 slices
+// one lane has them all in flight by itself (1024 x 4096 bf16 from 2: 30 us with 8 lanes, 11 with one); with more, as
+// small outputs have them, 8 lanes shorten the chain. A row takes a multiple of 8 fours, so that relu's bits are whole words.
+template <typename T, int PARTS>
 __global__ __launch_bounds__(256) void gemm_join_kernel(const Gemm g) {
-  __shared__ double sums[8][32][4];
-  const int four = threadIdx.x & 31, part = threadIdx.x >> 5;
+  constexpr int FOURS = 256 / PARTS;
+  __shared__ double sums[PARTS > 1 ? PARTS : 1][PARTS > 1 ? FOURS : 1][4];
+  const int four = threadIdx.x % FOURS, part = threadIdx.x / FOURS;
   const int64_t wide = (g.N + 31) / 32 * 8;
-  const int64_t at = (int64_t)blockIdx.x * 32 + four;
+  const int64_t at = (int64_t)blockIdx.x * FOURS + four;
   const int64_t row = at / wide, col = at % wide * 4;
   const int have = row < g.M && col < g.N ? (g.N - col >= 4 ? 4 : (int)(g.N - col)) : 0;
   double sum[4] = {0.0, 0.0, 0.0, 0.0};
   if (have) {
     const float* p = g.partial + row * g.N + col;
     const int64_t step = g.M * g.N;
-    for (int s = part; s < g.slices; s += 64) {
+    for (int s = part; s < g.slices; s += 8 * PARTS) {
       float t[8][4];
 #pragma unroll
       for (int u = 0; u < 8; ++u)
-        if (s + 8 * u < g.slices) load4(p + (s + 8 * u) * step, have, t[u]);
+        if (s + PARTS * u < g.slices) load4(p + (s + PARTS * u) * step, have, t[u]);
 #pragma unroll
       for (int u = 0; u < 8; ++u)
-        if (s + 8 * u < g.slices) {
+        if (s + PARTS * u < g.slices) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) sum[i] += t[u][i];
         }
     }
   }
+  if constexpr (PARTS > 1) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sums[part][four][i] = sum[i];
-  __syncthreads();
-  if (part) return;
+    for (int i = 0; i < 4; ++i) sums[part][four][i] = sum[i];
+    __syncthreads();
+    if (part) return;
+  }
   float bias[4] = {0.f, 0.f, 0.f, 0.f}, res[4] = {0.f, 0.f, 0.f, 0.f};
   if (have && g.bias) load4((const T*)g.bias + col, have, bias);
   if (have && g.residual) load4((const T*)g.residual + row * g.ld_residual + col, have, res);
+  if constexpr (PARTS > 1) {
 #pragma unroll
-  for (int k = 1; k < 8; ++k)
+    for (int k = 1; k < PARTS; ++k)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] += sums[k][four][i];
+      for (int i = 0; i < 4; ++i) sum[i] += sums[k][four][i];
+  }
   float v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = (float)sum[i];
   finish<T>(g, row, col, have, v, bias, res);
 }
 
-inline uint32_t join_blocks(const Gemm& g) { return (uint32_t)((g.M * ((g.N + 31) / 32 * 8) + 31) / 32); }
+template <typename T> void join(const Gemm& g) {
+  const int64_t fours = g.M * ((g.N + 31) / 32 * 8);
+  if (g.slices <= 8) hipLaunchKernelGGL((gemm_join_kernel<T, 1>), dim3((uint32_t)((fours + 255) / 256)), dim3(256), 0, g.stream, g);
+  else hipLaunchKernelGGL((gemm_join_kernel<T, 8>), dim3((uint32_t)((fours + 31) / 32)), dim3(256), 0, g.stream, g);
+}
 
 // ---------------------------------------------------------------------------------------
 // Many rows (forward and input gradient of whole graphs or batches). W is laid out first, once a call: zero-padded chunks in the
@@ -664,7 +702,7 @@ __device__ __forceinline__ void rows_out(const Gemm& g, const f16v (&acc)[TN], c
       }
     }
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = act_of(ACT, v[e]);
+    for (int e = 0; e < 16; ++e) v[e] = act_of<T>(ACT, v[e]);
     if (g.residual) {
       float r[16];
       Out<T>::unpack(res[j], r);
@@ -1131,7 +1169,7 @@ inline int columns_launch(const Gemm& g) {
   }
   DGNN_LAUNCHED();
   if (g.slices > 1) {
-    hipLaunchKernelGGL((gemm_join_kernel<float>), dim3(join_blocks(g)), dim3(256), 0, g.stream, g);
+    join<float>(g);
     DGNN_LAUNCHED();
   }
   return DGNN_OK;
@@ -1147,7 +1185,7 @@ inline int columns_launch(const Gemm& g) {
 // ---------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ void thin_out(const Gemm& g, int64_t row, int64_t col, float t) {
   if (g.save && g.act > ACT_RELU) ((float*)g.save)[row * g.ld_save + col] = t;
-  t = act_of(g.act, t);
+  t = act_of<T>(g.act, t);
   if (g.residual) t += (float)((const T*)g.residual)[row * g.ld_residual + col];
   ((T*)g.c)[row * g.ldc + col] = (T)t;
 }
@@ -1322,7 +1360,7 @@ int thin_launch(const Gemm& g) {
       const int64_t blocks = (cols + 64 * W - 1) / (64 * W);
       hipLaunchKernelGGL((thin_across_kernel<T, ROWS, 8, 16, 64, 64>), dim3((uint32_t)((blocks + 7) / 8 * 8), (uint32_t)g.slices), dim3(512), 0, g.stream, g, 64);
       DGNN_LAUNCHED();
-      hipLaunchKernelGGL((gemm_join_kernel<T>), dim3(join_blocks(g)), dim3(256), 0, g.stream, g);
+      join<T>(g);
     }
   }
   DGNN_LAUNCHED();
@@ -1362,7 +1400,7 @@ int gemm_launch(const Gemm& g) {
   }
   DGNN_LAUNCHED();
   if (g.slices > 1) {
-    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3(join_blocks(g)), dim3(256), 0, g.stream, g);
+    join<T>(g);
     DGNN_LAUNCHED();
   }
   return DGNN_OK;

@@ -23,15 +23,24 @@ struct Slope {
   int act, lanes;
 };
 
-__device__ __forceinline__ float slope_of(int act, float t) {
-  if (act == ACT_GELU) return 0.5f * (1.f + erff(t * 0.70710678118654752f)) + t * expf(-0.5f * t * t) * 0.39894228040143268f;
-  const float s = 1.f / (1.f + expf(-t));
+template <typename T> __device__ __forceinline__ float slope_of(int act, float t) {
+  if (act == ACT_GELU) {
+    if constexpr (sizeof(T) == 2) {
+      float e, tail;
+      normal_tail(t, e, tail);
+      return fmaf(t, e * 0.39894228040143268f, t < 0.f ? tail : 1.f - tail);
+    } else {
+      return 0.5f * (1.f + erff(t * 0.70710678118654752f)) + t * expf(-0.5f * t * t) * 0.39894228040143268f;
+    }
+  }
+  const float s = sigmoid_of<T>(t);
   return s * (1.f + t * (1.f - s));
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(const Slope g) {
   typedef T quad __attribute__((ext_vector_type(4), aligned(sizeof(T) == 4 ? 4 : 2)));
+  typedef float wide __attribute__((ext_vector_type(4), aligned(4)));
   __shared__ double sums[256][4];
   const int lane = threadIdx.x % g.lanes, group = threadIdx.x / g.lanes, groups = 256 / g.lanes;
   const int64_t col = ((int64_t)blockIdx.x * g.lanes + lane) * 4;
@@ -40,41 +49,61 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope g) {
   const int have = g.N - col >= 4 ? 4 : (g.N > col ? (int)(g.N - col) : 0);
   double sum[4] = {0.0, 0.0, 0.0, 0.0};
   if (have > 0) {
-    for (int64_t row = first + group; row < last; row += groups) {
-      const T* dy = (const T*)g.dy + row * g.ld_dy + col;
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (have == 4) {
-        const quad q = *reinterpret_cast<const quad*>(dy);
+    constexpr int AT_ONCE = 4;                               // rows whose loads are in flight together
+    for (int64_t row0 = first + group; row0 < last; row0 += AT_ONCE * groups) {
+      float v[AT_ONCE][4], pre[AT_ONCE][4];
+      uint32_t word[AT_ONCE];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (float)q[i];
-      } else {
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int64_t row = row0 + k * groups;
+        const bool in = row < last;
+        const T* dy = (const T*)g.dy + row * g.ld_dy + col;
+        if (in && have == 4) {
+          const quad q = *reinterpret_cast<const quad*>(dy);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < have) v[i] = (float)dy[i];
-      }
-      if (g.act == ACT_RELU) {
-        const uint32_t word = ((const uint32_t*)g.save)[row * g.ld_save + col / 32] >> (col & 31);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (word >> i) & 1 ? v[i] : 0.f;
-      } else if (g.act != ACT_NONE) {
-        const float* pre = (const float*)g.save + row * g.ld_save + col;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < have) v[i] *= slope_of(g.act, pre[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] += v[i];
-      if (g.p) {
-        T* p = (T*)g.p + row * g.ld_p + col;
-        if (have == 4) {
-          quad q;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) q[i] = (T)v[i];
-          *reinterpret_cast<quad*>(p) = q;
+          for (int i = 0; i < 4; ++i) v[k][i] = (float)q[i];
         } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (i < have) p[i] = (T)v[i];
+          for (int i = 0; i < 4; ++i) v[k][i] = in && i < have ? (float)dy[i] : 0.f;
+        }
+        if (g.act == ACT_RELU) word[k] = in ? ((const uint32_t*)g.save)[row * g.ld_save + col / 32] >> (col & 31) : 0;
+        else if (g.act != ACT_NONE) {
+          const float* at = (const float*)g.save + row * g.ld_save + col;
+          if (in && have == 4) {
+            const wide q = *reinterpret_cast<const wide*>(at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pre[k][i] = q[i];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pre[k][i] = in && i < have ? at[i] : 0.f;
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int64_t row = row0 + k * groups;
+        if (row >= last) break;
+        if (g.act == ACT_RELU) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[k][i] = (word[k] >> i) & 1 ? v[k][i] : 0.f;
+        } else if (g.act != ACT_NONE) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[k][i] *= slope_of<T>(g.act, pre[k][i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += v[k][i];
+        if (g.p) {
+          T* p = (T*)g.p + row * g.ld_p + col;
+          if (have == 4) {
+            quad q;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = (T)v[k][i];
+            *reinterpret_cast<quad*>(p) = q;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (i < have) p[i] = (T)v[k][i];
+          }
         }
       }
     }
@@ -156,7 +185,7 @@ __global__ __launch_bounds__(256) void small_backward_kernel(const Small g) {
     const int m = i / N, n = i % N;
     float v = (float)((const T*)g.dy)[m * g.ldd + n];
     if (g.act == ACT_RELU) v = ((const uint32_t*)g.save)[m * g.lds + n / 32] >> (n & 31) & 1 ? v : 0.f;
-    else if (g.act != ACT_NONE) v *= slope_of(g.act, ((const float*)g.save)[m * g.lds + n]);
+    else if (g.act != ACT_NONE) v *= slope_of<T>(g.act, ((const float*)g.save)[m * g.lds + n]);
     p[i] = v;
   }
   if (g.dw)

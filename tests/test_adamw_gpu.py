@@ -119,6 +119,30 @@ def test_steps_to_the_bit(dtype, master, bits):
     del buf
 
 
+@pytest.mark.parametrize('dtype,master', CASES)
+def test_codes_over_the_whole_range(dtype, master):
+    """Blocks of gradients that fit one another and blocks whose values lie many powers of ten apart, are zero but for one in
+    ten, or whose squares are below the normal numbers: the same bits, whichever way a wave rounds and takes its roots."""
+    params = _params((256 * 40 + 37, 256 * 8), DT[dtype], 11)
+    opt = spmm_cpp.AdamW(params, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=DECAY, state_bits=8, master_weights=master)
+    twins = [_Twin(p, 8, master, np.float32) for p in params]
+    rng = np.random.default_rng(5)
+    for k in range(3):
+        for p, t in zip(params, twins):
+            n = p.numel()
+            g, block = rng.standard_normal(n), np.arange(n) // 256
+            kind = (block + 3 * k) % 5
+            g = np.where(kind == 1, g * 10.0 ** rng.uniform(-12, 2, n), g)
+            g = np.where((kind == 2) & (rng.random(n) < 0.9), 0.0, g)
+            g = np.where(kind == 3, g * 1e-22, g)
+            g = np.where((kind == 4) & (block % 2 == 0), 0.0, g)
+            p.grad = torch.from_numpy(g.astype(np.float32)).cuda().to(p.dtype)
+        opt.step()
+        for p, t in zip(params, twins):
+            t.step(_np(p.grad).reshape(-1), DT[dtype])
+            _check_state(opt, p, t, DT[dtype], True)
+
+
 def test_against_64_bits():
     """fp32 moments and parameters after 5 steps within what their roundings allow: m and v lose at most 3 half steps a step
     (two products, a sum), the update 6 more relative to itself, the parameter 2 relative to itself."""
