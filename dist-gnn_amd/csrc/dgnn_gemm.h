@@ -715,7 +715,7 @@ __device__ __forceinline__ void rows_out(const Gemm& g, const f16v (&acc)[TN], c
   });
 }
 
-// What a wave of the two kernels below does: TN column tiles of 32 rows.
+// What a wave of rows_kernel does for a block of rows: TN column tiles of 32 rows.
 template <typename T, int TN> struct Wave {
   static constexpr int BK = Rows<T>::BK, CH = BK / 8, PL = Unit<T>::PLANES, BN = TN * 32, S = BK / 16;
   static constexpr int STAGE = PL * CH * BN * 16;             // bytes of a stage of W's image
@@ -736,7 +736,7 @@ template <typename T, int TN> struct Wave {
       }
   }
 
-  // stage kt of the row whose lane part begins at p; `to` may be another wave state's
+  // stage kt of the row whose lane part begins at p
   static __device__ __forceinline__ void fetch(const T* p, int64_t K, int kt, int half, bool over, Eight<T> (&to)[S]) {
     const T* q = p + (int64_t)kt * BK;
     const int64_t left = K - (int64_t)kt * BK;
@@ -751,9 +751,9 @@ template <typename T, int TN> struct Wave {
     }
   }
 
-  // `from` points at this lane's chunks: stage + ((lane / 32) BN + lane % 32) chunks. The next tile's chunks are read before
-  // a tile's products are issued.
-  __device__ __forceinline__ void multiply(const char* from) {
+  // Multiplies R blocks by the same stage of W. `from` points at this lane's chunks: stage + ((lane / 32) BN + lane % 32)
+  // chunks. The next tile's chunks are read before a tile's products are issued.
+  template <int R> static __device__ __forceinline__ void multiply(Wave (&v)[R], const char* from) {
     u4 y[2][PL];
     auto read = [&](int s, int j, u4 (&to)[PL]) __attribute__((always_inline)) {
 #pragma unroll
@@ -762,14 +762,17 @@ template <typename T, int TN> struct Wave {
     read(0, 0, y[0]);
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      u4 x[PL];
-      if constexpr (PL == 3) {
-        float v[8];
+      u4 x[R][PL];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(a[s].q[i / 4][i % 4]);
-        split8(v, x);
-      } else {
-        x[0] = a[s].q[0];
+      for (int r = 0; r < R; ++r) {
+        if constexpr (PL == 3) {
+          float w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = __uint_as_float(v[r].a[s].q[i / 4][i % 4]);
+          split8(w, x[r]);
+        } else {
+          x[r][0] = v[r].a[s].q[0];
+        }
       }
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
@@ -777,14 +780,17 @@ template <typename T, int TN> struct Wave {
         if (j + 1 < TN) read(s, j + 1, y[t ^ 1]);
         else if (s + 1 < S) read(s + 1, 0, y[t ^ 1]);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (PL == 3) {                               // small products first
-          acc[j] = mfma(y[t][0], x[2], acc[j], T());
-          acc[j] = mfma(y[t][2], x[0], acc[j], T());
-          acc[j] = mfma(y[t][1], x[1], acc[j], T());
-          acc[j] = mfma(y[t][0], x[1], acc[j], T());
-          acc[j] = mfma(y[t][1], x[0], acc[j], T());
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          if constexpr (PL == 3) {                             // small products first
+            v[r].acc[j] = mfma(y[t][0], x[r][2], v[r].acc[j], T());
+            v[r].acc[j] = mfma(y[t][2], x[r][0], v[r].acc[j], T());
+            v[r].acc[j] = mfma(y[t][1], x[r][1], v[r].acc[j], T());
+            v[r].acc[j] = mfma(y[t][0], x[r][1], v[r].acc[j], T());
+            v[r].acc[j] = mfma(y[t][1], x[r][0], v[r].acc[j], T());
+          }
+          v[r].acc[j] = mfma(y[t][0], x[r][0], v[r].acc[j], T());
         }
-        acc[j] = mfma(y[t][0], x[0], acc[j], T());
       }
     }
   }
@@ -840,8 +846,8 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 
 // W's stages go round two buffers in LDS, copied there by the memory unit itself while the stage before is multiplied; each
 // buffer is an array of its own, so that the compiler sees that a copy into one does not touch the reads of the other.
-template <typename T, int TN, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, 3) void rows_kernel(const Gemm g, const char* image, int ktiles) {
+template <typename T, int TN, int WAVES, int R>
+__global__ __launch_bounds__(WAVES * 64, R == 2 ? 2 : 3) void rows_kernel(const Gemm g, const char* image, int ktiles) {
   using V = Wave<T, TN>;
   constexpr int STAGE = V::STAGE, PIECES = STAGE / 1024, PER = (PIECES + WAVES - 1) / WAVES;
   __shared__ __attribute__((aligned(16))) char even[STAGE];
@@ -850,11 +856,17 @@ __global__ __launch_bounds__(WAVES * 64, 3) void rows_kernel(const Gemm g, const
   // consecutive workgroups go round the 8 XCDs: the column tiles of a row block stay on one of them, one after the other
   const int64_t ntiles = (g.N + V::BN - 1) / V::BN, turn = blockIdx.x / 8;
   const int64_t nt = turn % ntiles, group = turn / ntiles * 8 + blockIdx.x % 8;
-  const int64_t row = (group * WAVES + wave) * 32 + (lane & 31);
-  if (group * WAVES * 32 >= g.M) return;
+  const int64_t row = (group * WAVES + wave) * 32 * R + (lane & 31);
+  if (group * WAVES * 32 * R >= g.M) return;
   const char* w = image + nt * ktiles * STAGE + lane * 16;
-  const T* p = (const T*)g.a + (row < g.M ? row : g.M - 1) * g.lda + 8 * half;
-  const bool over = row + 1 < g.M && g.lda >= 8;
+  const T* p[R];
+  bool over[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t at = row + 32 * r;
+    p[r] = (const T*)g.a + (at < g.M ? at : g.M - 1) * g.lda + 8 * half;
+    over[r] = at + 1 < g.M && g.lda >= 8;
+  }
   auto send = [&](int kt, char* to) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -866,67 +878,31 @@ __global__ __launch_bounds__(WAVES * 64, 3) void rows_kernel(const Gemm g, const
   // everything on its way has arrived, and every wave is done with what it read
   auto meet = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
-  V v;
-  Eight<T> next[V::S];
+  V v[R];
+  Eight<T> next[R][V::S];
   send(0, even);
-  V::fetch(p, g.K, 0, half, over, v.a);
-  v.begin(g, nt * V::BN, half);
+#pragma unroll
+  for (int r = 0; r < R; ++r) V::fetch(p[r], g.K, 0, half, over[r], v[r].a);
+  each<0, R>([&](auto r) __attribute__((always_inline)) { v[r].begin(g, nt * V::BN, half); });
   meet();
   auto step = [&](int kt, const char* from, char* to) __attribute__((always_inline)) {
     if (kt + 1 < ktiles) {
       send(kt + 1, to);
-      V::fetch(p, g.K, kt + 1, half, over, next);
+#pragma unroll
+      for (int r = 0; r < R; ++r) V::fetch(p[r], g.K, kt + 1, half, over[r], next[r]);
     }
-    v.multiply(from + ((lane >> 5) * V::BN + (lane & 31)) * 16);
+    V::multiply(v, from + ((lane >> 5) * V::BN + (lane & 31)) * 16);
     meet();
 #pragma unroll
-    for (int s = 0; s < V::S; ++s) v.a[s] = next[s];
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int s = 0; s < V::S; ++s) v[r].a[s] = next[r][s];
   };
   for (int kt = 0; kt < ktiles; kt += 2) {
     step(kt, even, odd);
     if (kt + 1 < ktiles) step(kt + 1, odd, even);
   }
-  v.finish(g, row, nt * V::BN, half);
-}
-
-// The same where the whole image of W fits LDS: it is copied there once, and the waves walk over row blocks on their own,
-// the next stage of rows (the next block's first one at the end) always on its way.
-template <typename T, int TN, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, 2) void rows_resident_kernel(const Gemm g, const char* image, int ktiles) {
-  using V = Wave<T, TN>;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  for (int i = tid; i < ktiles * (V::STAGE / 16); i += WAVES * 64) reinterpret_cast<u4*>(lds)[i] = reinterpret_cast<const u4*>(image)[i];
-  __syncthreads();
-  const int64_t blocks = (g.M + 31) / 32, stride = (int64_t)gridDim.x * WAVES;
-  int64_t block = (int64_t)blockIdx.x * WAVES + wave;
-  if (block >= blocks) return;
-  bool over = false;
-  auto part = [&](int64_t at) __attribute__((always_inline)) {
-    const int64_t row = at * 32 + (lane & 31);
-    over = row + 1 < g.M && g.lda >= 8;
-    return (const T*)g.a + (row < g.M ? row : g.M - 1) * g.lda + 8 * half;
-  };
-  V v;
-  Eight<T> next[V::S];
-  const T* p = part(block);
-  V::fetch(p, g.K, 0, half, over, v.a);
-  for (; block < blocks; block += stride) {
-    asm volatile("" ::: "memory");                            // the bias is loaded for each block, not held in 16 TN registers
-    v.begin(g, 0, half);
-    for (int kt = 0; kt < ktiles; ++kt) {
-      if (kt + 1 < ktiles) {
-        V::fetch(p, g.K, kt + 1, half, over, next);
-      } else if (block + stride < blocks) {
-        p = part(block + stride);
-        V::fetch(p, g.K, 0, half, over, next);
-      }
-      v.multiply(lds + kt * V::STAGE + ((lane >> 5) * V::BN + (lane & 31)) * 16);
-#pragma unroll
-      for (int s = 0; s < V::S; ++s) v.a[s] = next[s];
-    }
-    v.finish(g, block * 32 + (lane & 31), 0, half);
-  }
+  each<0, R>([&](auto r) __attribute__((always_inline)) { v[r].finish(g, row + 32 * r, nt * V::BN, half); });
 }
 
 // Columns a wave takes: all of a narrow output, else 256.
@@ -942,6 +918,13 @@ inline bool rows_fit(const Gemm& g) {
   return g.a_along && g.K > 0 && groups >= 512 && groups < (1 << 28);
 }
 
+// A wave of 16-bit values takes R = 2 row blocks against each chunk of W it reads: with one, a matrix instruction's 32 cycles
+// take one 16-byte read a lane from LDS, which four such waves just saturate. That needs two workgroups for each compute unit
+// (8192 x 4096 x 1024, one each: 106 us against 95 with R = 1) and a contraction long enough to hide the second block's
+// epilogue. bf16, R = 1 against R = 2: 65536 x 1024 x 512 104, 87 us; 16384 x 1024 x 1024 59, 48; 8192 x 1024 x 4096 118, 103;
+// 2449029 x 256 x 256 775, 715, but with a residual and saved bits 1128, 1171; 232965 x 41 x 256 38, 41. fp32 has 6 products
+// to a chunk's three reads and stays at R = 1. (Keeping all of a narrow W in LDS and walking over the rows was slower:
+// 131072 x 256 x 128 bf16 30 us, this 22.)
 template <typename T, int TN>
 int rows_launch(const Gemm& g, char* image) {
   constexpr int BN = TN * 32, BK = Rows<T>::BK, CH = BK / 8, STAGE = Unit<T>::PLANES * CH * BN * 16;
@@ -951,16 +934,13 @@ int rows_launch(const Gemm& g, char* image) {
   hipLaunchKernelGGL((lay_out_kernel<T, BN>), dim3((uint32_t)((chunks + 255) / 256)), dim3(256), 0, g.stream, l);
   DGNN_LAUNCHED();
   const int64_t blocks = (g.M + 31) / 32;
-  if (ntiles == 1 && ktiles * STAGE <= 128 * 1024) {
-    constexpr int WAVES = 8;
-    const int64_t per = ktiles * STAGE <= 64 * 1024 ? 2 : 1;          // workgroups a compute unit
-    const int64_t want = (blocks + WAVES - 1) / WAVES, most = 256 * per;
-    hipLaunchKernelGGL((rows_resident_kernel<T, TN, WAVES>), dim3((uint32_t)(want < most ? want : most)), dim3(WAVES * 64), (uint32_t)(ktiles * STAGE),
-                       g.stream, g, image, (int)ktiles);
+  constexpr int WAVES = 4;
+  const int64_t groups = (blocks + WAVES - 1) / WAVES, pairs = (groups + 1) / 2;
+  if (sizeof(T) == 2 && TN == 4 && pairs * ntiles >= 512 && (g.K >= 512 || (g.K >= 128 && !g.residual && !g.save))) {
+    if constexpr (sizeof(T) == 2 && TN == 4)
+      hipLaunchKernelGGL((rows_kernel<T, TN, WAVES, 2>), dim3((uint32_t)((pairs + 7) / 8 * 8 * ntiles)), dim3(WAVES * 64), 0, g.stream, g, image, (int)ktiles);
   } else {
-    constexpr int WAVES = 4;
-    hipLaunchKernelGGL((rows_kernel<T, TN, WAVES>), dim3((uint32_t)(((blocks + WAVES - 1) / WAVES + 7) / 8 * 8 * ntiles)), dim3(WAVES * 64), 0,
-                       g.stream, g, image, (int)ktiles);
+    hipLaunchKernelGGL((rows_kernel<T, TN, WAVES, 1>), dim3((uint32_t)((groups + 7) / 8 * 8 * ntiles)), dim3(WAVES * 64), 0, g.stream, g, image, (int)ktiles);
   }
   DGNN_LAUNCHED();
   return DGNN_OK;

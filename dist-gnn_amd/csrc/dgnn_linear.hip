@@ -58,10 +58,10 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope g) {
         const int64_t row = row0 + k * groups;
         const bool in = row < last;
         const T* dy = (const T*)g.dy + row * g.ld_dy + col;
-        if (in && have == 4) {
+        if (in && (have == 4 || (g.M - 1 - row) * g.ld_dy + g.N >= col + 4)) {             // what a load runs over is the next row
           const quad q = *reinterpret_cast<const quad*>(dy);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[k][i] = (float)q[i];
+          for (int i = 0; i < 4; ++i) v[k][i] = i < have ? (float)q[i] : 0.f;
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[k][i] = in && i < have ? (float)dy[i] : 0.f;
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope g) {
         if (g.act == ACT_RELU) word[k] = in ? ((const uint32_t*)g.save)[row * g.ld_save + col / 32] >> (col & 31) : 0;
         else if (g.act != ACT_NONE) {
           const float* at = (const float*)g.save + row * g.ld_save + col;
-          if (in && have == 4) {
+          if (in && (have == 4 || (g.M - 1 - row) * g.ld_save + g.N >= col + 4)) {
             const wide q = *reinterpret_cast<const wide*>(at);
 #pragma unroll
             for (int i = 0; i < 4; ++i) pre[k][i] = q[i];
@@ -122,18 +122,18 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope g) {
   }
 }
 
-// sums of the slabs' columns: 16 columns a block, 16 lanes each take every 16th slab, added in their order
+// sums of the slabs' columns: 8 columns a block, 32 lanes each take every 32nd slab, added in their order
 template <typename T>
 __global__ __launch_bounds__(256) void slab_join_kernel(const double* __restrict__ partial, int64_t slabs, int64_t N, T* __restrict__ out) {
-  __shared__ double sums[16][17];
-  const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
-  const int64_t col = (int64_t)blockIdx.x * 16 + c;
+  __shared__ double sums[32][9];
+  const int c = threadIdx.x & 7, k = threadIdx.x >> 3;
+  const int64_t col = (int64_t)blockIdx.x * 8 + c;
   double t = 0.0;
   if (col < N) {
-    for (int64_t s = k; s < slabs; s += 128) {               // 8 loads in flight, added in their order
+    for (int64_t s = k; s < slabs; s += 256) {               // 8 loads in flight, added in their order
       double v[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = s + 16 * u < slabs ? partial[(s + 16 * u) * N + col] : 0.0;
+      for (int u = 0; u < 8; ++u) v[u] = s + 32 * u < slabs ? partial[(s + 32 * u) * N + col] : 0.0;
 #pragma unroll
       for (int u = 0; u < 8; ++u) t += v[u];
     }
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) void slab_join_kernel(const double* __restrict
   sums[k][c] = t;
   __syncthreads();
   if (k == 0 && col < N) {
-    for (int i = 1; i < 16; ++i) t += sums[i][c];
+    for (int i = 1; i < 32; ++i) t += sums[i][c];
     out[col] = (T)(float)t;
   }
 }
@@ -367,7 +367,7 @@ int dgnn_linear_slope(const void* dy, int64_t ldd, const void* save, int64_t lds
     DGNN_LAUNCHED();
   }
   if (dbias) {
-    const dim3 grid((uint32_t)ceil_div(N, 16));
+    const dim3 grid((uint32_t)ceil_div(N, 8));
     if (dtype == DGNN_F32) hipLaunchKernelGGL((slab_join_kernel<float>), grid, dim3(256), 0, s, (const double*)workspace, slabs, N, (float*)dbias);
     else if (dtype == DGNN_BF16) hipLaunchKernelGGL((slab_join_kernel<__bf16>), grid, dim3(256), 0, s, (const double*)workspace, slabs, N, (__bf16*)dbias);
     else hipLaunchKernelGGL((slab_join_kernel<_Float16>), grid, dim3(256), 0, s, (const double*)workspace, slabs, N, (_Float16*)dbias);
