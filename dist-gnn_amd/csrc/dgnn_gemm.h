@@ -908,14 +908,18 @@ __global__ __launch_bounds__(WAVES * 64, R == 2 ? 2 : 3) void rows_kernel(const 
 // Columns a wave takes: all of a narrow output, else 256.
 inline int rows_bn(int64_t N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }
 
-// Bytes of W's image, and whether this product runs on rows_kernel: from 1024 rows up, where laying W out is paid back.
+// Bytes of W's image.
 template <typename T> int64_t rows_image(const Gemm& g) {
   const int64_t bn = rows_bn(g.N), bk = Rows<T>::BK;
   return ((g.N + bn - 1) / bn) * bn * ((g.K + bk - 1) / bk) * bk * Unit<T>::PLANES * 2;
 }
+// Whether a product runs on rows_kernel: with two workgroups of 128 rows for each compute unit, or where the contraction is so
+// short that cutting it into slices would not pay for what that costs. rows_kernel against tiles: bf16 4096 x 1024 x 1024
+// 25.6, 29.6 us; 8192 x 256 x 256 9.7, 19.9; 2048 x 1024 x 1024 23.7, 24.2; fp32 2048 x 256 x 256 16.1, 21.8; 65536 x 64 x 16
+// 8.0, 9.4; but 16384 x 1433 x 16 46.9, 37.5, and bf16 1024 x 4096 x 4096 85.0, 58.2.
 inline bool rows_fit(const Gemm& g) {
   const int64_t bn = rows_bn(g.N), groups = (g.M + 127) / 128 * ((g.N + bn - 1) / bn);
-  return g.a_along && g.K > 0 && groups >= 512 && groups < (1 << 28);
+  return g.a_along && g.K > 0 && (groups >= 512 || (groups >= 32 && g.K <= 8 * groups)) && groups < (1 << 28);
 }
 
 // A wave of 16-bit values takes R = 2 row blocks against each chunk of W it reads: with one, a matrix instruction's 32 cycles
@@ -1118,12 +1122,15 @@ __global__ __launch_bounds__(256, 3) void columns_kernel(const Gemm g) {
   });
 }
 
-// From 16384 rows up, while a lane's distance from its row fits 32 bits.
-template <typename T> bool columns_fit(const Gemm& g) {
-  return sizeof(T) == 4 && !g.a_along && g.K >= 16384 && (8 * g.lda + g.M) * 4 <= 0xffffffffLL && 32 * g.ldb * 4 <= 0xffffffffLL;
-}
-
 inline int64_t columns_tiles(const Gemm& g) { return ((g.M + 127) / 128) * ((g.N + rows_bn(g.N) - 1) / rows_bn(g.N)); }
+
+// From 65536 rows up, 16384 where the output is large enough, while a lane's distance from its row fits 32 bits. Against tiles
+// (x^T p of 256 x 256): 32768 rows 64.4, 57.5 us, 65536 85.6, 103.6, 232965 239, 325; 1024 x 1024 from 16384 rows 240, 323;
+// 1024 x 4096 from 8192 459, 398.
+template <typename T> bool columns_fit(const Gemm& g) {
+  return sizeof(T) == 4 && !g.a_along && (g.K >= 65536 || (g.K >= 16384 && columns_tiles(g) >= 16))
+      && (8 * g.lda + g.M) * 4 <= 0xffffffffLL && 32 * g.ldb * 4 <= 0xffffffffLL;
+}
 
 // Slices for 3 workgroups a compute unit, as many for each XCD, 256 rows at least, and no more partial sums than a quarter
 // of what the operands weigh.
@@ -1307,14 +1314,20 @@ __global__ __launch_bounds__(256) void thin_along_kernel(const Gemm g) {
         thin_out<T>(g, m, col + c, g.bias ? acc[m][c] + (float)((const T*)g.bias)[col + c] : acc[m][c]);
 }
 
-inline bool thin_fit(const Gemm& g) { return g.a_along && g.M <= 8; }
+// fp32: up to 4 rows, 8 where W keeps the contraction contiguous; 16 bits: up to 2, because a tile's matrix instructions take
+// 32 rows as fast as one and 16-bit values as they come. These kernels against tiles: fp32 602 x 256 with 1, 4, 6 rows 4.6,
+// 8.8, 11.6 against 10.9 us, W^T with 6 rows 5.3 against 9.9; bf16 4096 x 4096 with 1, 2, 3, 6 rows 9.5, 10.3, 11.7, 15.7
+// against 11.4, 11.7, 11.9, 12.3, W^T with 2, 3 rows 9.7, 12.6 against 10.7.
+template <typename T> bool thin_fit(const Gemm& g) { return g.a_along && g.M <= (sizeof(T) == 2 ? 2 : g.b_along ? 8 : 4); }
 
-// Slices of W's rows: one while W is so small that the launch is what it costs; else as many as give 256 workgroups, which
-// then read 1 KiB of a row at a time (16-byte columns of a long matrix all lie in a few of the memory's channels).
+// Slices of W's rows: one while W times the rows is so small that the launch is what it costs (one row: fp32 1024 x 1024 5.0 us,
+// cut 7.3; 2048 x 2048 6.6, cut 7.7); else as many as give 256 workgroups, which then read 1 KiB of a row at a time (16-byte
+// columns of a long matrix all lie in a few of the memory's channels: one row, bf16 4096 x 4096 12.4 us, cut 9.5; four rows,
+// fp32 1024 x 2048 10.0, cut 8.4).
 template <typename T> void thin_cut(Gemm& g) {
   g.slices = 1;
   g.slice_k = g.K > 0 ? g.K : 1;
-  if (g.b_along || g.K * g.N * (int64_t)sizeof(T) <= (4 << 20)) return;
+  if (g.b_along || g.M * g.K * g.N * (int64_t)sizeof(T) <= (16 << 20)) return;
   const int64_t blocks = (g.N + 64 * Unit<T>::W - 1) / (64 * Unit<T>::W);
   int64_t want = 256 / (blocks < 256 ? blocks : 256);
   const int64_t most = (g.K + 31) / 32;
@@ -1324,11 +1337,18 @@ template <typename T> void thin_cut(Gemm& g) {
 }
 
 template <typename T, int ROWS>
+int thin_along_launch(const Gemm& g) {
+  if (g.N >= 4096) hipLaunchKernelGGL((thin_along_kernel<T, ROWS, 4>), dim3((uint32_t)((g.N + 15) / 16)), dim3(256), 0, g.stream, g);
+  else hipLaunchKernelGGL((thin_along_kernel<T, ROWS, 1>), dim3((uint32_t)((g.N + 3) / 4)), dim3(256), 0, g.stream, g);
+  DGNN_LAUNCHED();
+  return DGNN_OK;
+}
+
+template <typename T, int ROWS>
 int thin_launch(const Gemm& g) {
   constexpr int W = Unit<T>::W;
   if (g.b_along) {
-    if (g.N >= 4096) hipLaunchKernelGGL((thin_along_kernel<T, ROWS, 4>), dim3((uint32_t)((g.N + 15) / 16)), dim3(256), 0, g.stream, g);
-    else hipLaunchKernelGGL((thin_along_kernel<T, ROWS, 1>), dim3((uint32_t)((g.N + 3) / 4)), dim3(256), 0, g.stream, g);
+    return thin_along_launch<T, ROWS>(g);
   } else {
     const int64_t cols = (g.N + 31) / 32 * 32;
     if (g.slices == 1) {
@@ -1349,14 +1369,16 @@ int thin_launch(const Gemm& g) {
 
 struct Shape { int bm, bn; };
 
-// Tile by the sides of the output: the narrowest that covers it once, else 128 x 256 (the operand with fewer bytes a
-// multiply-add to move; 8 waves of 64 x 64).
-inline Shape shape_of(const Gemm& g) {
+// Tile by the sides of the output: the narrowest that covers it once (against the widest: 16 x 4096 x 4096 bf16 13.9, 18.0 us;
+// 2708 x 1433 x 16 fp32 13.4, 15.4; 16384 x 602 x 64 fp32 26.7, 35.9), else 128 x 256 on 8 waves of 64 x 64. 16-bit products whose
+// operands both have to be turned in registers do better with two smaller workgroups a compute unit, one turning while the
+// other multiplies (4096^3 bf16 202 us, 128 x 256 215; fp32, which multiplies six times as long, 1024^3 39.1, 128 x 256 34.6).
+template <typename T> Shape shape_of(const Gemm& g) {
   const int64_t M = g.M, N = g.N;
   if (M <= 32) return {32, 128};
   if (N <= 32) return {128, 32};
   if (N <= 64) return {128, 64};
-  if (N <= 128 || (!g.a_along && g.K >= 16384)) return {128, 128};
+  if (N <= 128 || (sizeof(T) == 2 && !g.a_along)) return {128, 128};
   return {128, 256};
 }
 
@@ -1367,7 +1389,7 @@ inline int64_t tiles_of(Shape s, int64_t M, int64_t N) { return ((M + s.bm - 1) 
 
 template <typename T, bool AA, bool BA>
 int gemm_launch(const Gemm& g) {
-  const Shape s = shape_of(g);
+  const Shape s = shape_of<T>(g);
   const int64_t tiles = tiles_of(s, g.M, g.N);
   if (tiles > 0x7fffffffLL) return dgnn_fail(DGNN_E_BADARG, "linear: too many tiles%s (%lld)", "", tiles);
   const dim3 grid((uint32_t)tiles, (uint32_t)g.slices);
@@ -1388,13 +1410,12 @@ int gemm_launch(const Gemm& g) {
 
 template <typename T>
 int gemm_typed(const Gemm& g) {
-  if (thin_fit(g)) {
-    switch (g.M) {
-      case 1: return thin_launch<T, 1>(g);
-      case 2: return thin_launch<T, 2>(g);
-      case 3: case 4: return thin_launch<T, 4>(g);
-      case 5: case 6: return thin_launch<T, 6>(g);
-      default: return thin_launch<T, 8>(g);
+  if (thin_fit<T>(g)) {
+    if (g.M == 1) return thin_launch<T, 1>(g);
+    if (g.M == 2) return thin_launch<T, 2>(g);
+    if constexpr (sizeof(T) == 4) {
+      if (g.M <= 4) return thin_launch<T, 4>(g);
+      return thin_along_launch<T, 8>(g);
     }
   }
   if (g.image) {

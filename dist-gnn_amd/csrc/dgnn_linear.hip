@@ -203,7 +203,11 @@ __global__ __launch_bounds__(256) void small_backward_kernel(const Small g) {
     small_sums<double>(N, M, [&](int n, int m, double t) { return t + p[m * N + n]; }, [&](int n, double t) { ((T*)g.db)[n] = (T)(float)t; });
 }
 
-bool small_fit(int64_t M, int64_t K, int64_t N) { return M > 0 && N > 0 && K > 0 && M <= kSmall && N <= kSmall && M * N <= kSmall; }
+// M N is what p takes of LDS; K N / 4096 workgroups each compute it, so that a large W is left to the launches of its own
+// (8 x 4096 x 512 fp32 51 us, both host-bound, with separate launches 62; 1 x 4096 x 4096 bf16 125 us, with separate launches 62).
+bool small_fit(int64_t M, int64_t K, int64_t N) {
+  return M > 0 && N > 0 && K > 0 && M <= kSmall && N <= kSmall && M * N <= kSmall && K * N <= (1 << 22);
+}
 
 // ---------------------------------------------------------------------------------------
 constexpr int64_t kCompute = 256;              // compute units
@@ -212,8 +216,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // A product whose output tiles do not fill the compute units is cut along its contraction, at 128 elements a slice or more:
 // for one workgroup a unit in any case, for as many as fit while the partial sums weigh less than half the operands.
-void cut(Gemm& g) {
-  const Shape shape = shape_of(g);
+void cut(Gemm& g, int32_t dtype) {
+  const Shape shape = dtype == DGNN_F32 ? shape_of<float>(g) : shape_of<_Float16>(g);
   const int64_t tiles = tiles_of(shape, g.M, g.N), one = kCompute / (tiles > 0 ? tiles : 1);
   const int64_t most = ceil_div(g.K, 128), light = g.M > 0 && g.N > 0 ? g.K * (g.M + g.N) / (4 * g.M * g.N) : 1;
   int64_t want = one > light ? one : light < one * resident_of(shape) ? light : one * resident_of(shape);
@@ -261,7 +265,7 @@ bool apart(const void* a, int64_t lda, int64_t ra, int64_t ca, const void* b, in
 // How a product runs, by its sizes: a handful of rows on plain multiply-adds, over W's laid-out image where there are many rows, else by tiles, cut along the
 // contraction where those are few. Returns the bytes of workspace that takes.
 int64_t plan(Gemm& g, int32_t dtype) {
-  if (thin_fit(g)) {
+  if (dtype == DGNN_F32 ? thin_fit<float>(g) : thin_fit<_Float16>(g)) {
     if (dtype == DGNN_F32) thin_cut<float>(g); else thin_cut<_Float16>(g);
     return g.slices > 1 ? (int64_t)g.slices * g.M * g.N * 4 : 0;
   }
@@ -273,7 +277,7 @@ int64_t plan(Gemm& g, int32_t dtype) {
     g.slices = 1;
     return dtype == DGNN_F32 ? rows_image<float>(g) : rows_image<_Float16>(g);
   }
-  cut(g);
+  cut(g, dtype);
   return g.slices > 1 ? (int64_t)g.slices * g.M * g.N * 4 : 0;
 }
 
