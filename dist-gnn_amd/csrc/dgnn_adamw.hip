@@ -39,6 +39,7 @@ struct Entry {
 
 struct Table {
   int32_t count;
+  uint32_t chunks;                 // of all tensors
   uint32_t first[kTable];          // first chunk of each tensor
   Entry t[kTable];
 };
@@ -109,7 +110,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(const Table tab, const State
   using V4 = typename Quad<T>::V;
   constexpr int EACH = each(BITS8, MASTER), LANES = kBlock / EACH;                          // elements of a lane, lanes of a block
   int lo = 0, hi = tab.count - 1;
-  const uint32_t chunk = blockIdx.x;
+  const uint32_t chunk = blockIdx.y * gridDim.x + blockIdx.x;
+  if (chunk >= tab.chunks) return;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (tab.first[mid] <= chunk) lo = mid; else hi = mid - 1;
@@ -301,8 +303,9 @@ __global__ __launch_bounds__(64) void adamw_tick_kernel(const Table tab, int64_t
 }
 
 template <typename T>
-void launch(const Table& tab, uint32_t chunks, const State& st, bool master, bool bits8, hipStream_t s) {
-  const dim3 g(chunks), b(256);
+void launch(const Table& tab, const State& st, bool master, bool bits8, hipStream_t s) {
+  constexpr uint32_t row = 1 << 23;                      // a grid holds fewer than 2^32 lanes along a side
+  const dim3 g(tab.chunks < row ? tab.chunks : row, (tab.chunks + row - 1) / row), b(256);
   if (bits8) {
     if (master) hipLaunchKernelGGL((adamw_kernel<T, true, true>), g, b, 0, s, tab, st);
     else hipLaunchKernelGGL((adamw_kernel<T, false, true>), g, b, 0, s, tab, st);
@@ -347,6 +350,7 @@ extern "C" int dgnn_adamw(const struct dgnn_adamw_tensor* tensors, int32_t count
   for (int32_t i = 0; i < count;) {
     Table tab;
     tab.count = 0;
+    tab.chunks = 0;
     int64_t chunks = 0;
     while (i < count && tab.count < kTable) {
       const struct dgnn_adamw_tensor& t = tensors[i];
@@ -365,9 +369,10 @@ extern "C" int dgnn_adamw(const struct dgnn_adamw_tensor* tensors, int32_t count
       DGNN_LAUNCHED();
     }
     if (chunks == 0) continue;
-    if (dtype == DGNN_F32) launch<float>(tab, (uint32_t)chunks, st, state->master != nullptr, state_bits == 8, s);
-    else if (dtype == DGNN_BF16) launch<__bf16>(tab, (uint32_t)chunks, st, state->master != nullptr, state_bits == 8, s);
-    else launch<_Float16>(tab, (uint32_t)chunks, st, state->master != nullptr, state_bits == 8, s);
+    tab.chunks = (uint32_t)chunks;
+    if (dtype == DGNN_F32) launch<float>(tab, st, state->master != nullptr, state_bits == 8, s);
+    else if (dtype == DGNN_BF16) launch<__bf16>(tab, st, state->master != nullptr, state_bits == 8, s);
+    else launch<_Float16>(tab, st, state->master != nullptr, state_bits == 8, s);
     DGNN_LAUNCHED();
   }
   return DGNN_OK;

@@ -386,6 +386,11 @@ __device__ __forceinline__ void epilogue(const Gemm& g, f16v (&acc)[TM][TN], flo
   }
 }
 
+// The product by tiles: while a stage is multiplied from one LDS buffer, the next one is on its way to registers and is then
+// written to the other. For weight gradients, for outputs too small for rows_kernel and for what is cut into slices. Bound by
+// LDS: a wave's 64 x 64 take a 16-byte read for each matrix instruction, and turned operands are written there 16 bytes a lane.
+// bf16 8192 x 1024 x 4096 (x^T p) 117 us, 590 TFLOP/s, where a large library product reaches 1138; fp32 232965 x 256 x 256 222 us,
+// 137 TFLOP/s (library 153); 2708 x 1433 x 16 fp32 13 us, which is latency: 22 row tiles, 12 slices, a join.
 template <typename T, bool AA, bool BA, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm g) {
   constexpr int THREADS = WM * WN * 64, BK = Unit<T>::BK, PL = Unit<T>::PLANES;
@@ -844,6 +849,9 @@ template <typename T, int TN> struct Wave {
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
+// fp32 232965 x 602 x 256 403 us, 178 TFLOP/s of fp32 products (1070 of bf16 ones), bound by the matrix cores; bf16 65536 x 1024 x
+// 512 87 us, 790 TFLOP/s, 8192 x 1024 x 4096 103, 665, bound by LDS reads and the barrier of each stage; 2449029 x 256 x 256 with
+// a residual 1073 us, 3.5 TB/s: its rows are written in 32-byte pieces.
 // W's stages go round two buffers in LDS, copied there by the memory unit itself while the stage before is multiplied; each
 // buffer is an array of its own, so that the compiler sees that a copy into one does not touch the reads of the other.
 template <typename T, int TN, int WAVES, int R>
@@ -919,7 +927,8 @@ template <typename T> int64_t rows_image(const Gemm& g) {
 // 8.0, 9.4; but 16384 x 1433 x 16 46.9, 37.5, and bf16 1024 x 4096 x 4096 85.0, 58.2.
 inline bool rows_fit(const Gemm& g) {
   const int64_t bn = rows_bn(g.N), groups = (g.M + 127) / 128 * ((g.N + bn - 1) / bn);
-  return g.a_along && g.K > 0 && (groups >= 512 || (groups >= 32 && g.K <= 8 * groups)) && groups < (1 << 28);
+  return g.a_along && g.K > 0 && (groups >= 512 || (groups >= 32 && g.K <= 8 * groups)) && groups < (1 << 23)
+      && g.K * g.N < (1LL << 34);                                      // launches stay below 2^32 lanes
 }
 
 // A wave of 16-bit values takes R = 2 row blocks against each chunk of W it reads: with one, a matrix instruction's 32 cycles
@@ -954,7 +963,8 @@ int rows_launch(const Gemm& g, char* image) {
 // x^T p of fp32 matrices, the weight gradient over many rows: both operands keep the contraction across rows, and it is long
 // (every node) while the output is small. A wave owns 32 columns of x and all the workgroup's columns of p; x goes from memory
 // straight to the lanes (8 rows' values of a column each), p is turned and split once a workgroup on its way to LDS. The rows
-// are cut into slices for 3 workgroups a compute unit, the tiles of a slice stay on one XCD, and a join adds the slices.
+// are cut into slices for 3 workgroups a compute unit, the tiles of a slice stay on one XCD, and a join adds the slices. Bound by
+// x's and p's bytes: 232965 x 256 x 41 86 us with its join, 277 MB, 3.2 TB/s.
 // (16-bit values would come 2 or 4 bytes a load here; the tiles of gemm_kernel load 16, which is worth more.)
 // ---------------------------------------------------------------------------------------
 template <int BN> struct Turn {                               // BN columns of 32 rows by 256 lanes: 8 rows of 2 columns a lane
@@ -1122,15 +1132,14 @@ __global__ __launch_bounds__(256, 3) void columns_kernel(const Gemm g) {
   });
 }
 
-inline int64_t columns_tiles(const Gemm& g) { return ((g.M + 127) / 128) * ((g.N + rows_bn(g.N) - 1) / rows_bn(g.N)); }
-
-// From 65536 rows up, 16384 where the output is large enough, while a lane's distance from its row fits 32 bits. Against tiles
-// (x^T p of 256 x 256): 32768 rows 64.4, 57.5 us, 65536 85.6, 103.6, 232965 239, 325; 1024 x 1024 from 16384 rows 240, 323;
-// 1024 x 4096 from 8192 459, 398.
+// From 65536 rows up for outputs of one column tile, while a lane's distance from its row fits 32 bits. Against tiles: x^T p of
+// 256 x 41 from 65536 rows 39.4, 47.4 us; 64 x 64 from 262144 57.8, 70.5. Wider outputs share the turned x among 256 columns
+// there: 256 x 256 from 65536 79.2, 70.7; 602 x 256 from 232965 521, 511.
 template <typename T> bool columns_fit(const Gemm& g) {
-  return sizeof(T) == 4 && !g.a_along && (g.K >= 65536 || (g.K >= 16384 && columns_tiles(g) >= 16))
-      && (8 * g.lda + g.M) * 4 <= 0xffffffffLL && 32 * g.ldb * 4 <= 0xffffffffLL;
+  return sizeof(T) == 4 && !g.a_along && g.K >= 65536 && g.N <= 128 && (8 * g.lda + g.M) * 4 <= 0xffffffffLL && 32 * g.ldb * 4 <= 0xffffffffLL;
 }
+
+inline int64_t columns_tiles(const Gemm& g) { return (g.M + 127) / 128; }
 
 // Slices for 3 workgroups a compute unit, as many for each XCD, 256 rows at least, and no more partial sums than a quarter
 // of what the operands weigh.
@@ -1147,7 +1156,6 @@ inline void columns_cut(Gemm& g) {
 
 inline int columns_launch(const Gemm& g) {
   const int64_t blocks = (g.slices >= 8 ? ((int64_t)g.slices + 7) / 8 * 8 : g.slices) * columns_tiles(g);
-  if (blocks > 0x7fffffffLL) return dgnn_fail(DGNN_E_BADARG, "linear_grad_weight: too many tiles%s");
   const dim3 grid((uint32_t)blocks);
   switch (rows_bn(g.N)) {
     case 32: hipLaunchKernelGGL((columns_kernel<1>), grid, dim3(256), 0, g.stream, g); break;
@@ -1163,12 +1171,13 @@ inline int columns_launch(const Gemm& g) {
 }
 
 // ---------------------------------------------------------------------------------------
-// A handful of rows (1..8): W's bytes are all there is, each is used once a row, so plain fused multiply-adds in fp32 keep up
-// and no sum is split over workgroups -- one launch. thin_across: W[k][n] with n contiguous; LANES lanes take 16 bytes each
-// of a row of W, the others and the 16 waves further rows, all loads of a lane are on their way together, and the rows'
-// sums meet by exchanges in the wave and through LDS. LANES is as small as it takes to have a workgroup for every compute unit;
-// neighbouring column blocks, which share cache lines, run on one XCD. thin_along: W[n][k] with the contraction contiguous; a
-// wave takes COLS outputs and all lanes their contraction.
+// A handful of rows: W's bytes are all there is, each is used once a row, so plain fused multiply-adds in fp32 keep up, in one
+// launch while W is small. thin_across: W[k][n] with n contiguous; LANES lanes take 16 bytes each of a row of W, the others and
+// the 16 waves further rows, all loads of a lane are on their way together, and the rows' sums meet by exchanges in the wave and
+// through LDS. LANES is as small as it takes to have a workgroup for every compute unit; neighbouring column blocks, which share
+// cache lines, run on one XCD. thin_along: W[n][k] with the contraction contiguous; a wave takes COLS outputs (4 where there
+// are 4096 columns or more, so that a lane has 4 rows of W on their way) and all lanes their contraction.
+// One row: fp32 602 x 256 4.6 us, which is a launch and one trip to memory; bf16 4096 x 4096 9.4 us with its join, 3.6 TB/s.
 // ---------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ void thin_out(const Gemm& g, int64_t row, int64_t col, float t) {
   if (g.save && g.act > ACT_RELU) ((float*)g.save)[row * g.ld_save + col] = t;
@@ -1391,7 +1400,7 @@ template <typename T, bool AA, bool BA>
 int gemm_launch(const Gemm& g) {
   const Shape s = shape_of<T>(g);
   const int64_t tiles = tiles_of(s, g.M, g.N);
-  if (tiles > 0x7fffffffLL) return dgnn_fail(DGNN_E_BADARG, "linear: too many tiles%s (%lld)", "", tiles);
+  if (tiles >= (1 << 23)) return dgnn_fail(DGNN_E_BADARG, "linear: too many tiles%s (%lld)", "", tiles);
   const dim3 grid((uint32_t)tiles, (uint32_t)g.slices);
   switch (s.bm * 1000 + s.bn) {
     case 32128: hipLaunchKernelGGL((gemm_kernel<T, AA, BA, 32, 128, 1, 4>), grid, dim3(256), 0, g.stream, g); break;

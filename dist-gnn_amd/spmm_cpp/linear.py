@@ -40,8 +40,7 @@ def linear(x, weight, bias=None, activation='none', residual=None):
 
 def linear_forward(x, weight, bias=None, activation='none', residual=None, save=False):
     """(y, saved): y = act(x W + b) + r and, with ``save``, what ``linear_slope`` needs (None for 'none'): one bit per value
-    for relu (int32 [M, ceil(N / 32)]), x W + b itself, in fp32, for
-    gelu and silu."""
+    for relu (int32 [M, ceil(N / 32)]), x W + b itself, in fp32, for gelu and silu."""
     return _call(_ext.linear_forward, x, weight, bias, _code(activation), residual, save)
 
 

@@ -21,7 +21,8 @@ extern "C" {
  * The layer transform  y = act(x W + b) + r  and its gradients. All matrices row-major with `ld*` elements between rows
  * (>= the row's width) and element-aligned, of one type (DGNN_F32 | DGNN_BF16 | DGNN_F16): x [M x K], W [K x N], b [N] or
  * NULL, r [M x N] or NULL, y [M x N]. Products and sums in fp32 (fp32 operands: six products of bf16 pieces, as close to
- * the exact sum as a chain of fp32 operations), one rounding at the end. relu(NaN) is NaN.
+ * the exact sum as a chain of fp32 operations), one rounding at the end. relu(NaN) is NaN. M up to 2^31 - 1, K and N up to 2^24,
+ * outputs up to 2^23 tiles of 128 x 32 to 128 x 256 (by N); more is refused.
  *   act    DGNN_ACT_*: none, relu, gelu (0.5 t (1 + erf(t / sqrt 2))), silu (t / (1 + e^-t))
  *   save   NULL, or what dgnn_linear_slope needs: for relu uint32 [M][lds], bit n % 32 of word n / 32 set where x W + b is
  *          not <= 0 (lds >= ceil(N / 32), bits past N zero); for gelu and silu x W + b as float (lds >= N)
@@ -71,7 +72,7 @@ int dgnn_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
  *
  *   param, grad   device, numel elements of `dtype` (DGNN_F32 | DGNN_BF16 | DGNN_F16), element-aligned, contiguous
  *   start         first element of the tensor in the state buffers, a multiple of 256
- *   index         the tensor's entry of `steps` / `factors` (only read when they are given)
+ *   index         the tensor's entry of `steps` / `factors`, one for each tensor (only read when they are given)
  *   decay, rate, root, turn    the factors above and t mod 2^32 (unused when `steps` is given)
  *
  * State buffers (device, 16-byte aligned, shared by all tensors of the call):

@@ -397,3 +397,17 @@ def test_element_numbers_past_32_bits():
     del opt, p, q
     torch.cuda.empty_cache()
 
+
+
+def test_more_chunks_than_one_side_of_a_grid():
+    """2^33 elements are 2^23 workgroups and some, more than a grid takes along one side."""
+    if torch.cuda.mem_get_info()[0] < 120 << 30:
+        pytest.skip('needs 120 GB of device memory')
+    n = (1 << 33) + 5000
+    p = torch.nn.Parameter(torch.ones(n, device='cuda', dtype=torch.bfloat16))
+    opt = spmm_cpp.AdamW([p], lr=0.5, weight_decay=0.0, state_bits=8, master_weights=True)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert bool((p == 0.5).all())
+    del opt, p
+    torch.cuda.empty_cache()

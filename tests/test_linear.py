@@ -50,6 +50,15 @@ def test_c_entries_refuse(call, kw):
     assert call(**kw) == 1 and b'linear' in lib.dgnn_last_error()
 
 
+@pytest.mark.parametrize('call,kw', [
+    (_forward, dict(K=(1 << 24) + 1)), (_forward, dict(N=(1 << 24) + 1)), (_grad_weight, dict(K=(1 << 24) + 1)), (_slope, dict(N=(1 << 24) + 1)),
+    (_forward, dict(M=(1 << 31) - 1, y=1 << 44, w=1 << 50)), (_grad_input, dict(M=(1 << 31) - 1, dx=1 << 44, w=1 << 50)),          # 2^24 tiles
+    (_grad_weight, dict(M=64, K=1 << 24, N=1 << 15, ldx=1 << 24, ldp=1 << 15, ldw=1 << 15, dw=1 << 50)),
+])
+def test_c_entries_refuse_what_a_launch_cannot_hold(call, kw):
+    assert call(**kw) == 1 and b'linear' in lib.dgnn_last_error()
+
+
 def test_c_entries_with_nothing_to_do():
     assert _forward(M=0, x=None, y=None) == 0 and _forward(N=0, w=None, y=None) == 0 and _grad_input(M=0, p=None, dx=None) == 0
     assert _grad_weight(K=0, x=None, dw=None) == 0 and _slope(N=0, dy=None, save=None, p=None) == 0 and _slope(M=0, dy=None, save=None, p=None) == 0
