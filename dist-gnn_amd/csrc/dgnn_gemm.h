@@ -924,10 +924,12 @@ template <typename T> int64_t rows_image(const Gemm& g) {
 // Whether a product runs on rows_kernel: with two workgroups of 128 rows for each compute unit, or where the contraction is so
 // short that cutting it into slices would not pay for what that costs. rows_kernel against tiles: bf16 4096 x 1024 x 1024
 // 25.6, 29.6 us; 8192 x 256 x 256 9.7, 19.9; 2048 x 1024 x 1024 23.7, 24.2; fp32 2048 x 256 x 256 16.1, 21.8; 65536 x 64 x 16
-// 8.0, 9.4; but 16384 x 1433 x 16 46.9, 37.5, and bf16 1024 x 4096 x 4096 85.0, 58.2.
+// 8.0, 9.4; but 16384 x 1433 x 16 46.9, 37.5, and bf16 1024 x 4096 x 4096 85.0, 58.2. A contraction of one or two stages leaves little
+// to win and W's layout is a launch of its own: fp32 2708 x 16 x 1433 14.3, 11.0; 32768 x 64 x 128 12.4, 13.2; 60000 x 32 x 128
+// 14.5, 19.4.
 inline bool rows_fit(const Gemm& g) {
   const int64_t bn = rows_bn(g.N), groups = (g.M + 127) / 128 * ((g.N + bn - 1) / bn);
-  return g.a_along && g.K > 0 && (groups >= 512 || (groups >= 32 && g.K <= 8 * groups)) && groups < (1 << 23)
+  return g.a_along && g.K > 0 && (groups >= 512 || (groups >= (g.K > 64 ? 32 : 384) && g.K <= 8 * groups)) && groups < (1 << 23)
       && g.K * g.N < (1LL << 34);                                      // launches stay below 2^32 lanes
 }
 
@@ -1379,14 +1381,16 @@ int thin_launch(const Gemm& g) {
 struct Shape { int bm, bn; };
 
 // Tile by the sides of the output: the narrowest that covers it once (against the widest: 16 x 4096 x 4096 bf16 13.9, 18.0 us;
-// 2708 x 1433 x 16 fp32 13.4, 15.4; 16384 x 602 x 64 fp32 26.7, 35.9), else 128 x 256 on 8 waves of 64 x 64. 16-bit products whose
-// operands both have to be turned in registers do better with two smaller workgroups a compute unit, one turning while the
-// other multiplies (4096^3 bf16 202 us, 128 x 256 215; fp32, which multiplies six times as long, 1024^3 39.1, 128 x 256 34.6).
+// 2708 x 1433 x 16 fp32 13.4, 15.4; 16384 x 602 x 64 fp32 26.7, 35.9). 128 x 64 also where the contraction is one or two stages,
+// which need workgroups more than shared reads (2708 x 16 x 1433 fp32 11.0, 128 x 256 23). Else 128 x 256 on 8 waves of 64 x 64.
+// 16-bit products whose operands both have to be turned in registers do better with two smaller workgroups a compute unit, one
+// turning while the other multiplies (4096^3 bf16 202 us, 128 x 256 215; fp32, which multiplies six times as long, 1024^3 39.1,
+// 128 x 256 34.6).
 template <typename T> Shape shape_of(const Gemm& g) {
   const int64_t M = g.M, N = g.N;
   if (M <= 32) return {32, 128};
   if (N <= 32) return {128, 32};
-  if (N <= 64) return {128, 64};
+  if (N <= 64 || (g.a_along && g.K <= 64)) return {128, 64};
   if (N <= 128 || (sizeof(T) == 2 && !g.a_along)) return {128, 128};
   return {128, 256};
 }
