@@ -122,6 +122,29 @@ def test_output_and_gradients(m, k, n, dtype):
         assert torch.equal(spmm_cpp.linear(case[0], case[1], case[2], act, case[3]), mine['y'])      # saving nothing: the same bits
 
 
+@pytest.mark.parametrize('dtype', list(DT))
+@pytest.mark.parametrize('m,k,n', [(65600, 70, 41), (65500, 130, 250), (33000, 520, 500)])
+def test_output_and_gradients_of_many_rows(m, k, n, dtype):
+    """Rows enough for weight gradients straight from memory and for two row blocks a wave, every side ragged."""
+    for act, residual, pad in (('none', False, 0), ('gelu', True, 3)):
+        case = _inputs(m, k, n, dtype, True, residual, seed=m + n, pad=pad)
+        want = _definition(*case, dtype, act)
+        mine = _run(*case, act)
+        for name, got in mine.items():
+            _near(got, *want[name], f'{act} {name}')
+        assert torch.equal(spmm_cpp.linear(case[0], case[1], case[2], act, case[3]), mine['y'])
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+def test_a_handful_of_rows(dtype):
+    """1 to 9 rows against W as it lies and W^T, few and many columns: the crossover from multiply-adds to tiles on both sides."""
+    for m, (k, n) in itertools.product((1, 2, 3, 4, 5, 8, 9), ((70, 41), (602, 256), (130, 4100), (2100, 1030))):
+        case = _inputs(m, k, n, dtype, True, True, seed=m + n, pad=m % 2)
+        want = _definition(*case, dtype, 'silu')
+        for name, got in _run(*case, 'silu').items():
+            _near(got, *want[name], f'{m}x{k}x{n} {name}')
+
+
 @pytest.mark.parametrize('m,k,n', [(0, 5, 4), (3, 0, 4), (3, 5, 0), (0, 0, 0), (1, 0, 1)])
 def test_empty_sides(m, k, n):
     for dtype, act in itertools.product(DT, ('none', 'relu', 'silu')):
