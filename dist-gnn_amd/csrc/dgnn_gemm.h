@@ -1177,8 +1177,8 @@ inline int columns_launch(const Gemm& g) {
 // launch while W is small. thin_across: W[k][n] with n contiguous; LANES lanes take 16 bytes each of a row of W, the others and
 // the 16 waves further rows, all loads of a lane are on their way together, and the rows' sums meet by exchanges in the wave and
 // through LDS. LANES is as small as it takes to have a workgroup for every compute unit; neighbouring column blocks, which share
-// cache lines, run on one XCD. thin_along: W[n][k] with the contraction contiguous; a wave takes COLS outputs (4 where there
-// are 4096 columns or more, so that a lane has 4 rows of W on their way) and all lanes their contraction.
+// cache lines, run on one XCD. thin_along: W[n][k] with the contraction contiguous; a wave takes an output and all its lanes the
+// contraction (four outputs a wave: 1 x 4096 x 4096 bf16 7.9 us against 6.2).
 // One row: fp32 602 x 256 4.6 us, which is a launch and one trip to memory; bf16 4096 x 4096 9.4 us with its join, 3.6 TB/s.
 // ---------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ void thin_out(const Gemm& g, int64_t row, int64_t col, float t) {
@@ -1273,56 +1273,42 @@ __global__ __launch_bounds__(WAVES * 64) void thin_across_kernel(const Gemm g, i
   }
 }
 
-template <typename T, int ROWS, int COLS>
+template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void thin_along_kernel(const Gemm g) {
   constexpr int W = Unit<T>::W;
   const int lane = threadIdx.x & 63;
-  const int64_t col = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * COLS;
+  const int64_t col = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (col >= g.N) return;
-  const T* x = (const T*)g.a;
-  float acc[ROWS][COLS];
+  const T* const w = (const T*)g.b + col * g.ldb;
+  float acc[ROWS];
 #pragma unroll
-  for (int m = 0; m < ROWS; ++m)
-#pragma unroll
-    for (int c = 0; c < COLS; ++c) acc[m][c] = 0.f;
+  for (int m = 0; m < ROWS; ++m) acc[m] = 0.f;
   for (int64_t k = lane * W; k < g.K; k += 64 * W) {
     const int64_t left = g.K - k;
-    u4 v[COLS], s[ROWS];
-#pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-      const T* w = (const T*)g.b + (col + c < g.N ? col + c : g.N - 1) * g.ldb + k;
-      v[c] = left >= W ? load16(w) : load_some(w, left);
-    }
+    u4 s[ROWS];
+    const u4 v = left >= W ? load16(w + k) : load_some(w + k, left);
 #pragma unroll
     for (int m = 0; m < ROWS; ++m) {
-      const T* p = x + (m < g.M ? m : g.M - 1) * g.lda + k;
+      const T* p = (const T*)g.a + (m < g.M ? m : g.M - 1) * g.lda + k;
       s[m] = left >= W ? load16(p) : load_some(p, left);
     }
+    float f[W];
+    widen16<T>(v, f);
 #pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-      float f[W];
-      widen16<T>(v[c], f);
+    for (int m = 0; m < ROWS; ++m) {
+      float e[W];
+      widen16<T>(s[m], e);
 #pragma unroll
-      for (int m = 0; m < ROWS; ++m) {
-        float e[W];
-        widen16<T>(s[m], e);
-#pragma unroll
-        for (int i = 0; i < W; ++i) acc[m][c] = fmaf(e[i], f[i], acc[m][c]);
-      }
+      for (int i = 0; i < W; ++i) acc[m] = fmaf(e[i], f[i], acc[m]);
     }
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1)
 #pragma unroll
-    for (int m = 0; m < ROWS; ++m)
-#pragma unroll
-      for (int c = 0; c < COLS; ++c) acc[m][c] += __shfl_xor(acc[m][c], d);
+    for (int m = 0; m < ROWS; ++m) acc[m] += __shfl_xor(acc[m], d);
 #pragma unroll
   for (int m = 0; m < ROWS; ++m)
-#pragma unroll
-    for (int c = 0; c < COLS; ++c)
-      if (lane == m * COLS + c && m < g.M && col + c < g.N)
-        thin_out<T>(g, m, col + c, g.bias ? acc[m][c] + (float)((const T*)g.bias)[col + c] : acc[m][c]);
+    if (lane == m && m < g.M) thin_out<T>(g, m, col, g.bias ? acc[m] + (float)((const T*)g.bias)[col] : acc[m]);
 }
 
 // fp32: up to 4 rows, 8 where W keeps the contraction contiguous; 16 bits: up to 2, because a tile's matrix instructions take
@@ -1349,8 +1335,7 @@ template <typename T> void thin_cut(Gemm& g) {
 
 template <typename T, int ROWS>
 int thin_along_launch(const Gemm& g) {
-  if (g.N >= 4096) hipLaunchKernelGGL((thin_along_kernel<T, ROWS, 4>), dim3((uint32_t)((g.N + 15) / 16)), dim3(256), 0, g.stream, g);
-  else hipLaunchKernelGGL((thin_along_kernel<T, ROWS, 1>), dim3((uint32_t)((g.N + 3) / 4)), dim3(256), 0, g.stream, g);
+  hipLaunchKernelGGL((thin_along_kernel<T, ROWS>), dim3((uint32_t)((g.N + 3) / 4)), dim3(256), 0, g.stream, g);
   DGNN_LAUNCHED();
   return DGNN_OK;
 }
@@ -1411,7 +1396,9 @@ int gemm_launch(const Gemm& g) {
     case 128032: hipLaunchKernelGGL((gemm_kernel<T, AA, BA, 128, 32, 4, 1>), grid, dim3(256), 0, g.stream, g); break;
     case 128064: hipLaunchKernelGGL((gemm_kernel<T, AA, BA, 128, 64, 4, 1>), grid, dim3(256), 0, g.stream, g); break;
     case 128128: hipLaunchKernelGGL((gemm_kernel<T, AA, BA, 128, 128, 2, 2>), grid, dim3(256), 0, g.stream, g); break;
-    default: hipLaunchKernelGGL((gemm_kernel<T, AA, BA, 128, 256, 2, 4>), grid, dim3(512), 0, g.stream, g); break;
+    default:
+      if constexpr (AA || sizeof(T) == 4) hipLaunchKernelGGL((gemm_kernel<T, AA, BA, 128, 256, 2, 4>), grid, dim3(512), 0, g.stream, g);
+      break;
   }
   DGNN_LAUNCHED();
   if (g.slices > 1) {
