@@ -1313,8 +1313,8 @@ __global__ __launch_bounds__(256) void thin_along_kernel(const Gemm g) {
 
 // fp32: up to 4 rows, 8 where W keeps the contraction contiguous; 16 bits: up to 2, because a tile's matrix instructions take
 // 32 rows as fast as one and 16-bit values as they come. These kernels against tiles: fp32 602 x 256 with 1, 4, 6 rows 4.6,
-// 8.8, 11.6 against 10.9 us, W^T with 6 rows 5.3 against 9.9; bf16 4096 x 4096 with 1, 2, 3, 6 rows 9.5, 10.3, 11.7, 15.7
-// against 11.4, 11.7, 11.9, 12.3, W^T with 2, 3 rows 9.7, 12.6 against 10.7.
+// 8.8, 11.6 against 10.9 us, W^T with 6 rows 5.9 against 9.9; bf16 4096 x 4096 with 1, 2, 3, 6 rows 9.5, 10.3, 11.7, 15.7
+// against 11.4, 11.7, 11.9, 12.3, W^T with 1, 2 rows 6.2, 7.3 against 10.7.
 template <typename T> bool thin_fit(const Gemm& g) { return g.a_along && g.M <= (sizeof(T) == 2 ? 2 : g.b_along ? 8 : 4); }
 
 // Slices of W's rows: one while W times the rows is so small that the launch is what it costs (one row: fp32 1024 x 1024 5.0 us,

@@ -28,7 +28,8 @@ extern "C" {
  *          not <= 0 (lds >= ceil(N / 32), bits past N zero); for gelu and silu x W + b as float (lds >= N)
  * With a gradient dy of y:
  *   dgnn_linear_slope         p = dy act'(x W + b) (p may be NULL), dbias[n] = sum over m of p[m][n] (may be NULL); p may be
- *                             dy itself. act DGNN_ACT_NONE: p is a copy of dy
+ *                             dy itself. act DGNN_ACT_NONE: p is a copy of dy. p is rounded to its type; dbias is not made from
+ *                             the rounded values
  *   dgnn_linear_grad_input    dx = p W^T + add    (add [M x K] or NULL: what else reaches x, a skip connection's gradient)
  *   dgnn_linear_grad_weight   dw = x^T p      (M = 0: zeros)
  *   dgnn_linear_backward      all of them in one call, p in the workspace; dx, dw and dbias may be NULL (x, w and save are then
