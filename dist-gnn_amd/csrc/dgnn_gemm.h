@@ -1389,7 +1389,6 @@ template <typename T, bool AA, bool BA>
 int gemm_launch(const Gemm& g) {
   const Shape s = shape_of<T>(g);
   const int64_t tiles = tiles_of(s, g.M, g.N);
-  if (tiles >= (1 << 23)) return dgnn_fail(DGNN_E_BADARG, "linear: too many tiles%s (%lld)", "", tiles);
   const dim3 grid((uint32_t)tiles, (uint32_t)g.slices);
   switch (s.bm * 1000 + s.bn) {
     case 32128: hipLaunchKernelGGL((gemm_kernel<T, AA, BA, 32, 128, 1, 4>), grid, dim3(256), 0, g.stream, g); break;

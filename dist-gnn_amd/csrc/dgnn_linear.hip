@@ -4,6 +4,8 @@
 
 #include "dgnn_gemm.h"
 
+#include <initializer_list>
+
 namespace {
 
 using namespace dgnn;
@@ -259,11 +261,43 @@ bool matrix_ok(const void* p, int64_t ld, int64_t rows, int64_t cols, int64_t w)
   return p && ld >= cols && (uintptr_t)p % (uintptr_t)w == 0;
 }
 
-bool apart(const void* a, int64_t lda, int64_t ra, int64_t ca, const void* b, int64_t ldb, int64_t rb, int64_t cb, int64_t w) {
-  if (!a || !b || ra == 0 || ca == 0 || rb == 0 || cb == 0) return true;
-  const char* a0 = (const char*)a, *b0 = (const char*)b;
-  const char* a1 = a0 + ((ra - 1) * lda + ca) * w, *b1 = b0 + ((rb - 1) * ldb + cb) * w;
-  return a1 <= b0 || b1 <= a0;
+// Where a matrix lies: rows of `row` bytes `pitch` apart (0: there is one), from `at` to before `end` (at == end: nowhere).
+struct Place {
+  uintptr_t at, end;
+  int64_t pitch, row;
+};
+
+Place place(const void* p, int64_t ld, int64_t rows, int64_t cols, int64_t w) {
+  if (!p || rows == 0 || cols == 0) return {0, 0, 0, 0};
+  return {(uintptr_t)p, (uintptr_t)p + (uintptr_t)(((rows - 1) * ld + cols) * w), rows > 1 ? ld * w : 0, cols * w};
+}
+
+// no byte of one is a byte of the other; columns of one buffer, whose rows take turns, are apart
+bool apart(const Place& a, const Place& b) {
+  if (a.at == a.end || b.at == b.end || a.end <= b.at || b.end <= a.at) return true;
+  const int64_t pitch = a.pitch ? a.pitch : b.pitch;
+  if (pitch == 0 || (b.pitch && b.pitch != pitch)) return false;
+  const int64_t d = a.at <= b.at ? (int64_t)(b.at - a.at) % pitch : (pitch - (int64_t)(a.at - b.at) % pitch) % pitch;
+  return d >= a.row && d + b.row <= pitch;
+}
+
+// what a call writes is apart from what it reads and from what else it writes
+bool apart(std::initializer_list<Place> written, std::initializer_list<Place> read) {
+  for (const Place* a = written.begin(); a != written.end(); ++a) {
+    for (const Place& b : read)
+      if (!apart(*a, b)) return false;
+    for (const Place* b = a + 1; b != written.end(); ++b)
+      if (!apart(*a, *b)) return false;
+  }
+  return true;
+}
+
+// what the forward pass saved: relu's words, the others' floats
+Place saved(const void* save, int64_t lds, int64_t M, int64_t N, int32_t act) {
+  return place(act == ACT_NONE ? nullptr : save, lds, M, act == ACT_RELU ? (N + 31) / 32 : N, 4);
+}
+bool saved_ok(const void* save, int64_t lds, int64_t M, int64_t N, int32_t act) {
+  return act == ACT_NONE || matrix_ok(save, lds, M, act == ACT_RELU ? (N + 31) / 32 : N, 4);
 }
 
 // How a product runs, by its sizes: a handful of rows on plain multiply-adds, over W's laid-out image where there are many rows,
@@ -285,7 +319,14 @@ int64_t plan(Gemm& g, int32_t dtype) {
   return g.slices > 1 ? (int64_t)g.slices * g.M * g.N * 4 : 0;
 }
 
+// whether a grid holds the output's tiles, where the product runs by tiles
+template <typename T> bool tiles_fit(const Gemm& g) {
+  return thin_fit<T>(g) || columns_fit<T>(g) || rows_fit(g) || tiles_of(shape_of<T>(g), g.M, g.N) < (1 << 23);
+}
+bool launch_fits(const Gemm& g, int32_t dtype) { return dtype == DGNN_F32 ? tiles_fit<float>(g) : tiles_fit<_Float16>(g); }
+
 int run(const Gemm& g, int32_t dtype, void* workspace, int64_t bytes, const char* who) {
+  if (!launch_fits(g, dtype)) return dgnn_fail(DGNN_E_BADARG, "%s: too many tiles of output", who);
   Gemm h = g;
   const int64_t need = plan(h, dtype);
   if (need && (!workspace || bytes < need || (uintptr_t)workspace % 16))
@@ -331,12 +372,10 @@ int dgnn_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, 
   if (!matrix_ok(x, ldx, M, K, b) || !matrix_ok(w, ldw, K, N, b) || !matrix_ok(y, ldy, M, N, b) || (uintptr_t)bias % b
       || (residual && !matrix_ok(residual, ldr, M, N, b)))
     return dgnn_fail(DGNN_E_BADARG, "linear_forward: null, misaligned or overlapping rows%s");
-  if (save && act != ACT_NONE) {
-    const bool fits = act == ACT_RELU ? lds >= (N + 31) / 32 && (uintptr_t)save % 4 == 0 : lds >= N && (uintptr_t)save % 4 == 0;
-    if (!fits) return dgnn_fail(DGNN_E_BADARG, "linear_forward: save is too narrow or misaligned%s");
-  }
-  if (!apart(y, ldy, M, N, x, ldx, M, K, b) || !apart(y, ldy, M, N, w, ldw, K, N, b) || !apart(y, ldy, M, N, residual, ldr, M, N, b))
-    return dgnn_fail(DGNN_E_BADARG, "linear_forward: y overlaps an input%s");
+  if (save && !saved_ok(save, lds, M, N, act)) return dgnn_fail(DGNN_E_BADARG, "linear_forward: save is too narrow or misaligned%s");
+  if (!apart({place(y, ldy, M, N, b), saved(save, lds, M, N, act)},
+             {place(x, ldx, M, K, b), place(w, ldw, K, N, b), place(bias, N, 1, N, b), place(residual, ldr, M, N, b)}))
+    return dgnn_fail(DGNN_E_BADARG, "linear_forward: y or save overlaps another operand%s");
   Gemm g{};
   g.a = x; g.lda = ldx; g.a_along = true;
   g.b = w; g.ldb = ldw; g.b_along = false;
@@ -359,9 +398,11 @@ int dgnn_linear_slope(const void* dy, int64_t ldd, const void* save, int64_t lds
   hipStream_t s = (hipStream_t)stream;
   if ((uintptr_t)dbias % b) return dgnn_fail(DGNN_E_BADARG, "linear_slope: misaligned dbias%s");
   if (M > 0) {
-    if (!matrix_ok(dy, ldd, M, N, b) || (p && !matrix_ok(p, ldp, M, N, b)) || (act == ACT_RELU && (!save || lds < (N + 31) / 32 || (uintptr_t)save % 4))
-        || (act > ACT_RELU && !matrix_ok(save, lds, M, N, 4)))
+    if (!matrix_ok(dy, ldd, M, N, b) || (p && !matrix_ok(p, ldp, M, N, b)) || !saved_ok(save, lds, M, N, act))
       return dgnn_fail(DGNN_E_BADARG, "linear_slope: null, misaligned or overlapping rows%s");
+    const Place from = place(p == dy && ldp == ldd ? nullptr : dy, ldd, M, N, b);          // p may be dy itself
+    if (!apart({place(p, ldp, M, N, b), place(dbias, N, 1, N, b)}, {from, saved(save, lds, M, N, act)}))
+      return dgnn_fail(DGNN_E_BADARG, "linear_slope: p or dbias overlaps another operand%s");
   }
   const int64_t lanes = slope_lanes(N), slab = M > 0 ? slope_slab(M, N) : 1, slabs = ceil_div(M, slab);
   if (dbias && slabs > 0 && (!workspace || workspace_bytes < slabs * N * 8 || (uintptr_t)workspace % 8))
@@ -393,7 +434,7 @@ int dgnn_linear_grad_input(const void* p, int64_t ldp, const void* w, int64_t ld
   if (!matrix_ok(p, ldp, M, N, b) || !matrix_ok(w, ldw, K, N, b) || !matrix_ok(dx, ldx, M, K, b)
       || (add && !matrix_ok(add, lda, M, K, b)))
     return dgnn_fail(DGNN_E_BADARG, "linear_grad_input: null, misaligned or overlapping rows%s");
-  if (!apart(dx, ldx, M, K, p, ldp, M, N, b) || !apart(dx, ldx, M, K, w, ldw, K, N, b) || !apart(dx, ldx, M, K, add, lda, M, K, b))
+  if (!apart({place(dx, ldx, M, K, b)}, {place(p, ldp, M, N, b), place(w, ldw, K, N, b), place(add, lda, M, K, b)}))
     return dgnn_fail(DGNN_E_BADARG, "linear_grad_input: dx overlaps an input%s");
   Gemm g{};
   g.a = p; g.lda = ldp; g.a_along = true;
@@ -413,7 +454,7 @@ int dgnn_linear_grad_weight(const void* x, int64_t ldx, const void* p, int64_t l
   const int64_t b = width(dtype);
   if (!matrix_ok(x, ldx, M, K, b) || !matrix_ok(p, ldp, M, N, b) || !matrix_ok(dw, ldw, K, N, b))
     return dgnn_fail(DGNN_E_BADARG, "linear_grad_weight: null, misaligned or overlapping rows%s");
-  if (!apart(dw, ldw, K, N, x, ldx, M, K, b) || !apart(dw, ldw, K, N, p, ldp, M, N, b))
+  if (!apart({place(dw, ldw, K, N, b)}, {place(x, ldx, M, K, b), place(p, ldp, M, N, b)}))
     return dgnn_fail(DGNN_E_BADARG, "linear_grad_weight: dw overlaps an input%s");
   Gemm g{};
   g.a = x; g.lda = ldx; g.a_along = false;
@@ -458,15 +499,14 @@ int dgnn_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
   const int64_t need = backward_parts(M, K, N, dtype, act, &p_bytes);
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return dgnn_fail(DGNN_E_BADARG, "linear_backward: workspace too small or misaligned%s (%lld bytes wanted)", "", need);
+  const int64_t b = width(dtype);
+  if (!matrix_ok(dy, ldd, M, N, b) || (dw && (!matrix_ok(x, ldx, M, K, b) || !matrix_ok(dw, lddw, K, N, b)))
+      || (dx && (!matrix_ok(w, ldw, K, N, b) || !matrix_ok(dx, lddx, M, K, b))) || (uintptr_t)dbias % b || !saved_ok(save, lds, M, N, act))
+    return dgnn_fail(DGNN_E_BADARG, "linear_backward: null, misaligned or overlapping rows%s");
+  if (!apart({place(dx, lddx, M, K, b), place(dw, lddw, K, N, b), place(dbias, N, 1, N, b)},
+             {place(dw ? x : nullptr, ldx, M, K, b), place(dx ? w : nullptr, ldw, K, N, b), place(dy, ldd, M, N, b), saved(save, lds, M, N, act)}))
+    return dgnn_fail(DGNN_E_BADARG, "linear_backward: an output overlaps another operand%s");
   if (small_fit(M, K, N)) {
-    const int64_t b = width(dtype);
-    if (!matrix_ok(dy, ldd, M, N, b) || (dw && (!matrix_ok(x, ldx, M, K, b) || !matrix_ok(dw, lddw, K, N, b)))
-        || (dx && (!matrix_ok(w, ldw, K, N, b) || !matrix_ok(dx, lddx, M, K, b))) || (uintptr_t)dbias % b
-        || (act == ACT_RELU && (!save || lds < (N + 31) / 32 || (uintptr_t)save % 4)) || (act > ACT_RELU && !matrix_ok(save, lds, M, N, 4)))
-      return dgnn_fail(DGNN_E_BADARG, "linear_backward: null, misaligned or overlapping rows%s");
-    if (!apart(dx, lddx, M, K, dy, ldd, M, N, b) || !apart(dx, lddx, M, K, w, ldw, K, N, b) || !apart(dw, lddw, K, N, x, ldx, M, K, b)
-        || !apart(dw, lddw, K, N, dy, ldd, M, N, b))
-      return dgnn_fail(DGNN_E_BADARG, "linear_backward: an output overlaps an input%s");
     if (!dx && !dw && !dbias) return DGNN_OK;
     const int64_t side = M > N ? M : N, chunk = kSmall / side < 1 ? 1 : kSmall / side < 16 ? kSmall / side : 16;
     const Small g{x, w, dy, save, dx, dw, dbias, ldx, ldw, ldd, lds, lddx, lddw, (int)M, (int)K, (int)N, (int)act, (int)chunk};
@@ -478,6 +518,10 @@ int dgnn_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
     DGNN_LAUNCHED();
     return DGNN_OK;
   }
+  Gemm to_x{}, to_w{};
+  to_x.M = M; to_x.N = K; to_x.K = N; to_x.a_along = to_x.b_along = true;
+  to_w.M = K; to_w.N = N; to_w.K = M; to_w.lda = ldx; to_w.ldb = act == ACT_NONE ? ldd : N;
+  if ((dx && !launch_fits(to_x, dtype)) || (dw && !launch_fits(to_w, dtype))) return dgnn_fail(DGNN_E_BADARG, "linear_backward: too many tiles of output%s");
   char* rest = (char*)workspace + p_bytes;
   const void* p = dy;
   int64_t ldp = ldd;

@@ -36,7 +36,8 @@ extern "C" {
  *                             only needed for what is asked for). Its workspace: dgnn_linear_backward_workspace
  * workspace: device memory of dgnn_linear_workspace(pass, ...) bytes, 16-byte aligned (0 bytes: may be NULL), free to be used
  * again once the call's kernels have run. Sums over many rows are cut by a rule of the sizes alone and joined in a fixed
- * order: the same bits every run. Outputs must not overlap inputs (but p may be dy).
+ * order: the same bits every run. What a call writes must not overlap what it reads or else writes (p alone may be dy itself):
+ * such a call is refused before anything is launched. Columns of one buffer, whose rows take turns, do not overlap.
  */
 #define DGNN_ACT_NONE 0
 #define DGNN_ACT_RELU 1

@@ -94,3 +94,31 @@ def test_binding_refuses_cpu_tensors_and_other_things():
             f(x, w)
     with pytest.raises(RuntimeError, match='no CPU path'):
         spmm_cpp.linear_slope(x.detach(), None, 'none')
+
+
+# 4 x 8 x 8 takes one launch, 600 x 8 x 8 a launch for each gradient; dx, dw, db, x, w, dy and what was saved all lie apart in _backward
+@pytest.mark.parametrize('M', [4, 600])
+@pytest.mark.parametrize('kw', [
+    dict(dx=A), dict(dx=A + 32), dict(dx=B), dict(dx=C), dict(dx=D), dict(dw=A), dict(dw=C + 96), dict(dw=D + 64), dict(db=A + 32), dict(db=B + 32),
+    dict(db=C), dict(db=D + 32), dict(dx=5 << 22, dw=5 << 22), dict(dx=5 << 22, db=(5 << 22) + 64), dict(dw=6 << 22, db=(6 << 22) + 32),
+    dict(dx=A, dw=None, w=A), dict(dw=B, dx=None, x=B),
+])
+def test_backward_refuses_outputs_that_overlap(M, kw):
+    """Before any launch, whichever way the sizes take: an input gradient over x would be read as x by x^T p."""
+    assert _backward(M=M, **kw) == 1 and b'overlap' in lib.dgnn_last_error()
+
+
+def test_backward_refuses_before_it_launches():
+    """Sizes that the last product of the call cannot launch, with every operand in order."""
+    big = dict(M=1 << 13, K=1 << 24, N=1 << 15, ldx=1 << 24, ldw=1 << 15, ldd=1 << 15, lds=1 << 15, lddx=1 << 24, lddw=1 << 15, act=0, x=1 << 50, w=2 << 50, dy=3 << 50,
+               dx=4 << 50, dw=5 << 50, db=6 << 50, n=1 << 60)
+    assert _backward(**big) == 1 and b'tiles' in lib.dgnn_last_error()
+
+
+@pytest.mark.parametrize('call,kw', [
+    (_forward, dict(save=C, lds=8, act=2)), (_forward, dict(save=A, lds=8, act=3)), (_forward, dict(save=B + 32, lds=1, act=1)), (_forward, dict(bias=C + 32)),
+    (_forward, dict(res=D, ldr=8, save=D, lds=8, act=2)), (_slope, dict(p=A + 32)), (_slope, dict(p=A, ldp=16)), (_slope, dict(p=B)), (_slope, dict(db=A, ws=D, n=1 << 20)),
+    (_slope, dict(db=B + 32, ws=D, n=1 << 20)), (_slope, dict(db=C, ws=D, n=1 << 20)), (_slope, dict(p=A, db=A + 32, ws=D, n=1 << 20)),
+])
+def test_passes_refuse_operands_that_overlap(call, kw):
+    assert call(**kw) == 1 and b'overlap' in lib.dgnn_last_error()

@@ -419,3 +419,32 @@ def test_a_training_run_of_both_operators():
     for p, q in zip(ps, qs):
         # a step is lr g / (|g| + eps)-like: its slope in g is at most lr / eps = 100, gradients are off by < 1e-7
         assert float((p.double().cpu() - q).abs().max()) < 3 * 100 * 1e-7 + 1e-6
+
+
+@pytest.mark.parametrize('m', [40, 3000])
+def test_operands_that_share_a_buffer_by_columns(m):
+    """x, y, what is saved, dx and dy in columns of one buffer, the bias gradient between two of its rows: nothing overlaps, and
+    the results are those of separate matrices. An input gradient over x itself is refused with nothing written."""
+    k, n = 40, 70
+    x, w, b, r, dy = _inputs(m, k, n, 'f32', True, False, 21)
+    y, saved = spmm_cpp.linear_forward(x, w, b, 'gelu', None, save=True)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(spmm_cpp.linear(*leaves, 'gelu'), leaves, dy)
+    lib, s, f = spmm_cpp.lib, spmm_cpp._stream(x), 4
+    pitch = k + 3 * n + k + n                                  # x | y | saved | dy | dx | room for db in a row
+    buf = torch.full((m, pitch), 7.0, device='cuda')
+    at = [buf.data_ptr() + f * o for o in (0, k, k + n, k + 2 * n, k + 3 * n, k + 3 * n + k)]
+    buf[:, :k], buf[:, k + 2 * n:k + 3 * n] = x, dy
+    ws = torch.empty(1 << 23, device='cuda')
+    assert lib.dgnn_linear_forward(at[0], pitch, w.data_ptr(), n, b.data_ptr(), None, 0, at[1], pitch, at[2], pitch, m, k, n, 0, 2, ws.data_ptr(), ws.numel() * 4, s) == 0
+    dw2 = torch.empty(k, n, device='cuda')
+    before = buf.clone()
+    assert lib.dgnn_linear_backward(at[0], pitch, w.data_ptr(), n, at[3], pitch, at[2], pitch, at[0], pitch, dw2.data_ptr(), n, at[5], m, k, n, 0, 2, ws.data_ptr(),
+                                    ws.numel() * 4, s) == 1
+    assert torch.equal(buf, before)
+    assert lib.dgnn_linear_backward(at[0], pitch, w.data_ptr(), n, at[3], pitch, at[2], pitch, at[4], pitch, dw2.data_ptr(), n, at[5], m, k, n, 0, 2, ws.data_ptr(),
+                                    ws.numel() * 4, s) == 0
+    parts = buf.split([k, n, n, n, k, n], 1)
+    for got, want in zip(parts, (x, y, saved, dy, dx)):
+        assert torch.equal(got, want)
+    assert torch.equal(parts[5][0], db) and bool((parts[5][1:] == 7).all()) and torch.equal(dw2, dw)
