@@ -2,6 +2,7 @@
 // node, C entry. The same in Python costs 40 to 100 us a call, several times what small kernels take on the GPU. No
 // arithmetic here; the C ABI's functions come from the library that spmm_cpp loaded (bind()).
 
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
@@ -67,10 +68,17 @@ using Guard = c10::hip::HIPGuardMasqueradingAsCUDA;
 // ------------------------------------------------------------------------------------------- layer transform
 struct Rows { void* p; int64_t ld; };
 
+// The kernels take plain addresses: what else a tensor carries would be dropped without a word.
+void plain(const Tensor& t, const std::string& who) {
+  if (t._fw_grad(0).defined()) refuse(who + " is a dual tensor; this operator has no forward-mode derivative");
+  if (torch::jit::tracer::isTracing()) refuse(who + " is traced; torch.jit.trace cannot record this operator");
+}
+
 // a 2-D operand with unit-stride rows; `like`: the operand whose type and device it has to have
 Rows rows(const Tensor& t, const char* name, const Tensor* like = nullptr) {
   const std::string who = std::string("spmm_cpp.linear: ") + name;
   if (!t.defined()) refuse(who + " is missing");
+  plain(t, who);
   if (!t.is_cuda()) refuse(who + " is on " + t.device().str() + "; this operator has no CPU path");
   if (t.layout() != at::kStrided) refuse(who + " must be dense");
   if (code_of(t.scalar_type()) < 0) refuse(who + " must be fp32, bf16 or fp16, got " + c10::toString(t.scalar_type()));
@@ -93,6 +101,7 @@ Rows rows(const MaybeTensor& t, const char* name, const Tensor& like, int64_t m,
 
 void* vector(const MaybeTensor& t, const char* name, int64_t n, const Tensor& like) {
   if (!t || !t->defined()) return nullptr;
+  plain(*t, std::string("spmm_cpp.linear: ") + name);
   if (t->dim() != 1 || t->numel() != n || t->scalar_type() != like.scalar_type() || t->device() != like.device() || !t->is_contiguous())
     refuse(std::string("spmm_cpp.linear: ") + name + " must be a contiguous vector of " + std::to_string(n) + " " + text(like));
   return t->data_ptr();

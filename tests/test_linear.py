@@ -122,3 +122,29 @@ def test_backward_refuses_before_it_launches():
 ])
 def test_passes_refuse_operands_that_overlap(call, kw):
     assert call(**kw) == 1 and b'overlap' in lib.dgnn_last_error()
+
+
+def _passes():
+    x, w, b, r = torch.zeros(3, 4), torch.zeros(4, 5), torch.zeros(5), torch.zeros(3, 5)
+    return {'linear': (spmm_cpp.linear, [x, w, b, 'none', r]), 'linear_forward': (spmm_cpp.linear_forward, [x, w, b, 'relu', r, True]),
+            'linear_slope': (spmm_cpp.linear_slope, [r, r, 'silu']), 'linear_grad_input': (spmm_cpp.linear_grad_input, [r, w, x]),
+            'linear_grad_weight': (spmm_cpp.linear_grad_weight, [x, r])}
+
+
+@pytest.mark.parametrize('name', ['linear', 'linear_forward', 'linear_slope', 'linear_grad_input', 'linear_grad_weight'])
+def test_forward_mode_derivatives_are_refused(name):
+    """A dual tensor's tangent would be dropped, and its derivative read as zero. Refused before the device is looked at."""
+    f, args = _passes()[name]
+    with torch.autograd.forward_ad.dual_level():
+        args[0] = torch.autograd.forward_ad.make_dual(args[0], torch.ones_like(args[0]))
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            f(*args)
+
+
+@pytest.mark.parametrize('name', ['linear', 'linear_forward', 'linear_slope', 'linear_grad_input', 'linear_grad_weight'])
+def test_tracing_is_refused(name):
+    """A trace would record the empty output alone and replay whatever its memory holds."""
+    f, args = _passes()[name]
+    first, rest = args[0], args[1:]
+    with pytest.raises(RuntimeError, match='torch.jit.trace'):
+        torch.jit.trace(lambda t: f(t, *rest), first, check_trace=False)

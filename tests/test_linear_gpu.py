@@ -448,3 +448,29 @@ def test_operands_that_share_a_buffer_by_columns(m):
     for got, want in zip(parts, (x, y, saved, dy, dx)):
         assert torch.equal(got, want)
     assert torch.equal(parts[5][0], db) and bool((parts[5][1:] == 7).all()) and torch.equal(dw2, dw)
+
+
+def test_derivatives_that_would_be_dropped_are_refused():
+    """Forward mode on each operand, forward over backward, a trace, and function transforms: none returns a value without its
+    derivative."""
+    x, w, b, r, dy = _inputs(6, 4, 5, 'f32', True, True, 22)
+    for at in range(4):
+        for grad in (False, True):
+            with torch.autograd.forward_ad.dual_level():
+                ops = [t.clone().requires_grad_(grad) for t in (x, w, b, r)]
+                ops[at] = torch.autograd.forward_ad.make_dual(ops[at], torch.ones_like(ops[at]))
+                with pytest.raises(RuntimeError, match='forward-mode|forward mode'):
+                    spmm_cpp.linear(ops[0], ops[1], ops[2], 'gelu', ops[3])
+    xl = x.clone().requires_grad_(True)
+    y = spmm_cpp.linear(xl, w, b, 'gelu', r)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            torch.autograd.grad(y, xl, torch.autograd.forward_ad.make_dual(dy, torch.ones_like(dy)))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: spmm_cpp.linear(t, w, b, 'gelu', r), (x,), (torch.ones_like(x),))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: spmm_cpp.linear(t, w, b, 'gelu', r).sum())(x)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: spmm_cpp.linear(t, w, b, 'gelu', r))(x.expand(3, 6, 4))
+    with pytest.raises(RuntimeError, match='torch.jit.trace'):
+        torch.jit.trace(lambda t: spmm_cpp.linear(t, w, b, 'gelu', r), x, check_trace=False)
