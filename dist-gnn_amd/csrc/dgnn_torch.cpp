@@ -71,6 +71,7 @@ struct Rows { void* p; int64_t ld; };
 // The kernels take plain addresses: what else a tensor carries would be dropped without a word.
 void plain(const Tensor& t, const std::string& who) {
   if (t._fw_grad(0).defined()) refuse(who + " is a dual tensor; this operator has no forward-mode derivative");
+  if (t.is_neg()) refuse(who + " is a view whose values are stored negated (of a conjugate's imaginary part); call resolve_neg()");
   if (torch::jit::tracer::isTracing()) refuse(who + " is traced; torch.jit.trace cannot record this operator");
 }
 
@@ -208,6 +209,7 @@ struct Linear : torch::autograd::Function<Linear> {
     Tensor dy = grads[0], dx, dw, db;
     const int64_t M = dy.size(0), N = dy.size(1);
     if (gx || gw || gb) {
+      dy = dy.resolve_neg();
       if ((N > 1 && dy.stride(1) != 1) || (M > 1 && dy.stride(0) < N)) dy = dy.contiguous();       // expanded or transposed
       const Rows d = rows(dy, "the gradient");
       const Guard guard(dy.device());
@@ -285,8 +287,8 @@ struct AdamTable {
                std::to_string(table[i].numel) + " elements on " + device.str() + " any more that its state was made for");
       if (g.layout() != at::kStrided || g.scalar_type() != dtype || g.device() != device || g.sizes() != p.sizes())
         refuse("AdamW: the gradient of parameter " + std::to_string(i) + " is not a dense " + c10::toString(dtype) + " tensor of its shape on " + device.str());
-      if (!g.is_contiguous()) {
-        g = g.contiguous();
+      if (!g.is_contiguous() || g.is_neg()) {
+        g = g.resolve_neg().contiguous();
         kept.push_back(g);
       }
       dgnn_adamw_tensor t = table[i];

@@ -411,3 +411,12 @@ def test_more_chunks_than_one_side_of_a_grid():
     assert bool((p == 0.5).all())
     del opt, p
     torch.cuda.empty_cache()
+
+
+def test_a_gradient_that_is_stored_negated():
+    p, q = (torch.nn.Parameter(torch.ones(300, device='cuda')) for _ in range(2))
+    g = torch.randn(300, device='cuda')
+    p.grad, q.grad = torch._neg_view(g), -g
+    assert p.grad.is_neg()
+    spmm_cpp.AdamW([p, q]).step()
+    assert torch.equal(p, q)

@@ -148,3 +148,11 @@ def test_tracing_is_refused(name):
     first, rest = args[0], args[1:]
     with pytest.raises(RuntimeError, match='torch.jit.trace'):
         torch.jit.trace(lambda t: f(t, *rest), first, check_trace=False)
+
+
+def test_values_that_are_stored_negated_are_refused():
+    """One column of a conjugate's imaginary part is a plain float column by its strides; its memory holds the values' negatives."""
+    z = torch.complex(torch.ones(3, 1), torch.ones(3, 1)).conj().imag
+    assert z.is_neg()
+    with pytest.raises(RuntimeError, match='resolve_neg'):
+        spmm_cpp.linear(z, torch.zeros(1, 5))

@@ -474,3 +474,15 @@ def test_derivatives_that_would_be_dropped_are_refused():
         torch.func.vmap(lambda t: spmm_cpp.linear(t, w, b, 'gelu', r))(x.expand(3, 6, 4))
     with pytest.raises(RuntimeError, match='torch.jit.trace'):
         torch.jit.trace(lambda t: spmm_cpp.linear(t, w, b, 'gelu', r), x, check_trace=False)
+
+
+def test_a_gradient_that_is_stored_negated():
+    """The gradient of a column that became the imaginary part of a conjugate comes back as a view with its sign set lazily."""
+    x, w, b, _, _ = _inputs(50, 4, 1, 'f32', True, False, 23)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = spmm_cpp.linear(*leaves, 'silu')
+    dy = torch._neg_view(torch.randn(50, 1, device='cuda'))
+    assert dy.is_neg()
+    got = torch.autograd.grad(y, leaves, dy)
+    want = torch.autograd.grad(spmm_cpp.linear(*leaves, 'silu'), leaves, dy.resolve_neg())
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
