@@ -142,27 +142,34 @@ class AdamW(torch.optim.Optimizer):
                 for i, p in enumerate(params):
                     one = seg.views(i)
                     if p in given:
+                        self._check(one, given[p])
                         self._take(one, given[p])
                     elif seg.has_master:
                         one['master'].copy_(p.detach())
                     self.state[p] = one
                 segments.append(seg)
 
-    def _take(self, to, given):
-        """Copies a state entry of a state dict (or of another copy of this optimiser) into the views ``to``."""
+    def _check(self, to, given):
+        """Refuses a state entry of a state dict (or of another copy of this optimiser) that does not fit the views ``to``."""
         if set(given) != set(to):
             raise ValueError(f'AdamW: a state with {sorted(given)} does not fit state_bits={self.state_bits}, '
                              f'master_weights={self.master_weights} (wanted: {sorted(to)})')
         for name, x in to.items():
             y = given[name]
             if name == 'step':
-                x.fill_(int(y))
-                continue
-            if not isinstance(y, torch.Tensor) or y.numel() != x.numel():
+                int(y)
+            elif not isinstance(y, torch.Tensor) or y.numel() != x.numel():
                 raise ValueError(f'AdamW: state {name} does not have the parameter\'s size')
-            if x.dtype.itemsize == 1:
-                if y.dtype != x.dtype:
-                    raise ValueError(f'AdamW: state {name} must be {x.dtype}, got {y.dtype}')
+            elif x.dtype.itemsize == 1 and y.dtype != x.dtype:
+                raise ValueError(f'AdamW: state {name} must be {x.dtype}, got {y.dtype}')
+
+    def _take(self, to, given):
+        """Copies a state entry that ``_check`` passed into the views ``to``."""
+        for name, x in to.items():
+            y = given[name]
+            if name == 'step':
+                x.fill_(int(y))
+            elif x.dtype.itemsize == 1:
                 x.view(torch.uint8).view(-1).copy_(y.contiguous().view(torch.uint8).view(-1))
             else:
                 x.view(-1).copy_(y.reshape(-1))
@@ -175,17 +182,40 @@ class AdamW(torch.optim.Optimizer):
         found = [s for segments in self._segments for s in segments]
         return {name + (f'.{i}' if i else ''): t for i, s in enumerate(found) for name, t in s.flat.items()}
 
+    @torch.no_grad()
     def load_state_dict(self, state_dict):
-        packed = state_dict['state']
-        super().load_state_dict({'state': {}, 'param_groups': state_dict['param_groups']})
-        ids = [i for g in state_dict['param_groups'] for i in g['params']]
-        params = [p for g in self.param_groups for p in g['params']]
-        self._segments = None
-        self.state.clear()
+        """Writes the state into the buffers that are there (a captured step goes on with it); a parameter without an entry
+        starts anew. A state that does not fit is refused with nothing written."""
         self.init_state()
-        for i, p in zip(ids, params):
-            if i in packed:
-                self._take(self.state[p], packed[i])
+        kept, found = (self._segments, self.state), {}
+        own = {t.untyped_storage().data_ptr() for segments in self._segments for s in segments for t in (*s.flat.values(), s.steps)}
+
+        def check(_, given):                              # behind the hooks that may change what is loaded
+            ids = [i for g in given['param_groups'] for i in g['params']]
+            for i, p in zip(ids, (p for g in self.param_groups for p in g['params'])):
+                if given['state'].get(i):
+                    self._check(self.state[p], given['state'][i])
+                    found[p] = {n: y.clone() if isinstance(y, torch.Tensor) and y.untyped_storage().data_ptr() in own else y
+                                for n, y in given['state'][i].items()}
+            return {**given, 'state': {}}
+
+        def fill(_):                                      # before the hooks that look at what was loaded
+            self._segments, self.state = kept
+            for group in self.param_groups:
+                for p in group['params']:
+                    to = self.state[p]
+                    if p in found:
+                        self._take(to, found[p])
+                        continue
+                    for name, x in to.items():
+                        x.copy_(p) if name == 'master' else (x.view(torch.uint8) if x.dtype.itemsize == 1 else x).zero_()
+
+        hooks = (self.register_load_state_dict_pre_hook(check), self.register_load_state_dict_post_hook(fill, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
 
     def __getstate__(self):
         return {**super().__getstate__(), 'state_bits': self.state_bits, 'master_weights': self.master_weights,

@@ -420,3 +420,83 @@ def test_a_gradient_that_is_stored_negated():
     assert p.grad.is_neg()
     spmm_cpp.AdamW([p, q]).step()
     assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize('bits,dtype,master', [(32, 'f32', False), (8, 'bf16', True)])
+def test_a_state_loaded_behind_a_captured_step(bits, dtype, master):
+    """A checkpoint is loaded into the buffers that a captured step writes: its replays go on from the loaded state, as an eager
+    optimiser that loads the same does."""
+    kw = dict(lr=LR, betas=(B1, B2), eps=EPS, weight_decay=DECAY, state_bits=bits, master_weights=master)
+    mine = _params((500, 4097, 3), DT[dtype], 16)
+    theirs = [torch.nn.Parameter(p.detach().clone()) for p in mine]
+    opt, eager = spmm_cpp.AdamW(mine, capturable=True, **kw), spmm_cpp.AdamW(theirs, **kw)
+    for k in range(2):
+        _grads(theirs, k)
+        for p, q in zip(mine, theirs):
+            p.grad = q.grad.clone()
+        opt.step()
+        eager.step()
+    saved = copy.deepcopy(opt.state_dict())
+    start = [p.detach().clone() for p in mine]
+    places = {n: t.data_ptr() for n, t in opt.state_buffers().items()}
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    opt.load_state_dict(saved)
+    eager.load_state_dict(saved)
+    assert places == {n: t.data_ptr() for n, t in opt.state_buffers().items()}
+    with torch.no_grad():
+        for p, q, s in zip(mine, theirs, start):
+            p.copy_(s)
+            q.copy_(s)
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(mine, theirs):
+            q.grad = p.grad.clone()
+        eager.step()
+        for p, q in zip(mine, theirs):
+            assert torch.equal(p, q) and int(opt.state[p]['step']) == int(eager.state[q]['step']) == k + 3
+            for n, x in opt.state[p].items():
+                assert n == 'step' or torch.equal(x.float(), eager.state[q][n].float()), n
+
+
+def test_a_state_that_does_not_fit_changes_nothing():
+    params = _params((300, 700), torch.float32, 17)
+    opt = spmm_cpp.AdamW(params, lr=LR)
+    _grads(params, 0)
+    opt.step()
+    good = copy.deepcopy(opt.state_dict())
+    before = {n: t.clone() for n, t in opt.state_buffers().items()}
+    short, odd, less = copy.deepcopy(good), copy.deepcopy(good), copy.deepcopy(good)
+    short['state'][1]['exp_avg_sq'] = short['state'][1]['exp_avg_sq'][:-1]
+    del odd['state'][1]['exp_avg']
+    less['param_groups'][0]['params'] = [0]
+    for bad in (short, odd, less):
+        with pytest.raises(ValueError):
+            opt.load_state_dict(bad)
+        assert all(torch.equal(t, before[n]) for n, t in opt.state_buffers().items()) and int(opt.state[params[1]]['step']) == 1
+        assert opt.state[params[0]]['exp_avg'].data_ptr() == opt.state_buffers()['exp_avg'].data_ptr()
+    opt.step()
+    assert int(opt.state[params[0]]['step']) == 2
+
+
+def test_loading_permuted_partial_and_hooked_states():
+    """Two parameters' own states exchanged, one left out, and hooks that change what is loaded and see what was."""
+    params = _params((300, 300), torch.float32, 18)
+    opt = spmm_cpp.AdamW(params, lr=LR)
+    _grads(params, 0)
+    opt.step()
+    a, b = (opt.state[p]['exp_avg'].clone() for p in params)
+    given = opt.state_dict()
+    opt.load_state_dict({**given, 'state': {0: given['state'][1], 1: given['state'][0]}})
+    assert torch.equal(opt.state[params[0]]['exp_avg'], b) and torch.equal(opt.state[params[1]]['exp_avg'], a)
+    given = copy.deepcopy(opt.state_dict())
+    opt.load_state_dict({**given, 'state': {0: given['state'][0]}})
+    assert torch.equal(opt.state[params[0]]['exp_avg'], b) and not opt.state[params[1]]['exp_avg'].any() and int(opt.state[params[1]]['step']) == 0
+    seen = []
+    opt.register_load_state_dict_pre_hook(lambda o, d: {**d, 'state': {i: {**s, 'step': 40 + i} for i, s in d['state'].items()}})
+    opt.register_load_state_dict_post_hook(lambda o: seen.append([int(o.state[p]['step']) for p in params]))
+    opt.load_state_dict(given)
+    assert seen == [[40, 41]]
