@@ -5,6 +5,7 @@ parameter. Here a step is one pass over parameter, gradient and moments, for up 
 in 32 or in 8 bits.
 """
 import math
+import operator
 
 import numpy as np
 import torch
@@ -84,7 +85,8 @@ class AdamW(torch.optim.Optimizer):
     ``init_state()``, before the capture. A counter belongs to a parameter: one without a gradient is left out and not counted.
 
     State tensors are views of flat buffers (``state_buffers()``): write into them or use ``load_state_dict``; putting
-    other tensors in their place is not seen. Parameters must be contiguous and must not overlap."""
+    other tensors in their place is not seen. Parameters must be contiguous and must not overlap, and stay in their group once
+    they have state."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False,
                  capturable=False):
@@ -102,6 +104,9 @@ class AdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------ state
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
+        self._check_params()
+
+    def _check_params(self):
         seen = set()
         for group in self.param_groups:
             for p in group['params']:
@@ -126,10 +131,15 @@ class AdamW(torch.optim.Optimizer):
     def init_state(self):
         """Allocates the state of parameters that have none yet (zeros; a master takes its parameter's value)."""
         if self._segments is None:
-            self._segments = [[] for _ in self.param_groups]
+            self._segments, self._known = [[] for _ in self.param_groups], []
             given = {p: s for p, s in self.state.items() if s}
         else:
             given = {}
+        self._check_params()
+        for known, params in zip(self._known, [g['params'] for g in self.param_groups] + [()] * len(self._known)):
+            if {id(p) for p in known} - {id(p) for p in params}:
+                raise RuntimeError('AdamW: a parameter was taken out of param_groups or replaced after its state was made; make a new '
+                                   'optimiser (load_state_dict brings the state along)')
         self._segments += [[] for _ in self.param_groups[len(self._segments):]]
         for group, segments in zip(self.param_groups, self._segments):
             known = {id(p) for s in segments for p in s.params}
@@ -148,6 +158,7 @@ class AdamW(torch.optim.Optimizer):
                         one['master'].copy_(p.detach())
                     self.state[p] = one
                 segments.append(seg)
+        self._known = [list(group['params']) for group in self.param_groups]
 
     def _check(self, to, given):
         """Refuses a state entry of a state dict (or of another copy of this optimiser) that does not fit the views ``to``."""
@@ -235,8 +246,8 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if self._segments is None or any(sum(len(s.params) for s in segs) != len(g['params'])
-                                         for segs, g in zip(self._segments + [[]] * len(self.param_groups), self.param_groups)):
+        if self._segments is None or len(self._known) != len(self.param_groups) or not all(
+                len(known) == len(g['params']) and all(map(operator.is_, known, g['params'])) for known, g in zip(self._known, self.param_groups)):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError('AdamW: take a step or call init_state() before capturing one in a graph')
             self.init_state()

@@ -500,3 +500,39 @@ def test_loading_permuted_partial_and_hooked_states():
     opt.register_load_state_dict_post_hook(lambda o: seen.append([int(o.state[p]['step']) for p in params]))
     opt.load_state_dict(given)
     assert seen == [[40, 41]]
+
+
+def test_parameters_that_left_their_group():
+    """The optimiser steps what param_groups holds, never a tensor that was replaced there; late additions get their state."""
+    a, b, c = (torch.nn.Parameter(torch.ones(n, device='cuda')) for n in (300, 20, 300))
+    opt = spmm_cpp.AdamW([a, b], lr=LR)
+    for p in (a, b, c):
+        p.grad = torch.ones_like(p)
+    opt.step()
+    kept = [p.detach().clone() for p in (a, b, c)]
+    group = opt.param_groups[0]
+    for params in ([c, b], [a], [a, c]):
+        group['params'] = params
+        with pytest.raises(RuntimeError, match='replaced'):
+            opt.step()
+        assert all(torch.equal(p, k) for p, k in zip((a, b, c), kept))
+    cpu = torch.nn.Parameter(torch.ones(3))
+    cpu.grad = torch.ones(3)
+    for params, why in (([a, b, cpu], 'no CPU path'), ([a, b, a], 'twice'), ([a, b, torch.nn.Parameter(a.detach()[5:9])], 'overlap')):
+        group['params'] = params
+        with pytest.raises(RuntimeError, match=why):
+            opt.step()
+    for params in ([b, a], [b, c, a]):
+        group['params'] = params
+        opt.step()
+    assert [int(opt.state[p]['step']) for p in (a, b, c)] == [3, 3, 1]
+    other = spmm_cpp.AdamW([c, b], lr=LR)
+    other.load_state_dict({'state': {1: opt.state_dict()['state'][0]}, 'param_groups': [{**other.state_dict()['param_groups'][0]}]})
+    assert int(other.state[b]['step']) == 3
+    group['params'] = [a, b, c]
+    opt.step()
+    opt.param_groups.append({**group, 'params': [torch.nn.Parameter(torch.ones(3, device='cuda'))]})
+    opt.init_state()
+    del opt.param_groups[1]
+    with pytest.raises(RuntimeError, match='replaced'):
+        opt.step()
