@@ -238,10 +238,14 @@ Tensor linear(const Tensor& x, const Tensor& w, const MaybeTensor& bias, int64_t
 }
 
 // ------------------------------------------------------------------------------------------- AdamW
-// The parameters of one optimiser segment and where their state lies; step() reads their gradients and launches.
+// The parameters of one optimiser segment and where their state lies; collect() reads and checks their gradients, launch()
+// steps what it found.
 struct AdamTable {
   std::vector<Tensor> params;
   std::vector<dgnn_adamw_tensor> table, live;
+  std::vector<size_t> which;        // live's parameters
+  std::vector<Tensor> kept;         // gradients that had to be made contiguous
+  double lr = 0, b1 = 0, b2 = 0, eps = 0;
   dgnn_adamw_state state{};
   Tensor steps;                     // host counters, or the device's where the step can be captured
   bool capturable;
@@ -270,11 +274,12 @@ struct AdamTable {
     }
   }
 
-  // one step of the parameters that have a gradient; returns how many
-  int64_t step(double lr, double b1, double b2, double eps, double decay) {
+  // the parameters that have a gradient; returns how many
+  int64_t collect(double lr_, double b1_, double b2_, double eps_, double decay) {
+    lr = lr_, b1 = b1_, b2 = b2_, eps = eps_;
     live.clear();
-    std::vector<Tensor> kept;       // gradients that had to be made contiguous
-    std::vector<size_t> which;
+    which.clear();
+    kept.clear();
     int64_t* const count = capturable ? nullptr : steps.data_ptr<int64_t>();
     int64_t last = -1;
     float rate = 0.f, root = 0.f;
@@ -309,7 +314,11 @@ struct AdamTable {
       live.push_back(t);
       which.push_back(i);
     }
-    if (live.empty()) return 0;
+    return (int64_t)live.size();
+  }
+
+  void launch() {
+    int64_t* const count = capturable ? nullptr : steps.data_ptr<int64_t>();
     const Guard guard(device);
     check(api.adamw(live.data(), (int32_t)live.size(), code_of(dtype), bits, &state, lr, b1, b2, eps, stream_of(params[0])), "adamw");
     for (size_t i : which) {
@@ -317,7 +326,7 @@ struct AdamTable {
       // the kernel writes behind autograd's back: a graph that saved a parameter has to notice
       if (!params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();
     }
-    return (int64_t)live.size();
+    kept.clear();
   }
 };
 
@@ -333,5 +342,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   py::class_<AdamTable>(m, "AdamTable")
       .def(py::init<const std::vector<Tensor>&, const std::vector<int64_t>&, int, const Tensor&, const Tensor&, const MaybeTensor&, const MaybeTensor&,
                     const MaybeTensor&, const Tensor&, const MaybeTensor&>())
-      .def("step", &AdamTable::step);
+      .def("collect", &AdamTable::collect)
+      .def("launch", &AdamTable::launch);
 }

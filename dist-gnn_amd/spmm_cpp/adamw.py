@@ -91,10 +91,8 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False,
                  capturable=False):
         for name, x in (('lr', lr), ('eps', eps), ('weight_decay', weight_decay)):
-            if isinstance(x, torch.Tensor) or not x >= 0 or math.isinf(x):
-                raise ValueError(f'AdamW: {name} must be a finite number >= 0, got {x!r}')
-        if len(betas) != 2 or not all(0 <= b < 1 for b in betas):
-            raise ValueError(f'AdamW: betas must lie in [0, 1), got {betas!r}')
+            if isinstance(x, torch.Tensor):
+                raise ValueError(f'AdamW: {name} must be a number, got {x!r}')
         if state_bits not in (8, 32):
             raise ValueError(f'AdamW: state_bits must be 8 or 32, got {state_bits!r}')
         self._segments = None
@@ -104,7 +102,18 @@ class AdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------ state
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
+        self._check_options(self.param_groups[-1])
         self._check_params()
+
+    @staticmethod
+    def _check_options(group):
+        for name in ('lr', 'eps', 'weight_decay'):
+            x = float(group[name])
+            if not x >= 0 or math.isinf(x):
+                raise ValueError(f'AdamW: {name} must be a finite number >= 0, got {x!r}')
+        betas = group['betas']
+        if len(betas) != 2 or not all(0 <= b < 1 for b in betas):
+            raise ValueError(f'AdamW: betas must lie in [0, 1), got {betas!r}')
 
     def _check_params(self):
         seen = set()
@@ -252,10 +261,15 @@ class AdamW(torch.optim.Optimizer):
                 raise RuntimeError('AdamW: take a step or call init_state() before capturing one in a graph')
             self.init_state()
         capturing = not self.capturable and torch.cuda.is_current_stream_capturing()
+        ready = []
         for group, segments in zip(self.param_groups, self._segments):
             if capturing and any(p.grad is not None for p in group['params']):
                 raise RuntimeError('AdamW: a step is captured in a graph, but the optimiser was made without capturable=True')
+            self._check_options(group)
             b1, b2 = group['betas']
             for seg in segments:
-                seg.table.step(float(group['lr']), b1, b2, float(group['eps']), float(group['weight_decay']))
+                if seg.table.collect(float(group['lr']), b1, b2, float(group['eps']), float(group['weight_decay'])):
+                    ready.append(seg.table)
+        for table in ready:                               # every parameter has passed its checks: all are stepped or none
+            table.launch()
         return loss

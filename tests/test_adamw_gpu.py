@@ -536,3 +536,26 @@ def test_parameters_that_left_their_group():
     del opt.param_groups[1]
     with pytest.raises(RuntimeError, match='replaced'):
         opt.step()
+
+
+def test_a_step_that_is_refused_steps_nothing():
+    """Whatever is wrong with a later group, the earlier ones stay as they are, and the next step is their first."""
+    a, b, c = (torch.nn.Parameter(torch.ones(n, device='cuda', dtype=t)) for n, t in ((300, torch.float32), (20, torch.bfloat16), (30, torch.float32)))
+    opt = spmm_cpp.AdamW([{'params': [a, b]}, {'params': [c]}], lr=LR)
+    for p in (a, b, c):
+        p.grad = torch.ones_like(p)
+    good, last = c.grad, opt.param_groups[1]
+    c.grad = good.to_sparse()
+    with pytest.raises(RuntimeError, match='gradient'):
+        opt.step()
+    c.grad = good
+    for name, x in (('lr', float('nan')), ('weight_decay', -1.0), ('weight_decay', float('nan')), ('eps', float('inf')), ('betas', (0.9, 1.0))):
+        kept = last[name]
+        last[name] = x
+        with pytest.raises(ValueError, match='AdamW'):
+            opt.step()
+        last[name] = kept
+    torch.cuda.synchronize()
+    assert all(bool((p == 1).all()) and int(opt.state[p]['step']) == 0 for p in (a, b, c))
+    opt.step()
+    assert all(bool((p < 1).all()) and int(opt.state[p]['step']) == 1 for p in (a, b, c))
