@@ -102,8 +102,12 @@ class AdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------ state
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
-        self._check_options(self.param_groups[-1])
-        self._check_params()
+        try:
+            self._check_options(self.param_groups[-1])
+            self._check_params()
+        except Exception:
+            self.param_groups.pop()                       # a group that is refused is not there
+            raise
 
     @staticmethod
     def _check_options(group):

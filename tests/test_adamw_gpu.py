@@ -559,3 +559,17 @@ def test_a_step_that_is_refused_steps_nothing():
     assert all(bool((p == 1).all()) and int(opt.state[p]['step']) == 0 for p in (a, b, c))
     opt.step()
     assert all(bool((p < 1).all()) and int(opt.state[p]['step']) == 1 for p in (a, b, c))
+
+
+def test_a_group_that_is_refused_is_not_there():
+    a, b = (torch.nn.Parameter(torch.ones(n, device='cuda')) for n in (300, 20))
+    opt = spmm_cpp.AdamW([a], lr=LR)
+    for bad in ({'params': [b], 'lr': -1.0}, {'params': [b], 'weight_decay': float('nan')}, {'params': [b], 'betas': (0.9,)},
+                {'params': [b, torch.nn.Parameter(a.detach()[3:9])]}, {'params': [torch.nn.Parameter(torch.ones(3))]}):
+        with pytest.raises((RuntimeError, ValueError), match='AdamW'):
+            opt.add_param_group(bad)
+        assert len(opt.param_groups) == 1
+    opt.add_param_group({'params': [b], 'lr': 0.0})
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    opt.step()
+    assert bool((a < 1).all()) and len(opt.param_groups) == 2 and int(opt.state[b]['step']) == 1
