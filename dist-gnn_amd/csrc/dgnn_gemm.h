@@ -336,6 +336,14 @@ __device__ __forceinline__ void finish(const Gemm& g, int64_t row, int64_t col, 
   store4((T*)g.c + row * g.ldc + col, have, v);
 }
 
+// Lanes of a wave exchange values through LDS: what was written before is there for what is read behind, whichever lane's it is.
+// The wave's LDS operations run in order, so this is an order for the compiler and no instruction.
+__device__ __forceinline__ void lanes_meet() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // A wave's TM x TN tiles of 32 x 32 from its accumulators to memory, 32 rows at a time through its own part of LDS: the
 // matrix cores leave a column's rows in a lane, memory wants a row's columns side by side (16 bytes of fp32 a lane). The
 // residual's rows are fetched before the turn, so that nothing waits for them one by one.
@@ -364,6 +372,7 @@ __device__ __forceinline__ void epilogue(const Gemm& g, f16v (&acc)[TM][TN], flo
 #pragma unroll
       for (int e = 0; e < 16; ++e)              // element e of a lane: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32
         room[(8 * (e / 4) + 4 * (lane >> 5) + e % 4) * PITCH + j * 32 + (lane & 31)] = acc[i][j][e];
+    lanes_meet();
 #pragma unroll
     for (int q = 0; q < TURNS; ++q) {
       const int64_t row = first + q * STEP;
@@ -383,6 +392,7 @@ __device__ __forceinline__ void epilogue(const Gemm& g, f16v (&acc)[TM][TN], flo
       if (whole) finish<T>(g, row, col, have, v, bias, res[q]);
       else store4(g.partial + ((int64_t)blockIdx.y * g.M + row) * g.N + col, have, v);
     }
+    lanes_meet();                               // the next 32 rows take the same room
   }
 }
 
