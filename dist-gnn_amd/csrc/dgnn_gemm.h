@@ -12,8 +12,9 @@
 // the split is exact up to 2^-25 |a|), and the six products of at least 2^-16 relative size are summed in the fp32
 // accumulators: a1 b1 + a1 b2 + a2 b1 + a2 b2 + a1 b3 + a3 b1. What is left out is at most 2^-24 |a| |b| a term, as much as
 // one fp32 rounding. Values under 2^-109 lose bits (their last pieces are below bf16's smallest number): absolute
-// errors of 2^-134 |b|. An infinity's pieces are not finite and would give NaN where fp32 gives infinity, so an output that
-// is not finite is computed again as a chain of fused multiply-adds, whose infinities and NaN are fp32's own.
+// errors of 2^-134 |b|. An infinity's pieces are not finite and would give NaN where fp32 gives infinity, so a tile of 32 x 32
+// outputs with some that are not finite is multiplied again by fp32's own matrix instruction (again() below), whose infinities
+// and NaN are those of fp32 operations; only the outputs that are not finite take its values.
 #pragma once
 #include "dgnn_internal.h"
 
@@ -269,6 +270,42 @@ __device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c, _Float16) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, y.h, c, 0, 0, 0);
 }
 
+// sums that are not finite: 0 if there are none, else NaN
+__device__ __forceinline__ float unsound(const f16v& acc) {
+  float seen = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) seen = fmaf(acc[e], 0.f, seen);
+  return seen;
+}
+
+// Those of a wave's 32 x 32 sums that are not finite, once more, from `t`: D[m][n] += sum over k of a(m, k) b(n, k), a lane's
+// a(lane % 32, k) at a + k ak and b(lane % 32, k) at b + k bk. All lanes take part. A step of two of the contraction takes 64
+// cycles, 2.7 times the six bf16 products, and its operands come from memory one by one: with every value NaN 232965 x 602 x 256
+// takes 2509 us (finite 522), 4096 x 256 x 256 84 (18.6); with one infinity in the latter's x 74. (A chain of multiply-adds by
+// the lane that holds a sum: 1935 and 1584.)
+__device__ __forceinline__ void again(f16v& acc, f16v t, const float* a, int64_t ak, const float* b, int64_t bk, int64_t k0, int64_t kend) {
+  constexpr int U = 4;                                         // loads of each operand in flight
+  const int64_t mine = U * ((threadIdx.x & 63) >> 5);
+  a += (k0 + mine) * ak;
+  b += (k0 + mine) * bk;
+#pragma unroll 1
+  for (int64_t left = kend - k0; left > 0; left -= 2 * U) {
+    float x[U], y[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const bool in = mine + i < left;
+      x[i] = in ? a[i * ak] : 0.f;
+      y[i] = in ? b[i * bk] : 0.f;
+    }
+    a += 2 * U * ak;
+    b += 2 * U * bk;
+#pragma unroll
+    for (int i = 0; i < U; ++i) t = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], t, 0, 0, 0);
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = fabsf(acc[e]) < __builtin_huge_valf() ? acc[e] : t[e];
+}
+
 template <typename T> struct Four { typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T) == 4 ? 4 : 2))); };
 
 // `have` (0..4) elements at p; the others are zero
@@ -356,6 +393,18 @@ __device__ __forceinline__ void epilogue(const Gemm& g, f16v (&acc)[TM][TN], flo
   const bool whole = g.slices == 1;
   float bias[4] = {0.f, 0.f, 0.f, 0.f};
   if (whole && g.bias) load4((const T*)g.bias + col, have_n, bias);
+  if constexpr (Unit<T>::PLANES == 3) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int64_t m = row0 + i * 32 + (lane & 31), n = col0 + j * 32 + (lane & 31);          // past the ends the last ones stand in
+        if (!__ballot(n < g.N && !(unsound(acc[i][j]) == 0.f))) continue;
+        const int64_t mi = m < g.M ? m : g.M - 1, ni = n < g.N ? n : g.N - 1;
+        again(acc[i][j], f16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}, (const T*)g.a + (AA ? mi * g.lda : mi), AA ? 1 : g.lda,
+              (const T*)g.b + (BA ? ni * g.ldb : ni), BA ? 1 : g.ldb, k0, kend);
+      }
+  }
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int64_t first = row0 + i * 32 + lane / LANES;
@@ -379,16 +428,6 @@ __device__ __forceinline__ void epilogue(const Gemm& g, f16v (&acc)[TM][TN], flo
       const int have = row < g.M ? have_n : 0;
       const float4 t = *reinterpret_cast<const float4*>(room + (lane / LANES + q * STEP) * PITCH + (lane % LANES) * 4);
       float v[4] = {t.x, t.y, t.z, t.w};
-      if constexpr (Unit<T>::PLANES == 3) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (c < have && !(fabsf(v[c]) < __builtin_huge_valf())) {
-            const T* a = (const T*)g.a + (AA ? row * g.lda : row);
-            const T* b = (const T*)g.b + (BA ? (col + c) * g.ldb : col + c);
-            v[c] = 0.f;
-            for (int64_t k = k0; k < kend; ++k) v[c] = fmaf((float)a[AA ? k : k * g.lda], (float)b[BA ? k : k * g.ldb], v[c]);
-          }
-      }
       if (whole) finish<T>(g, row, col, have, v, bias, res[q]);
       else store4(g.partial + ((int64_t)blockIdx.y * g.M + row) * g.N + col, have, v);
     }
@@ -738,17 +777,21 @@ template <typename T, int TN> struct Wave {
   Eight<T> a[S];                                              // this lane's part of its row: 8 elements of each 16
 
   // sums start at the bias: element e of a lane is column 8 (e / 4) + 4 half + e % 4 of the tile, row lane % 32
+  static __device__ __forceinline__ f16v bias_of(const Gemm& g, int64_t col0, int half) {
+    f16v t;
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      float b[4] = {0.f, 0.f, 0.f, 0.f};
+      const int64_t col = col0 + 2 * e + 4 * half;
+      if (g.bias) load4((const T*)g.bias + col, g.N - col >= 4 ? 4 : (g.N > col ? (int)(g.N - col) : 0), b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[e + i] = b[i];
+    }
+    return t;
+  }
   __device__ __forceinline__ void begin(const Gemm& g, int64_t col0, int half) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        float b[4] = {0.f, 0.f, 0.f, 0.f};
-        const int64_t col = col0 + j * 32 + 2 * e + 4 * half;
-        if (g.bias) load4((const T*)g.bias + col, g.N - col >= 4 ? 4 : (g.N > col ? (int)(g.N - col) : 0), b);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[j][e + i] = b[i];
-      }
+    for (int j = 0; j < TN; ++j) acc[j] = bias_of(g, col0 + j * 32, half);
   }
 
   // stage kt of the row whose lane part begins at p
@@ -813,26 +856,13 @@ template <typename T, int TN> struct Wave {
   __device__ __forceinline__ void finish(const Gemm& g, int64_t row, int64_t col0, int half) {
     const bool in = row < g.M;
     if constexpr (PL == 3) {
-      float seen = 0.f;                                       // 0, or NaN where a sum is not finite
-      each<0, TN>([&](auto j) __attribute__((always_inline)) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) seen = fmaf(acc[j][e], 0.f, seen);
-      });
+      float seen = 0.f;
+      each<0, TN>([&](auto j) __attribute__((always_inline)) { seen += unsound(acc[j]); });
       if (__ballot(!(seen == 0.f))) {
+        const int64_t mine = in ? row : g.M - 1;
         each<0, TN>([&](auto j) __attribute__((always_inline)) {
-#pragma unroll 1
-          for (int e = 0; e < 16; ++e) {
-            const int64_t col = col0 + j * 32 + 8 * (e / 4) + 4 * half + e % 4;
-            float t = acc[j][e];
-            if (in && col < g.N && !(fabsf(t) < __builtin_huge_valf())) {
-              const T* x = (const T*)g.a + row * g.lda;
-              const T* y = (const T*)g.b + (g.b_along ? col * g.ldb : col);
-              t = 0.f;
-              for (int64_t k = 0; k < g.K; ++k) t = fmaf((float)x[k], (float)y[g.b_along ? k : k * g.ldb], t);
-              if (g.bias) t += (float)((const T*)g.bias)[col];
-            }
-            acc[j][e] = t;
-          }
+          const int64_t n = col0 + j * 32 + (threadIdx.x & 31), ni = n < g.N ? n : g.N - 1;
+          again(acc[j], bias_of(g, col0 + j * 32, half), (const T*)g.b + (g.b_along ? ni * g.ldb : ni), g.b_along ? 1 : g.ldb, (const T*)g.a + mine * g.lda, 1, 0, g.K);
         });
       }
     }
@@ -865,7 +895,7 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 // W's stages go round two buffers in LDS, copied there by the memory unit itself while the stage before is multiplied; each
 // buffer is an array of its own, so that the compiler sees that a copy into one does not touch the reads of the other.
 template <typename T, int TN, int WAVES, int R>
-__global__ __launch_bounds__(WAVES * 64, R == 2 ? 2 : 3) void rows_kernel(const Gemm g, const char* image, int ktiles) {
+__global__ __launch_bounds__(WAVES * 64, R == 2 ? 2 : TN == 4 ? 3 : 4) void rows_kernel(const Gemm g, const char* image, int ktiles) {
   using V = Wave<T, TN>;
   constexpr int STAGE = V::STAGE, PIECES = STAGE / 1024, PER = (PIECES + WAVES - 1) / WAVES;
   __shared__ __attribute__((aligned(16))) char even[STAGE];
@@ -1118,21 +1148,8 @@ __global__ __launch_bounds__(256, 3) void columns_kernel(const Gemm g) {
 
   each<0, TN>([&](auto j) __attribute__((always_inline)) {
     const int64_t col = col0 + j * 32 + (lane & 31);
-    float seen = 0.f;                                          // 0, or NaN where a sum is not finite
-#pragma unroll
-    for (int e = 0; e < 16; ++e) seen = fmaf(acc[j][e], 0.f, seen);
-    if (__ballot(!(seen == 0.f))) {
-#pragma unroll 1
-      for (int e = 0; e < 16; ++e) {
-        const int64_t row = row0 + 8 * (e / 4) + 4 * half + e % 4;
-        float t = acc[j][e];
-        if (row < g.M && col < g.N && !(fabsf(t) < __builtin_huge_valf())) {
-          t = 0.f;
-          for (int64_t k = kbeg; k < kend; ++k) t = fmaf(x[k * g.lda + row], p[k * g.ldb + col], t);
-        }
-        acc[j][e] = t;
-      }
-    }
+    if (__ballot(col < g.N && !(unsound(acc[j]) == 0.f)))
+      again(acc[j], f16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}, x + (mine < g.M ? mine : g.M - 1), g.lda, p + (col < g.N ? col : g.N - 1), g.ldb, kbeg, kend);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int64_t row = row0 + 8 * (e / 4) + 4 * half + e % 4;

@@ -486,3 +486,91 @@ def test_a_gradient_that_is_stored_negated():
     got = torch.autograd.grad(y, leaves, dy)
     want = torch.autograd.grad(spmm_cpp.linear(*leaves, 'silu'), leaves, dy.resolve_neg())
     assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def _ieee(a, b):
+    """a b in 64 bits with every product of a row or column that is not finite as IEEE has it (inf * 0 is NaN), and the bound of
+    its finite values' fp32 sums."""
+    fa, fb = (torch.where(torch.isfinite(t), t, torch.zeros_like(t)) for t in (a, b))
+    out = fa @ fb
+    for i in torch.nonzero(~torch.isfinite(a).all(1)).view(-1).tolist():
+        out[i] = (a[i].unsqueeze(1) * b).sum(0)
+    for j in torch.nonzero(~torch.isfinite(b).all(0)).view(-1).tolist():
+        out[:, j] = (a * b[:, j]).sum(1)
+    return out, _sum_bound(a.shape[1], 'f32') * (fa.abs() @ fb.abs())
+
+
+def _like_ieee(got, clean, a, b, bias=None):
+    """Infinities and NaN are fp32's own, finite values hold their bound, rows and columns without such values (if there are some) the very bits
+    they have when there are none anywhere."""
+    a, b = _d(a), _d(b)
+    want, bound = _ieee(a, b)
+    if bias is not None:
+        want, bound = want + _d(bias), bound + U * _d(bias).abs()
+    want = want.float()                                       # past fp32's range is infinity
+    got, clean = got.cpu(), clean.cpu()
+    # where an infinity stands in a sum whose finite terms alone can pass fp32's range (bound / bound's factor is their absolute
+    # sum), a part of the sum can be an infinity of the other sign: which of infinity and NaN it gives is the order of the parts
+    both = torch.isinf(want) & (bound > 3.4e38 * _sum_bound(a.shape[1], 'f32')) & ~(torch.isfinite(a).all(1).unsqueeze(1) & torch.isfinite(b).all(0).unsqueeze(0))
+    assert not bool(torch.isfinite(got[both]).any())
+    got, want = got.masked_fill(both, 0), want.masked_fill(both, 0)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+    assert torch.equal(got[torch.isinf(got)], want[torch.isinf(want)])
+    fine = torch.isfinite(want)
+    assert bool(((got.double() - want.double()).abs() <= bound + 2 * U * want.double().abs())[fine].all())
+    same = (torch.isfinite(a) & (a.abs() < 1e30)).all(1).unsqueeze(1) & (torch.isfinite(b) & (b.abs() < 1e30)).all(0).unsqueeze(0)
+    assert torch.equal(got[same], clean[same])
+
+
+@pytest.mark.parametrize('m,k,n', [(4227, 203, 70), (4230, 130, 300), (12300, 70, 41), (16500, 9, 20), (300, 500, 50), (70, 64, 80)])
+def test_fp32_values_that_are_not_finite_at_many_sizes(m, k, n):
+    """Rows enough for the kernels that take rows straight from memory, W as it lies and W^T, every side ragged, NaN between the
+    rows; and the tiles' kernels, cut along the contraction or not."""
+    inf, nan, big = float('inf'), float('nan'), 3.4e38
+    x, w, b, _, p = _inputs(m, k, n, 'f32', True, False, 31, pad=3)
+
+    def mild(t):
+        return torch.where(t.abs() < 1e30, t, torch.zeros_like(t))
+
+    def spoil(t):
+        t = t.clone()
+        r, c = t.shape
+        t[3, 5], t[33, 1], t[r - 1, 0], t[40, 2], t[40, 7] = inf, -inf, nan, inf, -inf
+        t[64 % r, c - 1] = big                                # rounds to infinity in 8 bits
+        t[50, :] = 0
+        return t
+    xs, ps, ws = spoil(x), spoil(p), w.clone()
+    ws[:, 6] = 0                                              # inf * 0
+    ws[:, 8] = 0
+    ws[4, 8], ws[2, 9 % n], ws[k - 1, n - 1] = 100.0, inf, -big
+    for c in (w, ws):
+        _like_ieee(spmm_cpp.linear(xs, c, b), spmm_cpp.linear(mild(xs), mild(c), b), xs, c, b)
+    _like_ieee(spmm_cpp.linear_grad_input(ps, w), spmm_cpp.linear_grad_input(mild(ps), w), ps, w.t())
+    one = xs[:, 8:9]
+    _like_ieee(spmm_cpp.linear_grad_weight(one, p), spmm_cpp.linear_grad_weight(mild(one), p), one.t(), p)
+
+
+@pytest.mark.parametrize('m,k,n', [(65600, 70, 41), (65700, 140, 20), (66000, 33, 100)])
+def test_fp32_weight_gradients_of_many_rows_that_are_not_finite(m, k, n):
+    inf = float('inf')
+    x, _, _, _, p = _inputs(m, k, n, 'f32', False, False, 32, pad=1)
+    xs, ps = x.clone(), p.clone()
+    xs[70, 3], xs[40000, 3], xs[m - 1, 7], xs[12, 11], xs[5, 20], xs[9, 32] = inf, inf, -inf, float('nan'), 3.4e38, 3.0e38
+    ps[70, :] = ps[70, :].abs() + 1
+    ps[40000, :] = ps[40000, :].abs() + 1
+    ps[40000, 5] = -1.0                                       # inf - inf where row 70 and this one meet
+    ps[m - 1, 9] = 0.0                                        # inf * 0
+    ps[9, :] *= 100                                           # past fp32's range
+    ps[33, 15] = inf
+    mild = [torch.where(t.abs() < 1e30, t, torch.zeros_like(t)) for t in (xs, ps)]
+    _like_ieee(spmm_cpp.linear_grad_weight(xs, ps), spmm_cpp.linear_grad_weight(*mild), xs.t(), ps)
+
+
+def test_infinity_times_the_smallest_numbers():
+    """An infinity times a number below the normal ones is an infinity."""
+    for m in (70, 4230):
+        x, w, _, _, _ = _inputs(m, 130, 70, 'f32', False, False, 33)
+        x[5, 3], w[3, :] = float('inf'), 1e-40
+        w[3, 1] = -1e-42
+        y = spmm_cpp.linear(x, w)[5]
+        assert float(y[1]) == -float('inf') and bool((torch.cat([y[:1], y[2:]]) == float('inf')).all())
