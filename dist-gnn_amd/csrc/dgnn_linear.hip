@@ -153,12 +153,14 @@ __global__ __launch_bounds__(256) void slab_join_kernel(const double* __restrict
 }
 
 // ---------------------------------------------------------------------------------------
-// The whole backward pass of a small layer (M N <= 4096) in one launch, where the launches are what it costs: a workgroup
+// The whole backward pass of a small layer (small_fit below) in one launch, where the launches are what it costs: a workgroup
 // computes p = dy act'(x W + b) into LDS, in fp32 and for itself, and gives the gradients of `chunk` columns of x: their rows
 // of dw = x^T p, their columns of dx = p W^T; the first workgroup adds p's columns up. Plain fused multiply-adds in fp32: few
 // products average over few roundings, so p is not rounded to 16 bits here as it is on the way to the matrix cores.
 // ---------------------------------------------------------------------------------------
 constexpr int kSmall = 4096;
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Small {
   const void *x, *w, *dy, *save;
@@ -209,16 +211,23 @@ __global__ __launch_bounds__(256) void small_backward_kernel(const Small g) {
     small_sums<double>(N, M, [&](int n, int m, double t) { return t + p[m * N + n]; }, [&](int n, double t) { ((T*)g.db)[n] = (T)(float)t; });
 }
 
-// M N is what p takes of LDS; K N / 4096 workgroups each compute it, so that a large W is left to the launches of its own
-// (8 x 4096 x 512 fp32 51 us, both host-bound, with separate launches 62; 1 x 4096 x 4096 bf16 125 us, with separate launches 62).
+// Columns of x a workgroup takes: p, x's and W's parts each have 4096 floats of LDS.
+int64_t small_chunk(int64_t M, int64_t N) {
+  const int64_t side = M > N ? M : N;
+  return side <= kSmall / 16 ? 16 : kSmall / side;
+}
+
+// Each workgroup computes all of p for its own few columns, so what bounds the rule is that repeated work: p's values, and the
+// workgroups, at most two a compute unit. With tall or wide p the columns are so few that x is read in pieces of 4 to 16 bytes
+// a row. One launch against separate ones, gelu: fp32 8 x 1024 x 64 8.5, 19.2 us; 64 x 2048 x 32 19.6, 21.6; 1024 x 2048 x 4
+// 33.6, 35.2; beyond the values 64 x 64 x 64 33.4, 23.6; 256 x 1024 x 16 37.2, 29.0; bf16 8 x 256 x 512 26.6, 23.8; beyond the
+// workgroups fp32 1024 x 4096 x 1 46.0, 40.9; 4096 x 1024 x 1 74.6, 43.0; 4096 x 4096 x 1 289, 81; bf16 217, 58.
 bool small_fit(int64_t M, int64_t K, int64_t N) {
-  return M > 0 && N > 0 && K > 0 && M <= kSmall && N <= kSmall && M * N <= kSmall && K * N <= (1 << 22);
+  return M > 0 && N > 0 && K > 0 && M <= kSmall && N <= kSmall && M * N <= (N <= 4 ? kSmall : kSmall / 2) && ceil_div(K, small_chunk(M, N)) <= 512;
 }
 
 // ---------------------------------------------------------------------------------------
 constexpr int64_t kCompute = 256;              // compute units
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // A product whose output tiles do not fill the compute units is cut along its contraction, at 128 elements a slice or more:
 // for one workgroup a unit in any case, for as many as fit while the partial sums weigh less than half the operands (x^T p of
@@ -508,7 +517,7 @@ int dgnn_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
     return dgnn_fail(DGNN_E_BADARG, "linear_backward: an output overlaps another operand%s");
   if (small_fit(M, K, N)) {
     if (!dx && !dw && !dbias) return DGNN_OK;
-    const int64_t side = M > N ? M : N, chunk = kSmall / side < 1 ? 1 : kSmall / side < 16 ? kSmall / side : 16;
+    const int64_t chunk = small_chunk(M, N);
     const Small g{x, w, dy, save, dx, dw, dbias, ldx, ldw, ldd, lds, lddx, lddw, (int)M, (int)K, (int)N, (int)act, (int)chunk};
     const dim3 grid(dx || dw ? (uint32_t)ceil_div(K, chunk) : 1);
     hipStream_t s = (hipStream_t)stream;

@@ -156,3 +156,15 @@ def test_values_that_are_stored_negated_are_refused():
     assert z.is_neg()
     with pytest.raises(RuntimeError, match='resolve_neg'):
         spmm_cpp.linear(z, torch.zeros(1, 5))
+
+
+def test_small_backward_passes_are_bounded_by_what_they_repeat():
+    """A backward pass without workspace is the one that runs in one launch, whose workgroups each compute all of p. It has to
+    stop where p or the workgroups get many: tall, narrow layers once took it with a workgroup for each column of x."""
+    n = ctypes.c_int64()
+
+    def one(M, K, N):
+        assert lib.dgnn_linear_backward_workspace(M, K, N, 0, 2, ctypes.byref(n)) == 0
+        return n.value == 0
+    assert all(one(*s) for s in ((1, 602, 256), (8, 4096, 16), (64, 1433, 16), (1024, 256, 4), (1, 1, 1)))
+    assert not any(one(*s) for s in ((4096, 1024, 1), (4096, 4096, 1), (1024, 4096, 1), (2048, 1500, 2), (64, 64, 64), (256, 100, 16), (8, 602, 512), (1, 4096, 4096)))

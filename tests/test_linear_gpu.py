@@ -574,3 +574,14 @@ def test_infinity_times_the_smallest_numbers():
         w[3, 1] = -1e-42
         y = spmm_cpp.linear(x, w)[5]
         assert float(y[1]) == -float('inf') and bool((torch.cat([y[:1], y[2:]]) == float('inf')).all())
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+@pytest.mark.parametrize('m,k,n', [(4096, 1024, 1), (1024, 2050, 3), (4096, 250, 1), (2048, 500, 1), (1000, 2048, 4), (2049, 33, 1), (128, 70, 16), (129, 70, 16), (3, 600, 700)])
+def test_gradients_of_tall_narrow_layers(m, k, n, dtype):
+    """On both sides of the rule for backward passes in one launch."""
+    for act, pad in (('gelu', 0), ('relu', 3), ('none', 1)):
+        case = _inputs(m, k, n, dtype, True, act == 'relu', seed=m + k, pad=pad)
+        want = _definition(*case, dtype, act)
+        for name, got in _run(*case, act).items():
+            _near(got, *want[name], f'{act} {name}')
