@@ -22,6 +22,7 @@ Differences from the reference, on purpose:
 import ctypes
 import math
 import os
+import threading
 
 import torch
 
@@ -1465,22 +1466,43 @@ def _dense_for(A):
 
 
 # --------------------------------------------------------------------------- what a training step computes beside the aggregation
-def _load_torch_binding():
-    """lib/_dgnn_torch.so: the host side of the training operators over the same library."""
-    import importlib.util
-    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), '..', 'lib', '_dgnn_torch.so')
-    if not os.path.exists(path):
-        raise RuntimeError(f'spmm_cpp: {os.path.normpath(path)} is missing -- build it with '
-                           '`python -c "import __graft_entry__ as g; g.build()"`. There is no fallback.')
-    spec = importlib.util.spec_from_file_location('_dgnn_torch', path)
-    ext = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(ext)
-    ext.bind([ctypes.cast(getattr(_lib, n), ctypes.c_void_p).value for n in
-              ('dgnn_last_error', 'dgnn_linear_workspace', 'dgnn_linear_forward', 'dgnn_linear_slope', 'dgnn_linear_grad_input',
-               'dgnn_linear_grad_weight', 'dgnn_linear_backward_workspace', 'dgnn_linear_backward', 'dgnn_adamw')])
-    return ext
+_TORCH_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), '..', 'lib', '_dgnn_torch.so')
 
 
-_ext = _load_torch_binding()
+class _TorchBinding:
+    """lib/_dgnn_torch.so: the host side of the training operators over the same library, loaded at their first use. Unlike the
+    library it is built for one version of torch; callers of the SpMM alone do not need it."""
+
+    def __init__(self):
+        self._lock = threading.Lock()
+
+    def __getattr__(self, name):              # only until the binding is there
+        with self._lock:
+            if 'bind' not in self.__dict__:
+                self.__dict__.update(self._load())
+        if name not in self.__dict__:
+            raise AttributeError(name)
+        return self.__dict__[name]
+
+    @staticmethod
+    def _load():
+        import importlib.util
+        path = os.path.normpath(_TORCH_LIB_PATH)
+        rebuild = 'build it with `python -c "import __graft_entry__ as g; g.build()"`. There is no fallback.'
+        if not os.path.exists(_TORCH_LIB_PATH):
+            raise RuntimeError(f'spmm_cpp: {path} is missing -- {rebuild}')
+        try:
+            spec = importlib.util.spec_from_file_location('_dgnn_torch', _TORCH_LIB_PATH)
+            ext = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(ext)
+        except ImportError as e:
+            raise RuntimeError(f'spmm_cpp: {path} does not load ({e}); it is built for one version of torch -- {rebuild}') from e
+        ext.bind([ctypes.cast(getattr(_lib, n), ctypes.c_void_p).value for n in
+                  ('dgnn_last_error', 'dgnn_linear_workspace', 'dgnn_linear_forward', 'dgnn_linear_slope', 'dgnn_linear_grad_input',
+                   'dgnn_linear_grad_weight', 'dgnn_linear_backward_workspace', 'dgnn_linear_backward', 'dgnn_adamw')])
+        return {n: getattr(ext, n) for n in dir(ext) if not n.startswith('__')}
+
+
+_ext = _TorchBinding()
 from .adamw import AdamW  # noqa: E402,F401
 from .linear import ACTIVATIONS, linear, linear_forward, linear_grad_input, linear_grad_weight, linear_slope  # noqa: E402,F401
