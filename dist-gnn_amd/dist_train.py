@@ -65,8 +65,10 @@ def build_model(g, env, model='GCN', hidden_dim=256, num_layers=3, rep=2, bias=F
 
 def build_optimizer(params, optimizer='adam', lr=0.01, weight_decay=0.0):
     """'adam': the reference's torch.optim.Adam (dist_train.py:32); 'adamw' / 'adamw8': spmm_cpp.AdamW, one pass a step, with
-    moments in 32 or 8 bits. Every rank steps its own copy; sums are in a fixed order and the 8-bit rounding depends on element
-    and step alone, so copies stay equal."""
+    moments in 32 or 8 bits. ``weight_decay`` is Adam's own with 'adam' (added to the gradient, so the moments carry it) and
+    decoupled with the others (the weight shrinks by lr weight_decay a step): the same number is not the same decay. Every rank
+    steps its own copy; sums are in a fixed order and the 8-bit rounding depends on element and step alone, so copies stay
+    equal."""
     if optimizer == 'adam':
         return torch.optim.Adam(params, lr=lr, weight_decay=weight_decay)
     if optimizer in ('adamw', 'adamw8'):

@@ -38,8 +38,10 @@ def parse_args(argv=None):
     ap.add_argument('--hidden', type=int, default=256)
     ap.add_argument('--layers', type=int, default=3)
     ap.add_argument('--lr', type=float, default=0.01)
-    ap.add_argument('--optimizer', type=str, default='adam', choices=['adam', 'adamw', 'adamw8'])
-    ap.add_argument('--weight-decay', type=float, default=0.0)
+    ap.add_argument('--optimizer', type=str, default='adam', choices=['adam', 'adamw', 'adamw8'],
+                    help='adam: torch.optim.Adam; adamw, adamw8: spmm_cpp.AdamW with moments in 32 or 8 bits')
+    ap.add_argument('--weight-decay', type=float, default=0.0,
+                    help='adam: added to the gradient; adamw, adamw8: decoupled, the weight shrinks by lr * weight_decay a step')
     ap.add_argument('--bias', action='store_true')
     ap.add_argument('--activation', type=str, default='relu', choices=['none', 'relu', 'gelu', 'silu'])
     ap.add_argument('--skip', action='store_true')
