@@ -179,3 +179,34 @@ def test_options_are_checked():
     args = main.parse_args(['--optimizer', 'adamw8', '--skip', '--bias', '--activation', 'gelu', '--weight-decay', '0.1'])
     assert args.optimizer == 'adamw8' and args.skip and args.bias and args.activation == 'gelu' and args.weight_decay == 0.1
     assert main.parse_args([]).optimizer == 'adam' and not main.parse_args([]).bias
+
+
+def scenario_gradients(env, rank, world, gold_dir):
+    import coo_graph
+    import dist_train
+    gold = np.load(os.path.join(gold_dir, 'tiny_graph.npz'))
+    full = coo_graph.COO_Graph('tiny', attr_dict=_raw(gold))
+    out = {}
+    for model, blocks, block in (('GCN', world, rank), ('GCN15D', world // 2, rank // 2)):
+        if model == 'GCN15D' and world % 4:
+            continue
+        g = coo_graph.Parted_COO_Graph('tiny', block, blocks, attr_dict=full.partition(blocks, save=False)[block])
+        net = dist_train.build_model(g, env, model, hidden_dim=8, num_layers=3, bias=True, activation='gelu', skip=True)
+        with torch.no_grad():
+            for p in net.parameters():
+                p.sub_(0.4)
+        dist_train.train_step(net, torch.optim.SGD(net.parameters(), lr=0.01), lambda o, t: (torch.nn.functional.cross_entropy(o, t, reduction='sum') / 40), g, env)
+        out[model] = {n: p.grad.double().numpy() for n, p in net.named_parameters()}
+    return out
+
+
+def test_gradients_do_not_depend_on_the_ranks(tmp_path):
+    """The gradients themselves, before an optimiser makes steps of its own size of them: fp32 sums in another order, 1e-5 of the
+    largest value."""
+    one, four = _run(1, 'gradients', str(tmp_path))[0]['GCN'], _run(4, 'gradients', str(tmp_path))
+    for res in four.values():
+        assert set(res) == {'GCN', 'GCN15D'}
+        for model in res:
+            for name, want in one.items():
+                assert np.abs(want).max() > 0
+                assert np.abs(res[model][name] - want).max() <= 1e-5 * np.abs(want).max(), (model, name)
