@@ -585,3 +585,33 @@ def test_gradients_of_tall_narrow_layers(m, k, n, dtype):
         want = _definition(*case, dtype, act)
         for name, got in _run(*case, act).items():
             _near(got, *want[name], f'{act} {name}')
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+@pytest.mark.parametrize('m,k,n', [(4227, 203, 70), (12300, 40, 256), (33000, 520, 130), (65600, 16, 97)])
+def test_relu_over_several_words_of_saved_bits(m, k, n, dtype):
+    """Rows enough for the kernel that takes them straight from memory, more columns than one word, ragged or not."""
+    case = _inputs(m, k, n, dtype, True, n == 256, seed=41, pad=3)
+    want = _definition(*case, dtype, 'relu')
+    for name, got in _run(*case, 'relu').items():
+        _near(got, *want[name], f'relu {name}')
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+@pytest.mark.parametrize('m,k,n', [(1, 602, 256), (8, 100, 64), (64, 1433, 16), (33, 40, 31), (1024, 64, 2), (5, 3, 4)])
+def test_small_16_bit_layers_round_their_gradients_once(m, k, n, dtype):
+    """A backward pass in one launch keeps p = dy act'(x W + b) in fp32 (sizes of small_fit): its gradients carry their own
+    rounding and what fp32 arithmetic loses, not p's 16 bits."""
+    for act in ('gelu', 'silu'):
+        x, w, b, _, dy = case = _inputs(m, k, n, dtype, True, False, seed=42)
+        got = _run(*case, act)
+        h, tiny = HALF[dtype], 2.0 ** -25 if dtype == 'f16' else 0
+        x, w, b, dy = map(_d, (x, w, b, dy))
+        pre, size = x @ w + b, x.abs() @ w.abs() + b.abs()
+        e_pre = _sum_bound(k, dtype) * size + U * pre.abs()
+        p = dy * _act(pre, act)[1]
+        # act's 16-bit evaluation: a tail of 1e-6 relative error and the operations around it, within 32 U of the slope's terms
+        e_p = dy.abs() * (0.8 * (U * pre.abs() + 2 * e_pre) + 32 * U * (1 + pre.abs()))
+        for name, a, c, e, count in (('dx', p, w.t(), e_p @ w.abs().t(), n), ('dw', x.t(), p, x.abs().t() @ e_p, m)):
+            v = a @ c
+            _near(got[name], v, e + _sum_bound(count, 'f32') * (a.abs() @ c.abs() + e) + h * v.abs() + 1e-40 + tiny, f'{act} {name}')
