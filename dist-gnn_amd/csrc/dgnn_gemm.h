@@ -42,7 +42,7 @@ struct Gemm {
   int act;
   float* partial;          // slices x M x N when slices > 1
   int slices;
-  int64_t slice_k;         // contraction elements a slice takes, a multiple of 64
+  int64_t slice_k;         // contraction elements a slice takes, a multiple of 32 (of 64 by tiles)
   char* image;             // room for W's image where the product runs on rows_kernel, else null
   hipStream_t stream;
 };
@@ -953,7 +953,7 @@ __global__ __launch_bounds__(WAVES * 64, R == 2 ? 2 : TN == 4 ? 3 : 4) void rows
   each<0, R>([&](auto r) __attribute__((always_inline)) { v[r].finish(g, row + 32 * r, nt * V::BN, half); });
 }
 
-// Columns a wave takes: all of a narrow output, else 256.
+// Columns a wave takes: all of a narrow output, else 128.
 inline int rows_bn(int64_t N) { return N <= 32 ? 32 : N <= 64 ? 64 : 128; }
 
 // Bytes of W's image.
@@ -1021,7 +1021,7 @@ template <int BN> struct Turn {                               // BN columns of 3
   int col;
   bool pair;
 
-  // p: the tile's first column of row 0, `cols` columns from there on. A lane's distance from its row's start is 32 bits, the
+  // `cols`: p's columns. A lane's distance from its row's start is 32 bits, the
   // rows' starts are the workgroup's: addresses cost scalar registers. A lane past the columns reads the first ones (its sums
   // are not kept); a pair that ends past them reads on into the next row, or is two loads where none follows
   __device__ __forceinline__ void begin(int64_t ld, int64_t cols, int tid) {
@@ -1073,14 +1073,14 @@ __global__ __launch_bounds__(256, 3) void columns_kernel(const Gemm g) {
   __shared__ __attribute__((aligned(16))) char even[B::STAGE];
   __shared__ __attribute__((aligned(16))) char odd[B::STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  const int64_t tiles_m = (g.M + BM - 1) / BM, tiles_n = (g.N + BN - 1) / BN, tiles = tiles_m * tiles_n;
+  const int64_t tiles = (g.M + BM - 1) / BM;
   int64_t tile = blockIdx.x % tiles, slice = blockIdx.x / tiles;
   if (g.slices >= 8) {                                         // consecutive workgroups go round the 8 XCDs
     tile = blockIdx.x / 8 % tiles;
     slice = blockIdx.x / 8 / tiles * 8 + blockIdx.x % 8;
     if (slice >= g.slices) return;
   }
-  const int64_t row0 = tile / tiles_n * BM + wave * 32, col0 = tile % tiles_n * BN;           // of the output
+  const int64_t row0 = tile * BM + wave * 32;                  // of the output, whose columns are one tile
   const int64_t kbeg = slice * g.slice_k, kend = kbeg + g.slice_k < g.K ? kbeg + g.slice_k : g.K;
   const float* const x = (const float*)g.a;
   const float* const p = (const float*)g.b;
@@ -1103,9 +1103,9 @@ __global__ __launch_bounds__(256, 3) void columns_kernel(const Gemm g) {
       }
   };
   B b;
-  b.begin(g.ldb, g.N - col0, tid);
+  b.begin(g.ldb, g.N, tid);
   if (kbeg < kend) {
-    b.fetch(p + col0, g.ldb, kbeg, kend, g.K, tid);
+    b.fetch(p, g.ldb, kbeg, kend, g.K, tid);
     fetch_x(kbeg, cur);
     b.store(even, tid);
   }
@@ -1113,7 +1113,7 @@ __global__ __launch_bounds__(256, 3) void columns_kernel(const Gemm g) {
   auto step = [&](int64_t k, const char* from, char* to) __attribute__((always_inline)) {
     const bool more = k + BK < kend;
     if (more) {
-      b.fetch(p + col0, g.ldb, k + BK, kend, g.K, tid);
+      b.fetch(p, g.ldb, k + BK, kend, g.K, tid);
       fetch_x(k + BK, next);
     }
 #pragma unroll
@@ -1147,7 +1147,7 @@ __global__ __launch_bounds__(256, 3) void columns_kernel(const Gemm g) {
   }
 
   each<0, TN>([&](auto j) __attribute__((always_inline)) {
-    const int64_t col = col0 + j * 32 + (lane & 31);
+    const int64_t col = j * 32 + (lane & 31);
     if (__ballot(col < g.N && !(unsound(acc[j]) == 0.f)))
       again(acc[j], f16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}, x + (mine < g.M ? mine : g.M - 1), g.lda, p + (col < g.N ? col : g.N - 1), g.ldb, kbeg, kend);
 #pragma unroll
