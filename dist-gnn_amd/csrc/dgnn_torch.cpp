@@ -8,6 +8,7 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <stdexcept>
@@ -330,6 +331,15 @@ struct AdamTable {
   }
 };
 
+// whether two sequences hold the same objects (comparing tensors would compare their elements)
+bool same_objects(const py::object& a, const py::object& b) {
+  const auto x = py::reinterpret_steal<py::object>(PySequence_Fast(a.ptr(), "AdamW: a sequence of parameters")),
+             y = py::reinterpret_steal<py::object>(PySequence_Fast(b.ptr(), "AdamW: a sequence of parameters"));
+  if (!x || !y) throw py::error_already_set();
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(x.ptr());
+  return n == PySequence_Fast_GET_SIZE(y.ptr()) && std::equal(PySequence_Fast_ITEMS(x.ptr()), PySequence_Fast_ITEMS(x.ptr()) + n, PySequence_Fast_ITEMS(y.ptr()));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -339,6 +349,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_slope", &linear_slope);
   m.def("linear_grad_input", &linear_grad_input);
   m.def("linear_grad_weight", &linear_grad_weight);
+  m.def("same_objects", &same_objects);
   py::class_<AdamTable>(m, "AdamTable")
       .def(py::init<const std::vector<Tensor>&, const std::vector<int64_t>&, int, const Tensor&, const Tensor&, const MaybeTensor&, const MaybeTensor&,
                     const MaybeTensor&, const Tensor&, const MaybeTensor&>())

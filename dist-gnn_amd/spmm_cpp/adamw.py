@@ -5,7 +5,6 @@ parameter. Here a step is one pass over parameter, gradient and moments, for up 
 in 32 or in 8 bits.
 """
 import math
-import operator
 
 import numpy as np
 import torch
@@ -140,9 +139,16 @@ class AdamW(torch.optim.Optimizer):
             if a[0] == b[0] and b[1] < a[2]:
                 raise RuntimeError('AdamW: two parameters overlap in memory')
 
+    def _current(self):
+        """Whether param_groups hold the parameters that state was made for."""
+        return (self._segments is not None and len(self._known) == len(self.param_groups)
+                and all(_ext.same_objects(known, g['params']) for known, g in zip(self._known, self.param_groups)))
+
     @torch.no_grad()
     def init_state(self):
         """Allocates the state of parameters that have none yet (zeros; a master takes its parameter's value)."""
+        if self._current():
+            return
         if self._segments is None:
             self._segments, self._known = [[] for _ in self.param_groups], []
             given = {p: s for p, s in self.state.items() if s}
@@ -259,8 +265,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if self._segments is None or len(self._known) != len(self.param_groups) or not all(
-                len(known) == len(g['params']) and all(map(operator.is_, known, g['params'])) for known, g in zip(self._known, self.param_groups)):
+        if not self._current():
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError('AdamW: take a step or call init_state() before capturing one in a graph')
             self.init_state()
