@@ -889,9 +889,12 @@ template <typename T, int TN> struct Wave {
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
-// fp32 232965 x 602 x 256 403 us, 178 TFLOP/s of fp32 products (1070 of bf16 ones), bound by the matrix cores; bf16 65536 x 1024 x
+// fp32 232965 x 602 x 256 393 to 436 us, 165 to 183 TFLOP/s of fp32 products (990 to 1100 of bf16 ones), bound by the matrix cores,
+// whose clock follows the data (357 us with x all zero, 393 half zero, 436 with none); bf16 65536 x 1024 x
 // 512 87 us, 790 TFLOP/s, 8192 x 1024 x 4096 103, 665, bound by LDS reads and the barrier of each stage; 2449029 x 256 x 256 with
 // a residual 1073 us, 3.5 TB/s: its rows are written in 32-byte pieces.
+// With 128 columns fp32 takes all 168 registers of three waves a SIMD; its epilogue keeps up to 48 bytes a lane in scratch where the
+// residual's pieces wait, the loop over stages none.
 // W's stages go round two buffers in LDS, copied there by the memory unit itself while the stage before is multiplied; each
 // buffer is an array of its own, so that the compiler sees that a copy into one does not touch the reads of the other.
 template <typename T, int TN, int WAVES, int R>

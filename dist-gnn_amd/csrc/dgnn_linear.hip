@@ -12,7 +12,7 @@ using namespace dgnn;
 
 // ---------------------------------------------------------------------------------------
 // p = dy act'(x W + b) and the sums of p's columns. Reads dy and what the forward pass saved once and writes p once, which is
-// what bounds it: 232965 x 256 fp32 gelu 152 us, 716 MB, 4.7 TB/s; 8192 x 4096 bf16 gelu 65 us, 268 MB, 4.1 TB/s. A row is taken
+// what bounds it: 232965 x 256 fp32 gelu 152 to 171 us, 716 MB, 4.2 to 4.7 TB/s; 8192 x 4096 bf16 gelu 65 us, 268 MB, 4.1 TB/s. A row is taken
 // by the fewest lanes (a power of two) that cover it with 4 columns each, 64 at most, so narrow rows fill a wave too; a lane
 // keeps its columns' sums over the block's rows, in 64 bits (sums over every node cancel), the block adds its lanes in a fixed
 // order and a second launch adds the blocks': no atomics, the same bits every run. Of 16-bit types p is rounded to the type, which
