@@ -40,8 +40,9 @@ struct Gemm {
   void* save;
   int64_t ld_save;
   int act;
-  float* partial;          // slices x M x N when slices > 1
+  float* partial;          // slices x M x N when slices > 1 (x 2 N with `pieces`, however many slices)
   int slices;
+  bool pieces;             // b is M rows of 2 N values, each second N what rounding left of the first: c = a (first + second)
   int64_t slice_k;         // contraction elements a slice takes, a multiple of 32 (of 64 by tiles)
   char* image;             // room for W's image where the product runs on rows_kernel, else null
   hipStream_t stream;
@@ -390,7 +391,7 @@ __device__ __forceinline__ void epilogue(const Gemm& g, f16v (&acc)[TM][TN], flo
   const int lane = threadIdx.x & 63;
   const int64_t col = col0 + (lane % LANES) * 4;
   const int have_n = g.N - col >= 4 ? 4 : (g.N > col ? (int)(g.N - col) : 0);
-  const bool whole = g.slices == 1;
+  const bool whole = g.slices == 1 && !g.pieces;
   float bias[4] = {0.f, 0.f, 0.f, 0.f};
   if (whole && g.bias) load4((const T*)g.bias + col, have_n, bias);
   if constexpr (Unit<T>::PLANES == 3) {
@@ -570,6 +571,56 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const Gemm g) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = (float)sum[i];
   finish<T>(g, row, col, have, v, bias, res);
+}
+
+// The same for a product whose right operand came in two pieces: a four of columns adds its own sums and those of the second
+// pieces, N columns on. Where that is not finite the first pieces' sums alone stand, which are the product with p rounded to
+// 16 bits: an infinity times two pieces of opposite signs would be NaN.
+template <typename T>
+__global__ __launch_bounds__(256) void pieces_join_kernel(const Gemm g) {
+  constexpr int PARTS = 8, FOURS = 256 / PARTS;
+  __shared__ double sums[PARTS][FOURS][8];
+  const int four = threadIdx.x % FOURS, part = threadIdx.x / FOURS;
+  const int64_t wide = (g.N + 3) / 4, at = (int64_t)blockIdx.x * FOURS + four, row = at / wide, col = at % wide * 4;
+  const int have = row < g.M ? (g.N - col >= 4 ? 4 : (int)(g.N - col)) : 0;
+  double sum[8] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
+  if (have) {
+    const float* p = g.partial + row * 2 * g.N + col;
+    const int64_t step = g.M * 2 * g.N;
+    for (int s = part; s < g.slices; s += 4 * PARTS) {
+      float t[4][8];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (s + PARTS * u < g.slices) {
+          float first[4], second[4];
+          load4(p + (s + PARTS * u) * step, have, first);
+          load4(p + (s + PARTS * u) * step + g.N, have, second);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { t[u][i] = first[i]; t[u][4 + i] = second[i]; }
+        }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (s + PARTS * u < g.slices) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[i] += t[u][i];
+        }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sums[part][four][i] = sum[i];
+  __syncthreads();
+  if (part || !have) return;
+#pragma unroll
+  for (int k = 1; k < PARTS; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += sums[k][four][i];
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const double both = sum[i] + sum[4 + i];
+    v[i] = (float)(fabs(both) < __builtin_huge_val() ? both : sum[i]);
+  }
+  store4((T*)g.c + row * g.ldc + col, have, v);
 }
 
 template <typename T> void join(const Gemm& g) {
@@ -1430,15 +1481,36 @@ int gemm_launch(const Gemm& g) {
       break;
   }
   DGNN_LAUNCHED();
-  if (g.slices > 1) {
+  if (g.slices > 1 && !g.pieces) {
     join<T>(g);
     DGNN_LAUNCHED();
   }
   return DGNN_OK;
 }
 
+// What gemm_kernel multiplies where b comes in two pieces.
+inline Gemm both_pieces(const Gemm& g) {
+  Gemm wide = g;
+  wide.N = 2 * g.N;
+  return wide;
+}
+
+template <typename T>
+int pieces_launch(const Gemm& g) {
+  const int rc = gemm_launch<T, false, false>(both_pieces(g));
+  if (rc != DGNN_OK) return rc;
+  const int64_t fours = g.M * ((g.N + 3) / 4);
+  hipLaunchKernelGGL((pieces_join_kernel<T>), dim3((uint32_t)((fours + 31) / 32)), dim3(256), 0, g.stream, g);
+  DGNN_LAUNCHED();
+  return DGNN_OK;
+}
+
+
 template <typename T>
 int gemm_typed(const Gemm& g) {
+  if constexpr (sizeof(T) == 2) {
+    if (g.pieces) return pieces_launch<T>(g);
+  }
   if (thin_fit<T>(g)) {
     if (g.M == 1) return thin_launch<T, 1>(g);
     if (g.M == 2) return thin_launch<T, 2>(g);

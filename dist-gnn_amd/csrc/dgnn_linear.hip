@@ -12,19 +12,20 @@ using namespace dgnn;
 
 // ---------------------------------------------------------------------------------------
 // p = dy act'(x W + b) and the sums of p's columns. Reads dy and what the forward pass saved once and writes p once, which is
-// what bounds it: 232965 x 256 fp32 gelu 152 to 171 us, 716 MB, 4.2 to 4.7 TB/s; 8192 x 4096 bf16 gelu 65 us, 268 MB, 4.1 TB/s. A row is taken
-// by the fewest lanes (a power of two) that cover it with 4 columns each, 64 at most, so narrow rows fill a wave too; a lane
-// keeps its columns' sums over the block's rows, in 64 bits (sums over every node cancel), the block adds its lanes in a fixed
-// order and a second launch adds the blocks': no atomics, the same bits every run. Of 16-bit types p is rounded to the type, which
-// is what the matrix cores take: dx and dw then carry p's rounding and their own, where p in two pieces would carry only theirs
-// and cost each gradient product twice. Against 64 bits that is 1.4 times the error of their own rounding alone (2^-9 a value for
-// bf16), more where a gradient is a sum of a few values.
+// what bounds it: 232965 x 256 fp32 gelu 152 to 171 us, 716 MB, 4.2 to 4.7 TB/s; 8192 x 4096 bf16 gelu 65 us, 268 MB, 4.1
+// TB/s. A row is taken by the fewest lanes (a power of two) that cover it with 4 columns each, 64 at most, so narrow rows fill a
+// wave too; a lane keeps its columns' sums over the block's rows, in 64 bits (sums over every node cancel), the block adds its
+// lanes in a fixed order and a second launch adds the blocks': no atomics, the same bits every run. Of 16-bit types p is rounded to
+// the type, which is what the matrix cores take: dx and dw then carry p's rounding and their own, 1.4 times the error of their own
+// alone (2^-9 a value for bf16). Where dw's would be more, it takes p in two pieces (takes_pieces below), the second of which is
+// written behind the row's first ones.
 // ---------------------------------------------------------------------------------------
 struct Slope {
   const void* dy;
   const void* save;
   void* p;
   int64_t ld_dy, ld_save, ld_p, M, N, slab;      // rows a block takes
+  int64_t second;                                // elements from a value of p to what its rounding left (0: not wanted)
   double* partial;                               // gridDim.y x N, or null
   int act, lanes;
 };
@@ -100,15 +101,14 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope g) {
         for (int i = 0; i < 4; ++i) sum[i] += v[k][i];
         if (g.p) {
           T* p = (T*)g.p + row * g.ld_p + col;
-          if (have == 4) {
-            quad q;
+          store4(p, have, v[k]);
+          if (sizeof(T) == 2 && g.second) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = (T)v[k][i];
-            *reinterpret_cast<quad*>(p) = q;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (i < have) p[i] = (T)v[k][i];
+            for (int i = 0; i < 4; ++i) {
+              const float first = (float)(T)v[k][i];
+              v[k][i] = fabsf(first) < __builtin_huge_valf() ? v[k][i] - first : 0.f;
+            }
+            store4(p + g.second, have, v[k]);
           }
         }
       }
@@ -312,6 +312,13 @@ bool saved_ok(const void* save, int64_t lds, int64_t M, int64_t N, int32_t act) 
 // How a product runs, by its sizes: a handful of rows on plain multiply-adds, over W's laid-out image where there are many rows,
 // else by tiles, cut along the contraction where those are few. Returns the bytes of workspace that takes.
 int64_t plan(Gemm& g, int32_t dtype) {
+  if (g.pieces) {
+    Gemm wide = both_pieces(g);
+    cut(wide, dtype);
+    g.slices = wide.slices;
+    g.slice_k = wide.slice_k;
+    return (int64_t)g.slices * g.M * wide.N * 4;
+  }
   if (dtype == DGNN_F32 ? thin_fit<float>(g) : thin_fit<_Float16>(g)) {
     if (dtype == DGNN_F32) thin_cut<float>(g); else thin_cut<_Float16>(g);
     return g.slices > 1 ? (int64_t)g.slices * g.M * g.N * 4 : 0;
@@ -330,6 +337,7 @@ int64_t plan(Gemm& g, int32_t dtype) {
 
 // whether a grid holds the output's tiles, where the product runs by tiles
 template <typename T> bool tiles_fit(const Gemm& g) {
+  if (g.pieces) return tiles_of(shape_of<T>(both_pieces(g)), g.M, 2 * g.N) < (1 << 23);
   return thin_fit<T>(g) || columns_fit<T>(g) || rows_fit(g) || tiles_of(shape_of<T>(g), g.M, g.N) < (1 << 23);
 }
 bool launch_fits(const Gemm& g, int32_t dtype) { return dtype == DGNN_F32 ? tiles_fit<float>(g) : tiles_fit<_Float16>(g); }
@@ -340,7 +348,7 @@ int run(const Gemm& g, int32_t dtype, void* workspace, int64_t bytes, const char
   const int64_t need = plan(h, dtype);
   if (need && (!workspace || bytes < need || (uintptr_t)workspace % 16))
     return dgnn_fail(DGNN_E_BADARG, "%s: workspace too small or misaligned (%lld bytes wanted)", who, (long long)need);
-  if (h.slices > 1) h.partial = (float*)workspace;
+  if (h.slices > 1 || h.pieces) h.partial = (float*)workspace;
   else if (need) h.image = (char*)workspace;
   if (dtype == DGNN_F32) return gemm_f32(h);
   if (dtype == DGNN_BF16) return gemm_bf16(h);
@@ -397,8 +405,8 @@ int dgnn_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, 
   return run(g, dtype, workspace, workspace_bytes, "linear_forward");
 }
 
-int dgnn_linear_slope(const void* dy, int64_t ldd, const void* save, int64_t lds, void* p, int64_t ldp, void* dbias,
-                      int64_t M, int64_t N, int32_t dtype, int32_t act, void* workspace, int64_t workspace_bytes, void* stream) {
+static int slope(const void* dy, int64_t ldd, const void* save, int64_t lds, void* p, int64_t ldp, int64_t second, void* dbias,
+                 int64_t M, int64_t N, int32_t dtype, int32_t act, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!known_type(dtype)) return dgnn_fail(DGNN_E_BADARG, "linear_slope: unknown type%s (%lld)", "", dtype);
   if (act < ACT_NONE || act > ACT_SILU) return dgnn_fail(DGNN_E_BADARG, "linear_slope: unknown activation%s (%lld)", "", act);
   if (!sizes_ok(M, 0, N)) return dgnn_fail(DGNN_E_BADARG, "linear_slope: bad sizes%s");
@@ -417,7 +425,7 @@ int dgnn_linear_slope(const void* dy, int64_t ldd, const void* save, int64_t lds
   if (dbias && slabs > 0 && (!workspace || workspace_bytes < slabs * N * 8 || (uintptr_t)workspace % 8))
     return dgnn_fail(DGNN_E_BADARG, "linear_slope: workspace too small%s (%lld bytes wanted)", "", slabs * N * 8);
   if (M > 0 && (p || dbias)) {
-    const Slope g{dy, save, p, ldd, lds, ldp, M, N, slab, dbias ? (double*)workspace : nullptr, act, (int)lanes};
+    const Slope g{dy, save, p, ldd, lds, ldp, M, N, slab, second, dbias ? (double*)workspace : nullptr, act, (int)lanes};
     const dim3 grid((uint32_t)ceil_div(N, 4 * lanes), (uint32_t)slabs);
     if (dtype == DGNN_F32) hipLaunchKernelGGL((slope_kernel<float>), grid, dim3(256), 0, s, g);
     else if (dtype == DGNN_BF16) hipLaunchKernelGGL((slope_kernel<__bf16>), grid, dim3(256), 0, s, g);
@@ -432,6 +440,11 @@ int dgnn_linear_slope(const void* dy, int64_t ldd, const void* save, int64_t lds
     DGNN_LAUNCHED();
   }
   return DGNN_OK;
+}
+
+int dgnn_linear_slope(const void* dy, int64_t ldd, const void* save, int64_t lds, void* p, int64_t ldp, void* dbias,
+                      int64_t M, int64_t N, int32_t dtype, int32_t act, void* workspace, int64_t workspace_bytes, void* stream) {
+  return slope(dy, ldd, save, lds, p, ldp, 0, dbias, M, N, dtype, act, workspace, workspace_bytes, stream);
 }
 
 int dgnn_linear_grad_input(const void* p, int64_t ldp, const void* w, int64_t ldw, const void* add, int64_t lda,
@@ -455,8 +468,8 @@ int dgnn_linear_grad_input(const void* p, int64_t ldp, const void* w, int64_t ld
   return run(g, dtype, workspace, workspace_bytes, "linear_grad_input");
 }
 
-int dgnn_linear_grad_weight(const void* x, int64_t ldx, const void* p, int64_t ldp, void* dw, int64_t ldw,
-                            int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+static int grad_weight(const void* x, int64_t ldx, const void* p, int64_t ldp, bool pieces, void* dw, int64_t ldw,
+                       int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!known_type(dtype)) return dgnn_fail(DGNN_E_BADARG, "linear_grad_weight: unknown type%s (%lld)", "", dtype);
   if (!sizes_ok(M, K, N)) return dgnn_fail(DGNN_E_BADARG, "linear_grad_weight: bad sizes%s");
   if (K == 0 || N == 0) return DGNN_OK;
@@ -470,14 +483,40 @@ int dgnn_linear_grad_weight(const void* x, int64_t ldx, const void* p, int64_t l
   g.b = p; g.ldb = ldp; g.b_along = false;
   g.M = K; g.N = N; g.K = M;
   g.c = dw; g.ldc = ldw;
+  g.pieces = pieces;
   g.stream = (hipStream_t)stream;
   return run(g, dtype, workspace, workspace_bytes, "linear_grad_weight");
 }
 
+int dgnn_linear_grad_weight(const void* x, int64_t ldx, const void* p, int64_t ldp, void* dw, int64_t ldw,
+                            int64_t M, int64_t K, int64_t N, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  return grad_weight(x, ldx, p, ldp, false, dw, ldw, M, K, N, dtype, workspace, workspace_bytes, stream);
+}
+
 // Everything a gradient dy of y gives, in one call: what the three entries above compute, in the same order on the stream, so
 // that one workspace serves them one after the other behind p's part of it.
+// Where p of gelu or silu is rounded to 16 bits, a narrow layer's weight gradient takes it in two pieces, the rounded value and
+// what that left: its few columns, or few values in all, average over few roundings (x behind an activation is positive, so all of
+// a column's sums share the errors of its p), and a product that is bound by its bytes has room for the second pieces. All
+// gradients of bf16 gelu with rounded p and with its pieces: 232965 x 256 x 41 135, 145 us; 232965 x 602 x 41 253, 242; 2449029 x
+// 128 x 47 717, 834; 2000000 x 4 x 4 633, 438. Few weights in many columns pay more once p leaves the caches (1000000 x 1 x 88 376,
+// 582), so they take the pieces up to 2^24 values of p only. The input gradient and wider weight gradients, whose error is 1.4
+// times that of their own rounding, take the rounded values.
+static bool takes_pieces(int64_t M, int64_t K, int64_t N, int32_t dtype, int32_t act) {
+  if (dtype == DGNN_F32 || act <= ACT_RELU || M == 0 || K == 0 || N == 0 || small_fit(M, K, N)) return false;
+  return N <= 64 ? K * N <= (1 << 20) : K * N <= 4096 && M * N <= (1 << 24);
+}
+
+static Gemm weight_product(int64_t M, int64_t K, int64_t N, bool pieces) {
+  Gemm g{};
+  g.M = K; g.N = N; g.K = M;
+  g.pieces = pieces;
+  return g;
+}
+
 static int64_t backward_parts(int64_t M, int64_t K, int64_t N, int32_t dtype, int32_t act, int64_t* p_bytes) {
   int64_t most = 0;
+  const bool pieces = takes_pieces(M, K, N, dtype, act);
   for (int32_t pass = DGNN_LINEAR_SLOPE; pass <= DGNN_LINEAR_GRAD_WEIGHT; ++pass) {
     int64_t n = 0;
     (void)dgnn_linear_workspace(pass, M, K, N, dtype, &n);
@@ -485,7 +524,12 @@ static int64_t backward_parts(int64_t M, int64_t K, int64_t N, int32_t dtype, in
   }
   *p_bytes = 0;
   if (small_fit(M, K, N)) return 0;
-  *p_bytes = act == ACT_NONE ? 0 : ceil_div(M * N * width(dtype), 256) * 256;
+  if (pieces) {
+    Gemm g = weight_product(M, K, N, true);
+    const int64_t n = plan(g, dtype);
+    if (n > most) most = n;
+  }
+  *p_bytes = act == ACT_NONE ? 0 : ceil_div(M * N * width(dtype) * (pieces ? 2 : 1), 256) * 256;
   return *p_bytes + most;
 }
 
@@ -527,24 +571,26 @@ int dgnn_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
     DGNN_LAUNCHED();
     return DGNN_OK;
   }
-  Gemm to_x{}, to_w{};
+  const bool pieces = dw && takes_pieces(M, K, N, dtype, act);
+  const int64_t pitch = pieces ? 2 * N : N;
+  Gemm to_x{}, to_w = weight_product(M, K, N, pieces);
   to_x.M = M; to_x.N = K; to_x.K = N; to_x.a_along = to_x.b_along = true;
-  to_w.M = K; to_w.N = N; to_w.K = M; to_w.lda = ldx; to_w.ldb = act == ACT_NONE ? ldd : N;
+  to_w.lda = ldx; to_w.ldb = act == ACT_NONE ? ldd : pitch;
   if ((dx && !launch_fits(to_x, dtype)) || (dw && !launch_fits(to_w, dtype))) return dgnn_fail(DGNN_E_BADARG, "linear_backward: too many tiles of output%s");
   char* rest = (char*)workspace + p_bytes;
   const void* p = dy;
   int64_t ldp = ldd;
   if (act != ACT_NONE || dbias) {
     void* to = act != ACT_NONE && M > 0 && N > 0 ? workspace : nullptr;
-    const int rc = dgnn_linear_slope(dy, ldd, save, lds, to, N, dbias, M, N, dtype, act, rest, need - p_bytes, stream);
+    const int rc = slope(dy, ldd, save, lds, to, pitch, pieces ? N : 0, dbias, M, N, dtype, act, rest, need - p_bytes, stream);
     if (rc != DGNN_OK) return rc;
-    if (act != ACT_NONE) { p = workspace; ldp = N; }
+    if (act != ACT_NONE) { p = workspace; ldp = pitch; }
   }
   if (dx) {
     const int rc = dgnn_linear_grad_input(p, ldp, w, ldw, nullptr, 0, dx, lddx, M, K, N, dtype, rest, need - p_bytes, stream);
     if (rc != DGNN_OK) return rc;
   }
-  return dw ? dgnn_linear_grad_weight(x, ldx, p, ldp, dw, lddw, M, K, N, dtype, rest, need - p_bytes, stream) : DGNN_OK;
+  return dw ? grad_weight(x, ldx, p, ldp, pieces, dw, lddw, M, K, N, dtype, rest, need - p_bytes, stream) : DGNN_OK;
 }
 
 }  // extern "C"

@@ -615,3 +615,51 @@ def test_small_16_bit_layers_round_their_gradients_once(m, k, n, dtype):
         for name, a, c, e, count in (('dx', p, w.t(), e_p @ w.abs().t(), n), ('dw', x.t(), p, x.abs().t() @ e_p, m)):
             v = a @ c
             _near(got[name], v, e + _sum_bound(count, 'f32') * (a.abs() @ c.abs() + e) + h * v.abs() + 1e-40 + tiny, f'{act} {name}')
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+@pytest.mark.parametrize('m,k,n', [(3000, 20, 3), (6030, 3054, 1), (2200, 1, 88), (700, 33, 64), (700, 33, 65), (20000, 602, 41), (65600, 3, 5), (9, 2, 1973), (33, 5000, 63), (500, 63, 65)])
+def test_narrow_16_bit_layers_round_their_weight_gradients_once(m, k, n, dtype):
+    """dw of layers of few columns, or of few weights, carries its own rounding, what fp32 sums lose and the rounding of p's second
+    16-bit piece, not that of p = dy act'(x W + b) itself. x positive, as behind an activation, so that nothing averages."""
+    for act, pad in (('gelu', 0), ('silu', 3)):
+        x, w, b, _, dy = case = _inputs(m, k, n, dtype, True, False, seed=51, pad=pad)
+        x.abs_()
+        got = _run(*case, act)
+        h, tiny = HALF[dtype], 2.0 ** -25 if dtype == 'f16' else 0
+        x, w, b, dy = map(_d, (x, w, b, dy))
+        pre, size = x @ w + b, x.abs() @ w.abs() + b.abs()
+        e_pre = _sum_bound(k, dtype) * size + U * pre.abs()
+        p = dy * _act(pre, act)[1]
+        e_p = dy.abs() * (0.8 * (U * pre.abs() + 2 * e_pre) + 32 * U * (1 + pre.abs()))
+        e_p = e_p + h * h * (p.abs() + e_p) + tiny
+        v, e = x.t() @ p, x.abs().t() @ e_p
+        _near(got['dw'], v, (e + _sum_bound(m, dtype) * 2 * (x.abs().t() @ p.abs() + e)) * (1 + h) + h * v.abs() + 1e-40 + tiny, f'{act} dw')
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+def test_narrow_16_bit_weight_gradients_that_are_not_finite(dtype):
+    """An infinity times p is an infinity of its sign, whatever p's two pieces are; NaN stays where it is."""
+    m, k, n = 4000, 12, 9
+    x, w, b, _, dy = _inputs(m, k, n, dtype, True, False, 52)
+    x.mul_(0.25)
+    w[3], w[5], w[7] = 0, 0, 0                                # so that x W + b stays finite
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y = spmm_cpp.linear(*leaves, 'gelu')
+    clean = torch.autograd.grad(y, leaves[1], dy, retain_graph=True)[0]
+    inf = float('inf')
+    with torch.no_grad():
+        leaves[0].data[10, 3], leaves[0].data[20, 5], leaves[0].data[30, 5], leaves[0].data[40, 7] = inf, inf, -inf, float('nan')
+    got = torch.autograd.grad(y, leaves[1], dy)[0]
+    pre = _d(x) @ _d(w) + _d(b)
+    p = _d(dy) * _act(pre, 'gelu')[1]
+    assert bool((p[[10, 20, 30]].abs() > 1e-3).any())
+    want = torch.zeros(k, n, dtype=torch.float64)
+    want[3] = inf * p[10]
+    want[5] = inf * p[20] - inf * p[30]
+    want[7] = float('nan')
+    for row in (3, 5, 7):
+        g = got[row].cpu()
+        assert torch.equal(torch.isnan(g), torch.isnan(want[row])) and torch.equal(g[torch.isinf(g)].double(), want[row][torch.isinf(want[row])])
+    rest = [i for i in range(k) if i not in (3, 5, 7)]
+    assert torch.equal(got[rest], clean[rest])
