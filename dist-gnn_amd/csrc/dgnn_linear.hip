@@ -226,6 +226,53 @@ bool small_fit(int64_t M, int64_t K, int64_t N) {
   return M > 0 && N > 0 && K > 0 && M <= kSmall && N <= kSmall && M * N <= (N <= 4 ? kSmall : kSmall / 2) && ceil_div(K, small_chunk(M, N)) <= 512;
 }
 
+// dx of few values (takes_few below): a workgroup takes up to 8 of a row, p in fp32 from dy and what was saved, once for all of
+// them. It is latency that it takes: bf16 gelu, with the slope's launch, 77 x 23 x 300 8.4 us, on tiles 13.5; 77 x 23 x 4000 11.9,
+// 12.7; 2 x 1024 x 4096 11.2, 10.2; 2048 x 1 x 64 10.5, 8.2; past the rule 16 x 128 x 16384 22.3, 12.7.
+constexpr int kFew = 8;
+
+template <typename T>
+__global__ __launch_bounds__(256) void few_inputs_kernel(const Small g) {
+  __shared__ float sums[4][kFew];
+  const int groups = (g.K + kFew - 1) / kFew, m = blockIdx.x / groups, k0 = blockIdx.x % groups * kFew, lane = threadIdx.x & 63;
+  const T* const dy = (const T*)g.dy + m * g.ldd;
+  const float* const pre = (const float*)g.save + m * g.lds;
+  const T* w[kFew];
+  float t[kFew];
+#pragma unroll
+  for (int i = 0; i < kFew; ++i) {
+    w[i] = (const T*)g.w + (k0 + i < g.K ? k0 + i : g.K - 1) * g.ldw;             // past the end the last one stands in
+    t[i] = 0.f;
+  }
+  for (int n0 = threadIdx.x; n0 < g.N; n0 += 512) {            // two columns of each operand in flight
+    T c[2][kFew], d[2];
+    float f[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int n = n0 + 256 * u < g.N ? n0 + 256 * u : n0;
+      d[u] = dy[n];
+      f[u] = pre[n];
+#pragma unroll
+      for (int i = 0; i < kFew; ++i) c[u][i] = w[i][n];
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (n0 + 256 * u >= g.N) break;
+      const float p = (float)d[u] * slope_of<T>(g.act, f[u]);
+#pragma unroll
+      for (int i = 0; i < kFew; ++i) t[i] = fmaf(p, (float)c[u][i], t[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kFew; ++i) {
+    for (int d = 1; d < 64; d <<= 1) t[i] += __shfl_xor(t[i], d);
+    if (lane == 0) sums[threadIdx.x >> 6][i] = t[i];
+  }
+  __syncthreads();
+  const int k = threadIdx.x;
+  if (k < kFew && k0 + k < g.K) ((T*)g.dx)[m * g.lddx + k0 + k] = (T)(sums[0][k] + sums[1][k] + sums[2][k] + sums[3][k]);
+}
+
 // ---------------------------------------------------------------------------------------
 constexpr int64_t kCompute = 256;              // compute units
 
@@ -500,11 +547,16 @@ int dgnn_linear_grad_weight(const void* x, int64_t ldx, const void* p, int64_t l
 // a column's sums share the errors of its p), and a product that is bound by its bytes has room for the second pieces. All
 // gradients of bf16 gelu with rounded p and with its pieces: 232965 x 256 x 41 135, 145 us; 232965 x 602 x 41 253, 242; 2449029 x
 // 128 x 47 717, 834; 2000000 x 4 x 4 633, 438. Few weights in many columns pay more once p leaves the caches (1000000 x 1 x 88 376,
-// 582), so they take the pieces up to 2^24 values of p only. The input gradient and wider weight gradients, whose error is 1.4
-// times that of their own rounding, take the rounded values.
+// 582), so they take the pieces up to 2^24 values of p only. Wider weight gradients and the input gradient, whose error is 1.4 times
+// that of their own rounding, take the rounded values.
 static bool takes_pieces(int64_t M, int64_t K, int64_t N, int32_t dtype, int32_t act) {
   if (dtype == DGNN_F32 || act <= ACT_RELU || M == 0 || K == 0 || N == 0 || small_fit(M, K, N)) return false;
   return N <= 64 ? K * N <= (1 << 20) : K * N <= 4096 && M * N <= (1 << 24);
+}
+
+// Nor do the roundings of p average in an input gradient of a few values, whose product is no work.
+static bool takes_few(int64_t M, int64_t K, int64_t N, int32_t dtype, int32_t act) {
+  return dtype != DGNN_F32 && act > ACT_RELU && M > 0 && K > 0 && N > 0 && M * K <= 2048 && M * K * N <= (1 << 24);
 }
 
 static Gemm weight_product(int64_t M, int64_t K, int64_t N, bool pieces) {
@@ -580,13 +632,19 @@ int dgnn_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
   char* rest = (char*)workspace + p_bytes;
   const void* p = dy;
   int64_t ldp = ldd;
-  if (act != ACT_NONE || dbias) {
-    void* to = act != ACT_NONE && M > 0 && N > 0 ? workspace : nullptr;
-    const int rc = slope(dy, ldd, save, lds, to, pitch, pieces ? N : 0, dbias, M, N, dtype, act, rest, need - p_bytes, stream);
+  const bool few = takes_few(M, K, N, dtype, act), p_wanted = act != ACT_NONE && M > 0 && N > 0 && (dw || (dx && !few));
+  if (p_wanted || dbias) {
+    const int rc = slope(dy, ldd, save, lds, p_wanted ? workspace : nullptr, pitch, pieces ? N : 0, dbias, M, N, dtype, act, rest, need - p_bytes, stream);
     if (rc != DGNN_OK) return rc;
-    if (act != ACT_NONE) { p = workspace; ldp = pitch; }
   }
-  if (dx) {
+  if (act != ACT_NONE) { p = workspace; ldp = pitch; }
+  if (dx && few) {
+    const Small g{x, w, dy, save, dx, dw, dbias, ldx, ldw, ldd, lds, lddx, lddw, (int)M, (int)K, (int)N, (int)act, 0};
+    const dim3 grid((uint32_t)(M * ceil_div(K, kFew)));
+    if (dtype == DGNN_BF16) hipLaunchKernelGGL((few_inputs_kernel<__bf16>), grid, dim3(256), 0, (hipStream_t)stream, g);
+    else hipLaunchKernelGGL((few_inputs_kernel<_Float16>), grid, dim3(256), 0, (hipStream_t)stream, g);
+    DGNN_LAUNCHED();
+  } else if (dx) {
     const int rc = dgnn_linear_grad_input(p, ldp, w, ldw, nullptr, 0, dx, lddx, M, K, N, dtype, rest, need - p_bytes, stream);
     if (rc != DGNN_OK) return rc;
   }

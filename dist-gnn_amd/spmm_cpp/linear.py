@@ -7,7 +7,7 @@ passes are there for layers with something in between (a GCN layer aggregates th
 Matrices are 2-D, rows unit-stride (any distance between rows), of one type: fp32, bf16 or fp16. fp32 results are as close
 to the exact sums as fp32 arithmetic is; with 16-bit types the gradient behind gelu or silu is rounded to the type before its
 products, as a 16-bit tensor between two operations would be (not in ``linear``'s weight gradients of narrow layers, up to 64
-columns, nor in its backward pass of small ones). The order of the sums depends on the sizes alone, so runs agree to the bit.
+columns, its input gradients of up to 2048 values and its backward pass of small layers). The order of the sums depends on the sizes alone, so runs agree to the bit.
 There is no second derivative, no forward-mode derivative and no torch.jit.trace: each is an error.
 Checks, outputs, workspaces and the autograd node are in csrc/dgnn_torch.cpp; errors are RuntimeError.
 """

@@ -33,7 +33,8 @@ extern "C" {
  *   dgnn_linear_grad_input    dx = p W^T + add    (add [M x K] or NULL: what else reaches x, a skip connection's gradient)
  *   dgnn_linear_grad_weight   dw = x^T p      (M = 0: zeros)
  *   dgnn_linear_backward      all of them in one call, p in the workspace (where 16-bit p of gelu or silu is rounded to its type, dw
- *                             of narrow layers takes what the rounding left as well, and small layers take p in fp32); dx, dw and dbias may be NULL (x, w and save are then
+ *                             of narrow layers takes what the rounding left as well, and dx of few values and small layers take
+ *                             p in fp32); dx, dw and dbias may be NULL (x, w and save are then
  *                             only needed for what is asked for). Its workspace: dgnn_linear_backward_workspace
  * workspace: device memory of dgnn_linear_workspace(pass, ...) bytes, 16-byte aligned (0 bytes: may be NULL), free to be used
  * again once the call's kernels have run. Sums over many rows are cut by a rule of the sizes alone and joined in a fixed

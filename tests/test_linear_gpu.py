@@ -663,3 +663,23 @@ def test_narrow_16_bit_weight_gradients_that_are_not_finite(dtype):
         assert torch.equal(torch.isnan(g), torch.isnan(want[row])) and torch.equal(g[torch.isinf(g)].double(), want[row][torch.isinf(want[row])])
     rest = [i for i in range(k) if i not in (3, 5, 7)]
     assert torch.equal(got[rest], clean[rest])
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+@pytest.mark.parametrize('m,k,n', [(9, 2, 1973), (1, 46, 4251), (45, 1, 47), (77, 23, 300), (1, 2048, 2100), (2048, 1, 3), (2, 1024, 1030), (2, 1025, 1030)])
+def test_input_gradients_of_few_values_round_once(m, k, n, dtype):
+    """dx of at most 2048 values carries its own rounding and what fp32 sums lose; beyond, the rounding of p too."""
+    for act, pad in (('gelu', 3), ('silu', 0)):
+        x, w, b, _, dy = case = _inputs(m, k, n, dtype, True, False, seed=61, pad=pad)
+        w.abs_()
+        got = _run(*case, act)
+        h, tiny = HALF[dtype], 2.0 ** -25 if dtype == 'f16' else 0
+        x, w, b, dy = map(_d, (x, w, b, dy))
+        pre, size = x @ w + b, x.abs() @ w.abs() + b.abs()
+        e_pre = _sum_bound(k, dtype) * size + U * pre.abs()
+        p = dy * _act(pre, act)[1]
+        e_p = dy.abs() * (0.8 * (U * pre.abs() + 2 * e_pre) + 32 * U * (1 + pre.abs()))
+        if m * k > 2048:
+            e_p = e_p + h * (p.abs() + e_p) + tiny
+        v, e = p @ w.t(), e_p @ w.abs().t()
+        _near(got['dx'], v, (e + _sum_bound(n, 'f32') * (p.abs() @ w.abs().t() + e)) * (1 + h) + h * v.abs() + 1e-40 + tiny, f'{act} dx')
