@@ -149,12 +149,9 @@ class AdamW(torch.optim.Optimizer):
         """Allocates the state of parameters that have none yet (zeros; a master takes its parameter's value)."""
         if self._current():
             return
-        if self._segments is None:
-            self._segments, self._known = [[] for _ in self.param_groups], []
-            given = {p: s for p, s in self.state.items() if s}
-        else:
-            given = {}
         self._check_params()
+        if self._segments is None:
+            self._segments, self._known = [], []
         for known, params in zip(self._known, [g['params'] for g in self.param_groups] + [()] * len(self._known)):
             if {id(p) for p in known} - {id(p) for p in params}:
                 raise RuntimeError('AdamW: a parameter was taken out of param_groups or replaced after its state was made; make a new '
@@ -168,11 +165,13 @@ class AdamW(torch.optim.Optimizer):
                     sorts.setdefault((p.device, p.dtype), []).append(p)
             for params in sorts.values():
                 seg = _Segment(params, self.state_bits, self.master_weights, self.capturable)
-                for i, p in enumerate(params):
-                    one = seg.views(i)
-                    if p in given:
-                        self._check(one, given[p])
-                        self._take(one, given[p])
+                made = [seg.views(i) for i in range(len(params))]
+                for one, p in zip(made, params):
+                    if self.state.get(p):                 # a copy's
+                        self._check(one, self.state[p])
+                for one, p in zip(made, params):
+                    if self.state.get(p):
+                        self._take(one, self.state[p])
                     elif seg.has_master:
                         one['master'].copy_(p.detach())
                     self.state[p] = one

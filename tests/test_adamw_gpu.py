@@ -573,3 +573,28 @@ def test_a_group_that_is_refused_is_not_there():
     a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
     opt.step()
     assert bool((a < 1).all()) and len(opt.param_groups) == 2 and int(opt.state[b]['step']) == 1
+
+
+def test_a_given_state_survives_a_refusal():
+    """A state that a copy brought along is still there after a first step that was refused for another parameter."""
+    a, b = _params((300, 20), torch.float32, 19)
+    first = spmm_cpp.AdamW([a, b], lr=LR)
+    _grads([a, b], 0)
+    first.step()
+    opt = spmm_cpp.AdamW([a, b], lr=LR)
+    for p in (a, b):
+        opt.state[p] = {n: x.clone() for n, x in first.state[p].items()}
+    group = opt.param_groups[0]
+    group['params'] = [a, b, torch.nn.Parameter(torch.ones(3))]
+    with pytest.raises(RuntimeError, match='no CPU path'):
+        opt.step()
+    group['params'] = [a, b]
+    opt.state[b]['exp_avg'] = opt.state[b]['exp_avg'][:-1]
+    with pytest.raises(ValueError, match='size'):
+        opt.step()
+    opt.state[b]['exp_avg'] = first.state[b]['exp_avg'].clone()
+    opt.step()
+    first.param_groups[0]['lr'] = 0.0
+    first.step()
+    for p in (a, b):
+        assert int(opt.state[p]['step']) == 2 and torch.equal(opt.state[p]['exp_avg'], first.state[p]['exp_avg'])
