@@ -8,7 +8,9 @@ Matrices are 2-D, rows unit-stride (any distance between rows), of one type: fp3
 to the exact sums as fp32 arithmetic is; with 16-bit types the gradient behind gelu or silu is rounded to the type before its
 products, as a 16-bit tensor between two operations would be (not in ``linear``'s weight gradients of narrow layers, up to 64
 columns, its input gradients of up to 2048 values and its backward pass of small layers). The order of the sums depends on the sizes alone, so runs agree to the bit.
-There is no second derivative, no forward-mode derivative and no torch.jit.trace: each is an error.
+There is no second derivative, no forward-mode derivative and no torch.jit.trace: each is an error. Calls can be captured in a
+graph; as with every torch operator, ``backward()`` of a captured call needs leaves that no live eager graph holds, whose accumulation
+belongs to the eager stream.
 Checks, outputs, workspaces and the autograd node are in csrc/dgnn_torch.cpp; errors are RuntimeError.
 """
 import torch

@@ -683,3 +683,9 @@ def test_input_gradients_of_few_values_round_once(m, k, n, dtype):
             e_p = e_p + h * (p.abs() + e_p) + tiny
         v, e = p @ w.t(), e_p @ w.abs().t()
         _near(got['dx'], v, (e + _sum_bound(n, 'f32') * (p.abs() @ w.abs().t() + e)) * (1 + h) + h * v.abs() + 1e-40 + tiny, f'{act} dx')
+
+
+@pytest.mark.parametrize('dtype,act,shape', [('bf16', 'gelu', (40, 30, 64)), ('f16', 'silu', (3000, 20, 41)), ('f32', 'gelu', (4230, 130, 70))])
+def test_captured_and_replayed_on_other_kernels(dtype, act, shape):
+    """Weight gradients from two pieces of p, input gradients of few values, rows straight from memory."""
+    test_captured_and_replayed(dtype, act, shape)
